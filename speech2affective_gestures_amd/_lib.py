@@ -83,6 +83,16 @@ class Tcn32(C.Structure):         # s2ag_tcn32_args
                 ('keep', vp), ('gy', vp), ('gx', vp), ('gp1', vp * 4), ('gp2', vp * 4)]
 
 
+class ClipTensor(C.Structure):    # s2ag_clip_tensor
+    _fields_ = [('src', vp), ('dst', vp), ('n', cll), ('src_bf16', ci), ('dst_bf16', ci)]
+
+
+class LceArgs(C.Structure):       # s2ag_lce_args
+    _fields_ = [('x', vp), ('w', vp), ('target', vp), ('target_i32', ci), ('bf16', ci), ('rows', cll), ('vocab', cll), ('ldx', cll),
+                ('ldw', cll), ('ignore_index', cll), ('dim', ci), ('reduction', ci), ('loss', vp), ('state', vp), ('grad_out', vp),
+                ('dx', vp), ('dw', vp), ('dw_accumulate', ci), ('workspace', vp), ('workspace_bytes', cll)]
+
+
 MAX_JOBS = 8
 MAX_WGRAD_JOBS = 4
 BF16_MAX_PACK = 32
@@ -239,6 +249,20 @@ SIGNATURES = {
     's2ag_normal_noise': [vp, cu, cll, vp, vp],
 }
 
+# include/s2ag_text.h
+TEXT_SIGNATURES = {
+    's2ag_clip_partials': [C.POINTER(ClipTensor), ci],
+    's2ag_clip_grads': [C.POINTER(ClipTensor), ci, cf, ci, vp, vp, vp],
+    's2ag_emb_lookup': [vp, ci, vp, ci, cll, ci, cll, cf, vp, vp],
+    's2ag_emb_grad_workspace_bytes': [cll, ci, cll],
+    's2ag_emb_grad': [vp, ci, vp, cll, ci, cll, ci, cll, cll, cf, vp, ci, vp, cll, vp],
+    's2ag_lce_state_bytes': [cll],
+    's2ag_lce_workspace_bytes': [C.POINTER(LceArgs), ci],
+    's2ag_lce_fwd': [C.POINTER(LceArgs), vp],
+    's2ag_lce_bwd': [C.POINTER(LceArgs), vp],
+}
+TEXT_SIZES = ('s2ag_clip_partials', 's2ag_emb_grad_workspace_bytes', 's2ag_lce_state_bytes', 's2ag_lce_workspace_bytes')
+
 _lib = None
 
 
@@ -258,7 +282,7 @@ def load():
             f'{path} not found: the S2AG HIP kernels are not built. Run '
             f'`python -m speech2affective_gestures_amd.build` (hipcc, gfx950). There is no CPU fallback.')
     lib = C.CDLL(path)
-    for name, args in SIGNATURES.items():
+    for name, args in {**SIGNATURES, **TEXT_SIGNATURES}.items():
         try:
             fn = getattr(lib, name)
         except AttributeError as e:
@@ -266,7 +290,7 @@ def load():
         fn.argtypes = args
         fn.restype = cll if name in ('s2ag_gru_coop_workspace_bytes', 's2ag_gru_coop_fwd_multi_workspace_bytes', 's2ag_bf16_tcn_pack_elems', 's2ag_bf16_tcn_sign_bytes', 's2ag_bf16_tcn_keep_bytes',
                               's2ag_bf16_conv_wgrad_scratch_floats', 's2ag_bf16_conv_wgrad_tr_scratch_floats',
-                              's2ag_f32_wgrad_tr_scratch_floats', 's2ag_f32_wgrad_tr_scratch_floats_n', 's2ag_tcn32_pack_elems', 's2ag_tcn32_keep_bytes') else ci
+                              's2ag_f32_wgrad_tr_scratch_floats', 's2ag_f32_wgrad_tr_scratch_floats_n', 's2ag_tcn32_pack_elems', 's2ag_tcn32_keep_bytes') + TEXT_SIZES else ci
     if lib.s2ag_abi_version() != ABI_VERSION:
         raise S2AGLibraryError(f'ABI version mismatch: _lib.py binds version {ABI_VERSION} of include/s2ag_hip.h, {path} is '
                                f'version {lib.s2ag_abi_version()}; rebuild it')

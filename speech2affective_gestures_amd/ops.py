@@ -2089,3 +2089,9 @@ class sequential_branches:
 
     def __exit__(self, *a):
         _NO_BRANCH_DEPTH[0] -= 1
+
+
+# ----------------------------------------------------------------------------------------------------
+# text-model operators (text.py, csrc/text/)
+# ----------------------------------------------------------------------------------------------------
+from .text import embedding_sorted, linear_cross_entropy  # noqa: E402,F401

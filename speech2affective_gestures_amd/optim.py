@@ -6,7 +6,8 @@ kernel launch per optimizer (s2ag_adam_step), and the data-parallel gradient exc
 all-reduce over the arena (parallel.py) instead of one collective per tensor.
 """
 import ctypes as C
-from typing import Iterable, List
+import math
+from typing import Iterable, List, Optional, Sequence, Union
 
 import torch
 
@@ -85,6 +86,10 @@ class FusedAdam:
                                    C.c_void_p(self.step_count.data_ptr()), float(grad_scale), s), 'adam_step')
         a.epoch += 1            # tensors derived from these parameters (ops._DerivedGroup) are stale now
 
+    def clip_grad_norm(self, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
+        """Clips the arena's gradients in place (``clip_grads``); call it between the backward pass and ``step``."""
+        return clip_grads([self.arena.grad], max_norm, norm_type)
+
     def state_dict(self):
         return dict(exp_avg=self.exp_avg, exp_avg_sq=self.exp_avg_sq, step=self.step_count, lr=self.param_groups[0]['lr'])
 
@@ -93,3 +98,95 @@ class FusedAdam:
         self.exp_avg_sq.copy_(sd['exp_avg_sq'])
         self.step_count.copy_(sd['step'])
         self.param_groups[0]['lr'] = sd['lr']
+
+
+_CLIP_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Whether the elements fill one piece of memory, in whatever order of the dimensions."""
+    if t.is_contiguous():
+        return True
+    need = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1):
+        if stride != need:
+            return False
+        need *= size
+    return True
+
+
+def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float = 2.0,
+               out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
+    """Scales gradients by ``min(1, max_norm / (norm + 1e-6))`` and returns their global norm, a 0-dim fp32 tensor on the device.
+
+    norm: the root of the sum of all squares (``norm_type`` 2, summed in 64 bits) or the largest magnitude (``math.inf``).  grads:
+    fp32 or bf16 tensors of one device, in any mix, each dense in memory (any order of dimensions); a tensor that is listed twice
+    counts once, two that share a part of their memory are refused.  out: where the results go, shaped and strided like grads, fp32
+    or bf16; None: in place (nothing is written where the factor is 1).  A norm that is not finite follows the formula: NaN
+    gradients for a NaN norm, zeros for an infinite one (and NaN for the infinities themselves).  Two launches per 128 tensors, no
+    synchronisation; can be captured into a graph."""
+    grads = list(grads)
+    inf = norm_type == math.inf
+    if not inf and norm_type != 2.0:
+        raise ValueError(f'clip_grads: norm_type must be 2 or inf, got {norm_type}')
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f'clip_grads: max_norm must not be negative, got {max_norm}')
+    if not grads:
+        raise ValueError('clip_grads: no gradients')
+    if out is not None:
+        out = list(out)
+        if len(out) != len(grads):
+            raise ValueError(f'clip_grads: {len(grads)} gradients and {len(out)} outputs')
+    dev = grads[0].device
+    table = (L.ClipTensor * len(grads))()
+    spans, seen, k = [], {}, 0
+    for i, g in enumerate(grads):
+        o = g if out is None else out[i]
+        for t in (g,) if o is g else (g, o):
+            if not t.is_cuda:
+                raise RuntimeError('clip_grads: got a CPU tensor; the S2AG ops run on MI355X only and there is no CPU fallback')
+            if t.device != dev:
+                raise ValueError(f'clip_grads: tensors on {dev} and {t.device}')
+            if t.dtype not in _CLIP_DTYPES:
+                raise TypeError(f'clip_grads: tensors must be float32 or bfloat16, got {t.dtype}')
+            if t.layout != torch.strided or not _dense(t):
+                raise ValueError(f'clip_grads: a tensor of shape {tuple(t.shape)} and strides {tuple(t.stride())} is not dense in memory')
+        if o is not g and (o.shape != g.shape or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()))):
+            raise ValueError(f'clip_grads: output {tuple(o.shape)} / {tuple(o.stride())} for a gradient {tuple(g.shape)} / {tuple(g.stride())}')
+        n = g.numel()
+        if n == 0:
+            continue
+        src, dst = g.data_ptr(), o.data_ptr()
+        key = (src, n, g.dtype)
+        if key in seen:
+            if seen[key] != dst:
+                raise ValueError('clip_grads: a gradient that is listed twice has two outputs')
+            continue
+        seen[key] = dst
+        q = table[k]
+        q.src, q.dst, q.n, q.src_bf16, q.dst_bf16 = src, dst, n, _CLIP_DTYPES[g.dtype], _CLIP_DTYPES[o.dtype]
+        spans.append((src, src + n * g.element_size()))
+        if dst != src:
+            spans.append((dst, dst + n * o.element_size()))
+        elif o.dtype != g.dtype:
+            raise ValueError('clip_grads: an output overlaps a gradient of another type')
+        k += 1
+    spans.sort()
+    for (_, end), (begin, _) in zip(spans, spans[1:]):
+        if begin < end:
+            raise ValueError('clip_grads: two of the tensors share memory')
+    lib = L.load()
+    with torch.cuda.device(dev):
+        partials = torch.empty(lib.s2ag_clip_partials(table, k), dtype=torch.float64, device=dev)
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        L.check(lib.s2ag_clip_grads(table, k, max_norm, int(inf), C.c_void_p(partials.data_ptr()), C.c_void_p(norm.data_ptr()),
+                                    C.c_void_p(torch.cuda.current_stream().cuda_stream)), 'clip_grads')
+    return norm
+
+
+def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
+    """``clip_grads`` in place over the ``.grad`` of the parameters that have one (torch.nn.utils.clip_grad_norm_'s call)."""
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    return clip_grads([p.grad for p in parameters if p.grad is not None], max_norm, norm_type)

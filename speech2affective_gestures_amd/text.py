@@ -1,0 +1,218 @@
+"""Operators of a text model's two ends: the word embedding with a gradient by sorted ids, and the softmax cross entropy of the
+output layer over a large vocabulary without its logits (kernels: csrc/text/, C ABI: include/s2ag_text.h).
+
+Public names: ``ops.embedding_sorted`` and ``ops.linear_cross_entropy``.  Both take fp32 or bf16, run on torch's current
+stream of their tensors' device, can be captured into a graph (kernels only, memory from the caching allocator), and give the same
+bits for the same inputs."""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional
+
+import torch
+
+from . import _lib as L
+
+Tensor = torch.Tensor
+_DTYPES = (torch.float32, torch.bfloat16)
+_IDS = (torch.int64, torch.int32)
+_REDUCTIONS = {'mean': 0, 'sum': 1, 'none': 2}
+MAX_ROWS = MAX_WORDS = 1 << 21         # linear_cross_entropy: rows of x, rows of weight
+
+
+def _p(t: Optional[Tensor]):
+    return None if t is None else C.c_void_p(t.data_ptr())
+
+
+def _stream():
+    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def _check_tensors(what: str, **ts) -> torch.device:
+    dev = None
+    for name, t in ts.items():
+        if not isinstance(t, Tensor):
+            raise TypeError(f'{what}: {name} must be a tensor, got {type(t).__name__}')
+        if not t.is_cuda:
+            raise RuntimeError(f'{what}: {name} is a CPU tensor; the S2AG ops run on MI355X only and there is no CPU fallback')
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f'{what}: tensors on {dev} and {t.device}')
+    return dev
+
+
+def _check_ids(what: str, name: str, t: Tensor) -> None:
+    if t.dtype not in _IDS:
+        raise TypeError(f'{what}: {name} must be int64 or int32, got {t.dtype}')
+
+
+def _check_matrix(what: str, name: str, t: Tensor) -> None:
+    if t.dtype not in _DTYPES:
+        raise TypeError(f'{what}: {name} must be float32 or bfloat16, got {t.dtype}')
+    if t.dim() != 2 or t.shape[0] == 0 or t.shape[1] == 0:
+        raise ValueError(f'{what}: {name} must be a matrix with rows and columns, got shape {tuple(t.shape)}')
+
+
+def _rows(t: Tensor):
+    """(tensor, row pitch): ``t`` as a matrix with unit column stride; a copy only if its rows do not lie at one pitch."""
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    if t.numel() and (t.stride(1) != 1 and t.shape[1] > 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
+        t = t.contiguous()
+    return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+
+
+def _arena_slot(p: Tensor) -> Optional[Tensor]:
+    """The gradient of a parameter that lives in an optim.ParamArena: the kernels add to it in place."""
+    from .ops import _grad_slot
+    return _grad_slot(p) if getattr(p, '_s2ag_arena', None) is not None else None
+
+
+# ----------------------------------------------------------------------------------------------------
+# embedding
+# ----------------------------------------------------------------------------------------------------
+class _EmbeddingSorted(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, table, scale, padding_idx):
+        with torch.cuda.device(table.device):
+            ids = ids.contiguous()
+            data = table.contiguous()
+            n, (entries, dim) = ids.numel(), data.shape
+            out = torch.empty(*ids.shape, dim, dtype=data.dtype, device=data.device)
+            L.check(L.load().s2ag_emb_lookup(_p(ids), int(ids.dtype == torch.int32), _p(data), int(data.dtype == torch.bfloat16), n, dim,
+                                             entries, scale, _p(out), _stream()), 'emb_lookup')
+        ctx.save_for_backward(ids)
+        ctx.table, ctx.scale, ctx.padding_idx = table, scale, padding_idx
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        (ids,) = ctx.saved_tensors
+        table = ctx.table
+        entries, dim = table.shape
+        n, lib = ids.numel(), L.load()
+        with torch.cuda.device(table.device):
+            dy, ld = _rows(dy)
+            slot = _arena_slot(table)
+            dt = torch.empty(entries, dim, dtype=table.dtype, device=table.device) if slot is None else slot
+            ws_bytes = lib.s2ag_emb_grad_workspace_bytes(n, dim, entries)
+            ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=table.device)
+            L.check(lib.s2ag_emb_grad(_p(ids), int(ids.dtype == torch.int32), _p(dy), ld, int(table.dtype == torch.bfloat16), n, dim, entries,
+                                      ctx.padding_idx, ctx.scale, _p(dt), int(slot is not None), _p(ws), ws.numel(), _stream()), 'emb_grad')
+        return None, (dt if slot is None else None), None, None
+
+
+def embedding_sorted(ids: Tensor, table: Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> Tensor:
+    """``scale * table[ids]`` in the table's type, rounded once: (*ids.shape, dim).
+
+    ids: int64 or int32, any shape; an id outside the table reads as a row of zeros and sends no gradient.  table: (n, dim) fp32 or
+    bf16.  padding_idx: a row that is looked up like any other and gets no gradient.
+    The table's gradient is summed per id in the order of the positions, in fp32, and rounded once.  Where the table is a parameter of
+    an optim.ParamArena, the backward pass adds to its gradient there, in the rows that were looked up, and hands autograd None."""
+    what = 'embedding_sorted'
+    _check_tensors(what, ids=ids, table=table)
+    _check_ids(what, 'ids', ids)
+    _check_matrix(what, 'table', table)
+    n, dim = table.shape
+    if ids.numel() >= (1 << 31) - 65536 or n >= (1 << 30) or dim > (1 << 24):
+        raise ValueError(f'{what}: {ids.numel()} ids in a table of shape {tuple(table.shape)} is more than the kernels index')
+    pad = -1
+    if padding_idx is not None:
+        pad = int(padding_idx) + (n if padding_idx < 0 else 0)
+        if not 0 <= pad < n:
+            raise ValueError(f'{what}: padding_idx {padding_idx} is not a row of a table of {n}')
+    return _EmbeddingSorted.apply(ids, table, float(scale), pad)
+
+
+# ----------------------------------------------------------------------------------------------------
+# linear + softmax cross entropy
+# ----------------------------------------------------------------------------------------------------
+def _lce_args(x, w, target, ldx, ldw, ignore_index, reduction, state) -> 'L.LceArgs':
+    a = L.LceArgs()
+    a.x, a.w, a.target, a.state = x.data_ptr(), w.data_ptr(), target.data_ptr(), state.data_ptr()
+    a.target_i32, a.bf16 = int(target.dtype == torch.int32), int(x.dtype == torch.bfloat16)
+    a.rows, a.dim, a.vocab, a.ldx, a.ldw = x.shape[0], x.shape[1], w.shape[0], ldx, ldw
+    a.ignore_index, a.reduction = ignore_index, reduction
+    return a
+
+
+def _lce_workspace(a, backward: bool, device) -> Tensor:
+    n = L.load().s2ag_lce_workspace_bytes(C.byref(a), int(backward))
+    if n < 0:
+        raise RuntimeError(f'linear_cross_entropy: sizes refused ({n})')
+    ws = torch.empty(max(n, 16), dtype=torch.uint8, device=device)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    return ws
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, target, ignore_index, reduction):
+        lib = L.load()
+        with torch.cuda.device(x.device):
+            xr, ldx = _rows(x)
+            w, ldw = _rows(weight)
+            t = target.contiguous().view(-1)
+            state = torch.empty(lib.s2ag_lce_state_bytes(xr.shape[0]) // 4, dtype=torch.int32, device=x.device)
+            loss = torch.empty(target.shape if reduction == 2 else (), dtype=torch.float32, device=x.device)
+            a = _lce_args(xr, w, t, ldx, ldw, ignore_index, reduction, state)
+            a.loss = loss.data_ptr() or state.data_ptr()          # (no rows, no reduction: nothing is written)
+            ws = _lce_workspace(a, False, x.device)
+            L.check(lib.s2ag_lce_fwd(C.byref(a), _stream()), 'lce_fwd')
+            del ws
+        ctx.save_for_backward(x, weight, t, state)
+        ctx.weight_leaf, ctx.meta = weight, (ignore_index, reduction)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        x, weight, t, state = ctx.saved_tensors
+        need_x, need_w = ctx.needs_input_grad[:2]
+        lib = L.load()
+        with torch.cuda.device(x.device):
+            slot = _arena_slot(ctx.weight_leaf) if need_w else None
+            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+            dw = None
+            if need_w:
+                dw = slot if slot is not None else torch.empty(weight.shape, dtype=weight.dtype, device=x.device)
+            xr, ldx = _rows(x)
+            w, ldw = _rows(weight)
+            if xr.shape[0] == 0:
+                if dw is not None and slot is None:
+                    dw.zero_()
+            else:
+                g = dloss.to(torch.float32).contiguous()
+                a = _lce_args(xr, w, t, ldx, ldw, *ctx.meta, state)
+                a.grad_out = g.data_ptr()
+                a.dx, a.dw, a.dw_accumulate = (None if dx is None else dx.data_ptr()), (None if dw is None else dw.data_ptr()), int(slot is not None)
+                ws = _lce_workspace(a, True, x.device)
+                L.check(lib.s2ag_lce_bwd(C.byref(a), _stream()), 'lce_bwd')
+                del ws
+        return dx, (dw if slot is None else None), None, None, None
+
+
+def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int = -100, reduction: str = 'mean') -> Tensor:
+    """Softmax cross entropy of the logits ``x @ weight.T`` against ``target``, in fp32; the logits are never stored.
+
+    x: (..., dim), weight: (vocab, dim), both fp32 or both bf16; target: (...) int64 or int32.  Rows whose target is
+    ``ignore_index`` have a loss and a gradient of zero and are left out of every product.  reduction: 'mean' over the other rows
+    (0 if there are none), 'sum', or 'none' (target's shape).  A target outside the vocabulary that is not ``ignore_index`` makes that
+    row's loss NaN, and every gradient that it enters.
+    At most 2^21 rows and 2^21 words.  Where the weight is a parameter of an optim.ParamArena, the backward pass adds to its gradient
+    there and hands autograd None."""
+    what = 'linear_cross_entropy'
+    _check_tensors(what, x=x, weight=weight, target=target)
+    _check_ids(what, 'target', target)
+    _check_matrix(what, 'weight', weight)
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"{what}: reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
+    if x.dtype != weight.dtype:
+        raise TypeError(f'{what}: x is {x.dtype} and weight {weight.dtype}')
+    if x.dim() < 1 or x.shape[-1] != weight.shape[1] or x.shape[:-1] != target.shape:
+        raise ValueError(f'{what}: x {tuple(x.shape)}, weight {tuple(weight.shape)} and target {tuple(target.shape)} do not go together')
+    if target.numel() > MAX_ROWS or weight.shape[0] > MAX_WORDS or weight.shape[1] > (1 << 20):
+        raise ValueError(f'{what}: at most {MAX_ROWS} rows, {MAX_WORDS} words and {1 << 20} columns')
+    return _LinearCrossEntropy.apply(x, weight, target, int(ignore_index), _REDUCTIONS[reduction])

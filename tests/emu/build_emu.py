@@ -47,14 +47,17 @@ def rewrite(text: str) -> str:
 
 
 def sources():
-    return sorted(glob.glob(os.path.join(CSRC, '*.hip')))
+    return sorted(glob.glob(os.path.join(CSRC, '*.hip'))) + sorted(glob.glob(os.path.join(CSRC, 'text', '*.hip')))
+
+
+def headers():
+    return sorted(glob.glob(os.path.join(CSRC, '*.h'))) + sorted(glob.glob(os.path.join(CSRC, 'text', '*.h')))
 
 
 def _digest():
     h = hashlib.sha256()
-    files = sources() + sorted(glob.glob(os.path.join(CSRC, '*.h'))) + [os.path.join(ROOT, 'include', 's2ag_hip.h'),
-                                                                       os.path.join(HERE, 'hip', 'hip_runtime.h'),
-                                                                       os.path.join(HERE, 'emu_rt.cpp'), os.path.abspath(__file__)]
+    files = sources() + headers() + sorted(glob.glob(os.path.join(ROOT, 'include', '*.h'))) + [
+        os.path.join(HERE, 'hip', 'hip_runtime.h'), os.path.join(HERE, 'emu_rt.cpp'), os.path.abspath(__file__)]
     for f in files:
         h.update(f.encode())
         h.update(open(f, 'rb').read())
@@ -67,19 +70,20 @@ def build(force: bool = False, verbose: bool = False) -> str:
     dig = _digest()
     if not force and os.path.exists(LIB) and os.path.exists(stamp) and open(stamp).read() == dig:
         return LIB
-    for h in glob.glob(os.path.join(CSRC, '*.h')):
-        open(os.path.join(OUT, 'src', os.path.basename(h)), 'w').write(rewrite(open(h).read()))
+    os.makedirs(os.path.join(OUT, 'src', 'text'), exist_ok=True)
+    for h in headers():
+        open(os.path.join(OUT, 'src', os.path.relpath(h, CSRC)), 'w').write(rewrite(open(h).read()))
     jobs = []
     for s in sources():
         base = os.path.basename(s)[:-4]
-        cpp = os.path.join(OUT, 'src', base + '.cpp')
+        cpp = os.path.join(OUT, 'src', os.path.relpath(s, CSRC)[:-4] + '.cpp')
         new = rewrite(open(s).read())
         if force or not os.path.exists(cpp) or open(cpp).read() != new:
             open(cpp, 'w').write(new)
         jobs.append((cpp, os.path.join(OUT, base + '.o')))
     jobs.append((os.path.join(HERE, 'emu_rt.cpp'), os.path.join(OUT, 'emu_rt.o')))
-    hdr_time = max(os.path.getmtime(f) for f in glob.glob(os.path.join(OUT, 'src', '*.h')) +
-                   [os.path.join(HERE, 'hip', 'hip_runtime.h'), os.path.join(ROOT, 'include', 's2ag_hip.h')])
+    hdr_time = max(os.path.getmtime(f) for f in glob.glob(os.path.join(OUT, 'src', '*.h')) + glob.glob(os.path.join(OUT, 'src', 'text', '*.h')) +
+                   glob.glob(os.path.join(ROOT, 'include', '*.h')) + [os.path.join(HERE, 'hip', 'hip_runtime.h')])
 
     def compile_one(job):
         src, obj = job

@@ -1,0 +1,539 @@
+"""Text-model operators (ops.embedding_sorted, ops.linear_cross_entropy, optim.clip_grads) against their definitions in 64 bits.
+
+Tolerances are bounds, element by element, from the roundings that the kernels make: u = 2^-24 for each fp32 operation, half an
+epsilon of the output's type (bf16 2^-8, fp32 2^-24) for each rounding to it."""
+import math
+import os
+import sys
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+sys.path.insert(0, os.path.join(os.path.dirname(__file__), 'golden'))
+
+EMU = os.environ.get('S2AG_EMU', '0') == '1'
+U = 2.0 ** -24
+DTYPES = {'fp32': torch.float32, 'bf16': torch.bfloat16}
+
+
+@pytest.fixture(scope='module')
+def S():
+    from speech2affective_gestures_amd import _lib, ops, optim
+    return dict(ops=ops, optim=optim, lib=_lib)
+
+
+def half_eps(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def within(got, ref, bound):
+    got, ref, bound = got.detach().cpu().double(), ref.double(), bound.double()
+    assert got.shape == ref.shape
+    assert torch.isfinite(got).all()
+    over = (got - ref).abs() - bound
+    worst = int(over.argmax()) if over.numel() else 0
+    assert over.numel() == 0 or float(over.max()) <= 0, (worst, got.reshape(-1)[worst], ref.reshape(-1)[worst], bound.reshape(-1)[worst])
+
+
+# ---- embedding --------------------------------------------------------------------------------------------------------------
+def embedding_reference(ids, table, dy, scale, padding_idx, dtype):
+    """(y, bound), (dtable, bound) on the CPU in 64 bits."""
+    n_entries, dim = table.shape
+    flat = ids.reshape(-1)
+    ok = (flat >= 0) & (flat < n_entries)
+    at = torch.where(ok, flat, torch.zeros_like(flat))
+    y = table.double()[at] * scale * ok[:, None]
+    h = half_eps(dtype)
+    y_bound = y.abs() * (U + h * (1 + U))                                   # one product, one rounding
+    if padding_idx is not None:
+        ok = ok & (flat != padding_idx)
+    g = dy.double().reshape(-1, dim) * ok[:, None]
+    dt = torch.zeros(n_entries, dim, dtype=torch.float64).index_add_(0, at, g)
+    s = torch.zeros(n_entries, dim, dtype=torch.float64).index_add_(0, at, g.abs()) * abs(scale)
+    m = torch.zeros(n_entries, dtype=torch.float64).index_add_(0, at, ok.double())[:, None]
+    dt *= scale
+    err = s * (m + 2) * U * 1.01                                            # m - 1 sums and a product, in any order
+    return (y.reshape(*ids.shape, dim), y_bound.reshape(*ids.shape, dim)), (dt, err + h * (dt.abs() + err))
+
+
+def ids_of(kind, n, entries, g):
+    ids = torch.randint(0, entries, (n,), generator=g)
+    if kind == 'padded':                       # transcripts: most positions hold one id
+        ids[torch.rand(n, generator=g) < 0.85] = 0
+    elif kind == 'one':
+        ids[:] = entries - 1
+    elif kind == 'runs':
+        ids = ids.sort().values
+    elif kind == 'outside':
+        ids[::3] = -1
+        ids[1::5] = entries
+    return ids
+
+
+# (positions, dim, rows of the table): around the lengths of a tile (16, 64), of the two sorts (8192; 4096), of a vector and a chunk of columns
+EMB_CASES = [(1, 1, 1), (1, 8, 3), (2, 300, 2), (15, 7, 40), (16, 64, 16), (17, 64, 16), (33, 257, 5), (64, 512, 700), (136, 300, 2000),
+             (1000, 36, 255), (1023, 5, 256), (1025, 5, 257), (4097, 12, 65537), (8192, 4, 90), (8193, 4, 511), (8193, 9, 140000), (12289, 16, 513)]
+
+
+@pytest.mark.parametrize('dtype', list(DTYPES))
+@pytest.mark.parametrize('kind', ['even', 'padded', 'one', 'outside'])
+@pytest.mark.parametrize('case', EMB_CASES)
+def test_embedding_sorted(S, case, kind, dtype):
+    n, dim, entries = case
+    dt = DTYPES[dtype]
+    g = torch.Generator().manual_seed(n * 7 + dim + entries)
+    ids = ids_of(kind, n, entries, g)
+    table, dy = torch.randn(entries, dim, generator=g).to(dt), torch.randn(n, dim, generator=g).to(dt)
+    scale = math.sqrt(dim)
+    (y, yb), (gr, gb) = embedding_reference(ids, table, dy, scale, None, dt)
+    t = table.cuda().requires_grad_(True)
+    out = S['ops'].embedding_sorted(ids.cuda(), t, scale=scale)
+    assert out.dtype == dt
+    within(out, y, yb)
+    out.backward(dy.cuda())
+    assert t.grad.dtype == dt
+    within(t.grad, gr, gb)
+    first = t.grad.clone()                      # the same bits again
+    t.grad = None
+    S['ops'].embedding_sorted(ids.cuda(), t, scale=scale).backward(dy.cuda())
+    assert torch.equal(first, t.grad)
+
+
+def test_embedding_sorted_padding_row_shapes_and_small_ids(S):
+    g = torch.Generator().manual_seed(3)
+    ids = ids_of('padded', 6 * 35, 50, g).view(6, 35)
+    table, dy = torch.randn(50, 24, generator=g), torch.randn(6, 35, 24, generator=g)
+    for pad in (0, -50, 7):
+        (y, yb), (gr, gb) = embedding_reference(ids, table, dy, 1.0, pad % 50, torch.float32)
+        t = table.cuda().requires_grad_(True)
+        out = S['ops'].embedding_sorted(ids.to(torch.int32).cuda(), t, padding_idx=pad)
+        within(out, y, yb)
+        out.backward(dy.cuda())
+        within(t.grad, gr, gb)
+        assert float(t.grad[pad % 50].abs().max()) == 0.0
+
+
+@pytest.mark.parametrize('dtype', list(DTYPES))
+def test_embedding_sorted_strides_and_offsets(S, dtype):
+    """ids and dy that are slices, transposed or broadcast; a table that does not begin at a multiple of 16 bytes."""
+    dt = DTYPES[dtype]
+    g = torch.Generator().manual_seed(5)
+    wide = torch.randint(0, 30, (9, 40), generator=g)
+    ids = wide[:, 3:37].t()
+    flat = torch.randn(30 * 16 + 1, generator=g).to(dt)
+    table = flat[1:].view(30, 16)
+    dy_wide = torch.randn(34, 9, 20, generator=g).to(dt)
+    for dy in (dy_wide[:, :, 2:18], dy_wide[:, :, 4:20], dy_wide[:, :1, :16].expand(34, 9, 16), dy_wide[:, :, :1].expand(34, 9, 16)):
+        (y, yb), (gr, gb) = embedding_reference(ids, table, dy, 2.0, None, dt)
+        t = flat.cuda()[1:].view(30, 16).requires_grad_(True)
+        base = dy_wide.cuda()
+        dyc = torch.as_strided(base, dy.shape, dy.stride(), dy.storage_offset())
+        out = S['ops'].embedding_sorted(wide.cuda()[:, 3:37].t(), t, scale=2.0)
+        within(out, y, yb)
+        (grad,) = torch.autograd.grad(out, t, dyc)
+        within(grad, gr, gb)
+
+
+def test_embedding_sorted_no_ids_and_rows_without_an_id(S):
+    t = torch.randn(40, 12, generator=torch.Generator().manual_seed(1)).cuda().requires_grad_(True)
+    out = S['ops'].embedding_sorted(torch.zeros(3, 0, dtype=torch.int64).cuda(), t)
+    assert out.shape == (3, 0, 12)
+    out.sum().backward()
+    assert float(t.grad.abs().max()) == 0.0
+    t.grad = None
+    out = S['ops'].embedding_sorted(torch.full((70,), -5).cuda(), t)
+    assert float(out.abs().max()) == 0.0
+    out.sum().backward()
+    assert float(t.grad.abs().max()) == 0.0
+
+
+def test_embedding_sorted_adds_to_the_arena(S):
+    """A table of a ParamArena: the backward pass adds to its gradient there; other rows and other parameters stay as they are."""
+    g = torch.Generator().manual_seed(9)
+    table, other = torch.randn(60, 20, generator=g), torch.randn(7, generator=g)
+    ids, dy = ids_of('padded', 90, 50, g), torch.randn(90, 20, generator=g)
+    a, b = torch.nn.Parameter(table.cuda()), torch.nn.Parameter(other.cuda())
+    arena = S['optim'].ParamArena([a, b])
+    start = torch.randn(arena.numel, generator=g)
+    arena.grad.copy_(start.cuda())
+    _, (gr, gb) = embedding_reference(ids, table, dy, 0.5, None, torch.float32)
+    S['ops'].embedding_sorted(ids.cuda(), a, scale=0.5).backward(dy.cuda())
+    before = start[:1200].view(60, 20).double()
+    within(a.grad, before + gr, gb + U * (before.abs() + gr.abs() + gb) * 1.01)
+    assert torch.equal(a.grad.cpu()[50:], start[:1200].view(60, 20)[50:])
+    assert torch.equal(arena.grad.cpu()[1200:], start[1200:])
+
+
+def test_embedding_sorted_refusals(S):
+    f = S['ops'].embedding_sorted
+    ids, table = torch.zeros(4, dtype=torch.int64).cuda(), torch.zeros(5, 6).cuda()
+    for a, kw, err in [((ids.float(), table), {}, TypeError), ((ids, table.double()), {}, TypeError), ((ids, table.half()), {}, TypeError),
+                       ((ids, table[0]), {}, ValueError), ((ids, table[:0]), {}, ValueError), ((ids, table[:, :0]), {}, ValueError),
+                       ((ids, table), dict(padding_idx=5), ValueError), ((ids, table), dict(padding_idx=-6), ValueError), ((None, table), {}, TypeError)]:
+        with pytest.raises(err):
+            f(*a, **kw)
+
+
+# ---- linear cross entropy ----------------------------------------------------------------------------------------------------
+IGNORE = -100
+
+
+def lce_reference(x, w, target, gout, reduction, ignore=IGNORE):
+    """(loss, bound), (dx, bound), (dw, bound) in 64 bits.  The bounds follow the kernels: a logit is a sum of `terms` fp32 terms;
+    an exponential of an argument of size s is off by s u + 4 u of itself (its argument's product with log2 e, its own rounding);
+    G is rounded to bf16 for bf16 operands, its and the other operand's pieces carry 2^-23 for fp32."""
+    dt = x.dtype
+    pieces = 6 if dt == torch.float32 else 1
+    x64, w64 = x.double(), w.double()
+    n, d = x.shape
+    z = x64 @ w64.t()
+    za = (x64.abs() @ w64.abs().t()).max() if n else torch.tensor(0.0)
+    dz = float(za) * ((d * pieces + 4) * U + (4 * U if pieces > 1 else 0))          # sums; pieces that are left out
+    keep = target != ignore
+    at = torch.where(keep, target, torch.zeros_like(target)).long()
+    lse = torch.logsumexp(z, 1)
+    spread = float(z.max() - z.min()) + dz if n else 0.0
+    de = (2 * spread + 16 + w.shape[0] ** 0.5) * U                                  # exponentials, their sum in steps, the joins
+    dl = 2 * dz + de + 4 * U * (float(lse.abs().max()) if n else 0.0)
+    loss = (lse - z[torch.arange(n), at]) * keep
+    loss_bound = (dl + 2 * U * (lse.abs() + loss.abs())) * keep
+    m = int(keep.sum())
+    f = {'mean': gout / max(m, 1), 'sum': gout, 'none': gout}[reduction]
+    f = f.double() * keep                                                            # (rows,)
+    p = torch.softmax(z, 1)
+    one = torch.zeros_like(p)
+    one[torch.arange(n), at] = 1.0
+    g = (p - one) * f[:, None]
+    ga = p * f.abs()[:, None] * (dl + de + dz) * 1.1 + g.abs() * 4 * U               # G in fp32
+    ga = ga + (g.abs() + ga) * (half_eps(torch.bfloat16) if pieces == 1 else 4 * U)  # as the products read it
+    h = half_eps(dt)
+
+    def product(a, da, b, terms):
+        r = a @ b
+        e = da @ b.abs() + (a.abs() + da) @ b.abs() * ((terms * pieces + 8) * U)
+        return r, e + h * (r.abs() + e)
+    dx, dxb = product(g, ga, w64, w.shape[0])
+    dw, dwb = product(g.t(), ga.t(), x64, n)
+    if reduction == 'none':
+        return (loss, loss_bound), (dx, dxb), (dw, dwb)
+    s, sb = loss.sum(), loss_bound.sum()
+    if reduction == 'mean':
+        s, sb = s / max(m, 1), sb / max(m, 1)
+    return (s, sb + 2 * U * s.abs()), (dx, dxb), (dw, dwb)
+
+
+def lce_case(n, d, v, dtype, ignored, seed=0):
+    g = torch.Generator().manual_seed(n * 31 + d * 7 + v + seed)
+    x, w = torch.randn(n, d, generator=g).to(DTYPES[dtype]), (torch.randn(v, d, generator=g) * 2 / math.sqrt(d)).to(DTYPES[dtype])
+    t = torch.randint(0, v, (n,), generator=g)
+    t[torch.rand(n, generator=g) < ignored] = IGNORE
+    return x, w, t, g
+
+
+def lce_check(S, x, w, t, g, reduction):
+    gout = torch.randn(t.shape if reduction == 'none' else (), generator=g)
+    (l, lb), (dx, dxb), (dw, dwb) = lce_reference(x, w, t, gout, reduction)
+    xg, wg, tg = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True), t.cuda()
+    loss = S['ops'].linear_cross_entropy(xg, wg, tg, reduction=reduction)
+    assert loss.dtype == torch.float32 and loss.shape == l.shape
+    within(loss, l, lb)
+    loss.backward(gout.cuda())
+    within(xg.grad, dx, dxb)
+    within(wg.grad, dw, dwb)
+    again = torch.autograd.grad(S['ops'].linear_cross_entropy(xg, wg, tg, reduction=reduction), (xg, wg), gout.cuda())
+    assert torch.equal(again[0], xg.grad) and torch.equal(again[1], wg.grad)
+
+
+# (rows, dim, words): one of each, around a stage of k (64), the tiles (128, 256), a transposed block, an odd pitch
+LCE_CASES = [(1, 1, 1), (1, 64, 2), (2, 8, 300), (3, 300, 129), (17, 65, 257), (64, 63, 1000), (127, 128, 128), (129, 130, 511), (257, 64, 513),
+             (300, 36, 2049), (136, 300, 1000)]
+
+
+@pytest.mark.parametrize('ignored', [0.0, 0.6])
+@pytest.mark.parametrize('dtype', list(DTYPES))
+@pytest.mark.parametrize('case', LCE_CASES)
+def test_linear_cross_entropy(S, case, dtype, ignored):
+    x, w, t, g = lce_case(*case, dtype, ignored)
+    lce_check(S, x, w, t, g, 'mean')
+
+
+@pytest.mark.parametrize('dtype', list(DTYPES))
+@pytest.mark.parametrize('reduction', ['sum', 'none'])
+def test_linear_cross_entropy_reductions(S, reduction, dtype):
+    x, w, t, g = lce_case(70, 96, 333, dtype, 0.3)
+    lce_check(S, x, w, t, g, reduction)
+
+
+@pytest.mark.skipif(EMU, reason='hundreds of large tiles: minutes on the device model')
+@pytest.mark.parametrize('dtype', list(DTYPES))
+@pytest.mark.parametrize('case', [(250, 64, 65536), (65530, 40, 300), (1100, 520, 50021)])
+def test_linear_cross_entropy_large_tiles(S, case, dtype):
+    x, w, t, g = lce_case(*case, dtype, 0.2)
+    lce_check(S, x, w, t, g, 'mean')
+
+
+@pytest.mark.skipif(EMU, reason='hundreds of large tiles: minutes on the device model')
+@pytest.mark.parametrize('dtype', list(DTYPES))
+def test_linear_cross_entropy_in_pieces_of_the_vocabulary(S, dtype):
+    """More rows times words than one piece holds."""
+    n, d, v = 20000, 8, 9001
+    x, w, t, g = lce_case(n, d, v, dtype, 0.1)
+    lce_check(S, x, w, t, g, 'mean')
+
+
+@pytest.mark.parametrize('dtype', list(DTYPES))
+def test_linear_cross_entropy_all_rows_ignored(S, dtype):
+    x, w, t, g = lce_case(40, 24, 77, dtype, 0.0)
+    t[:] = IGNORE
+    for reduction in ('mean', 'sum', 'none'):
+        xg, wg = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+        loss = S['ops'].linear_cross_entropy(xg, wg, t.cuda(), reduction=reduction)
+        assert float(loss.abs().max()) == 0.0
+        loss.sum().backward()
+        assert float(xg.grad.abs().max()) == 0.0 and float(wg.grad.abs().max()) == 0.0
+
+
+def test_linear_cross_entropy_no_rows(S):
+    x, w = torch.zeros(0, 24).cuda().requires_grad_(True), torch.randn(77, 24).cuda().requires_grad_(True)
+    for reduction in ('mean', 'sum', 'none'):
+        loss = S['ops'].linear_cross_entropy(x, w, torch.zeros(0, dtype=torch.int64).cuda(), reduction=reduction)
+        assert float(loss.sum()) == 0.0
+        w.grad = None
+        loss.sum().backward()
+        assert float(w.grad.abs().max()) == 0.0
+
+
+@pytest.mark.parametrize('dtype', list(DTYPES))
+def test_linear_cross_entropy_values_of_ignored_rows_do_not_matter(S, dtype):
+    """Infinities and NaN in rows that are ignored: the same bits as zeros there, and a gradient of zero."""
+    x, w, t, g = lce_case(50, 40, 200, dtype, 0.4)
+    res = []
+    for fill in (0.0, float('nan'), float('inf'), -torch.finfo(DTYPES[dtype]).max):
+        y = x.clone()
+        y[t == IGNORE] = fill
+        xg, wg = y.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+        loss = S['ops'].linear_cross_entropy(xg, wg, t.cuda())
+        loss.backward()
+        res.append((loss.detach().clone(), xg.grad, wg.grad))
+        assert float(xg.grad.cpu()[t == IGNORE].abs().max()) == 0.0
+    for r in res[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(res[0], r))
+
+
+def test_linear_cross_entropy_unknown_target_is_nan(S):
+    x, w, t, g = lce_case(20, 24, 50, 'fp32', 0.0)
+    for bad in (50, -1, 1 << 40):
+        t2 = t.clone()
+        t2[7] = bad
+        xg, wg = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+        loss = S['ops'].linear_cross_entropy(xg, wg, t2.cuda(), reduction='none')
+        ok = torch.arange(20) != 7
+        assert torch.isnan(loss[7]) and torch.isfinite(loss.detach().cpu()[ok]).all()
+        loss.sum().backward()
+        assert torch.isnan(xg.grad[7]).all() and torch.isfinite(xg.grad.cpu()[ok]).all() and torch.isnan(wg.grad).all()
+
+
+def test_linear_cross_entropy_large_logits(S):
+    """Logits of hundreds: the exponentials do not overflow, a certain target has a loss of 0, an impossible one its distance."""
+    w = torch.eye(8, 64)
+    x = torch.zeros(3, 64)
+    x[:, 2] = 600.0
+    t = torch.tensor([2, 5, IGNORE])
+    xg, wg = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    loss = S['ops'].linear_cross_entropy(xg, wg, t.cuda(), reduction='none')
+    assert loss.tolist() == [0.0, 600.0, 0.0]
+    loss.sum().backward()
+    want = torch.zeros(3, 64)
+    want[1, 2], want[1, 5] = 1.0, -1.0
+    assert torch.equal(xg.grad.cpu(), want)
+
+
+@pytest.mark.parametrize('dtype', list(DTYPES))
+def test_linear_cross_entropy_strides(S, dtype):
+    """x as a slice, transposed and broadcast; weight as a slice of columns and at an odd offset; targets int32 and strided."""
+    g = torch.Generator().manual_seed(17)
+    xb, wb = torch.randn(6, 30, 80, generator=g).to(DTYPES[dtype]), torch.randn(301, 80, generator=g).to(DTYPES[dtype])
+    t = torch.randint(0, 300, (30, 6), generator=g)
+    views = [(lambda b: b[:, :, 5:69].transpose(0, 1), lambda b: b[1:, 9:73]), (lambda b: b[:, :, 8:72].transpose(0, 1), lambda b: b[:300, 8:72]),
+             (lambda b: b[:1, :, :64].expand(6, 30, 64).transpose(0, 1), lambda b: b[:300, :1].expand(300, 64))]
+    for xv, wv in views:
+        x, w = xv(xb), wv(wb)
+        gout = torch.tensor(0.7)
+        (l, lb), (dx, dxb), (dw, dwb) = lce_reference(x.reshape(-1, 64), w, t.reshape(-1), gout, 'mean')
+        xg, wg = xv(xb.cuda()).detach().requires_grad_(True), wv(wb.cuda()).detach().requires_grad_(True)
+        loss = S['ops'].linear_cross_entropy(xg, wg, t.to(torch.int32).cuda())
+        within(loss, l, lb)
+        gx, gw = torch.autograd.grad(loss, (xg, wg), gout.cuda())
+        within(gx.reshape(-1, 64), dx, dxb)
+        within(gw, dw, dwb)
+
+
+def test_linear_cross_entropy_one_gradient_only(S):
+    x, w, t, g = lce_case(60, 48, 300, 'bf16', 0.2)
+    xg, wg = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    both = torch.autograd.grad(S['ops'].linear_cross_entropy(xg, wg, t.cuda()), (xg, wg))
+    (dx,) = torch.autograd.grad(S['ops'].linear_cross_entropy(xg, w.cuda(), t.cuda()), (xg,))
+    (dw,) = torch.autograd.grad(S['ops'].linear_cross_entropy(x.cuda(), wg, t.cuda()), (wg,))
+    assert torch.equal(dx, both[0]) and torch.equal(dw, both[1])
+
+
+def test_linear_cross_entropy_gradient_against_differences(S):
+    """The change of the loss along a direction: central differences of a loss in 64 bits at a step whose own errors are small."""
+    x, w, t, g = lce_case(12, 20, 40, 'fp32', 0.25)
+    xg, wg = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    gx, gw = torch.autograd.grad(S['ops'].linear_cross_entropy(xg, wg, t.cuda()), (xg, wg))
+    ux, uw = torch.randn(x.shape, generator=g).double(), torch.randn(w.shape, generator=g).double()
+
+    def loss(h):
+        return lce_reference((x.double() + h * ux), (w.double() + h * uw), t, torch.tensor(1.0), 'mean')[0][0]
+    h = 1e-5
+    slope = float((loss(h) - loss(-h)) / (2 * h))
+    got = float((gx.cpu().double() * ux).sum() + (gw.cpu().double() * uw).sum())
+    # differences: h^2 times a third derivative of order (|u| |x|)^3 ~ 1e3 -> 1e-7; gradients: fp32 sums, 1e-5 of them at most
+    assert abs(slope - got) < 1e-5 * (float((gx.cpu().double() * ux).abs().sum() + (gw.cpu().double() * uw).abs().sum())) + 1e-6
+
+
+def test_linear_cross_entropy_adds_to_the_arena(S):
+    x, w, t, g = lce_case(33, 20, 90, 'fp32', 0.3)
+    p = torch.nn.Parameter(w.cuda())
+    arena = S['optim'].ParamArena([p])
+    start = torch.randn(arena.numel, generator=g)
+    arena.grad.copy_(start.cuda())
+    _, _, (dw, dwb) = lce_reference(x, w, t, torch.tensor(1.0), 'mean')
+    S['ops'].linear_cross_entropy(x.cuda(), p, t.cuda()).backward()
+    before = start[:w.numel()].view(w.shape).double()
+    within(p.grad, before + dw, dwb + U * (before.abs() + dw.abs() + dwb) * 1.01)
+
+
+def test_linear_cross_entropy_refusals(S):
+    f = S['ops'].linear_cross_entropy
+    x, w, t = torch.zeros(4, 6).cuda(), torch.zeros(5, 6).cuda(), torch.zeros(4, dtype=torch.int64).cuda()
+    for a, kw, err in [((x.half(), w.half(), t), {}, TypeError), ((x, w.bfloat16(), t), {}, TypeError), ((x, w, t.float()), {}, TypeError),
+                       ((x, w[:, :5], t), {}, ValueError), ((x, w, t[:3]), {}, ValueError), ((x, w[:0], t), {}, ValueError),
+                       ((x, w, t), dict(reduction='median'), ValueError), ((x[0, 0], w, t), {}, ValueError), ((x, w, None), {}, TypeError)]:
+        with pytest.raises(err):
+            f(*a, **kw)
+
+
+# ---- gradient norm and clipping ------------------------------------------------------------------------------------------------
+def clip_reference(grads, max_norm, norm_type):
+    gs = [t.detach().cpu().double() for t in grads]
+    norm = math.sqrt(sum(float(t.square().sum()) for t in gs)) if norm_type == 2 else max([float(t.abs().max()) for t in gs if t.numel()], default=0.0)
+    return norm, min(1.0, max_norm / (norm + 1e-6)), gs
+
+
+def clip_check(S, grads, max_norm, norm_type=2.0, out=None):
+    norm, f, gs = clip_reference(grads, max_norm, norm_type)
+    got = S['optim'].clip_grads(grads, max_norm, norm_type, out=out)
+    assert got.dtype == torch.float32 and got.dim() == 0
+    assert abs(float(got) - norm) <= norm * 2 * U
+    for t, o in zip(gs, grads if out is None else out):
+        # the norm rounded, 1e-6 added, the quotient, the product: 4 u and what they compound to
+        within(o, t * f, (t * f).abs() * (6 * U + half_eps(o.dtype) * (1 + 6 * U)))
+
+
+SIZES = [[1], [7, 0, 3], [16384], [16385, 16383, 1], [5, 100000, 33, 2, 70001], [3] * 130, [2048] * 257]
+
+
+@pytest.mark.parametrize('norm_type', [2.0, math.inf])
+@pytest.mark.parametrize('dtype', ['fp32', 'bf16', 'mixed'])
+@pytest.mark.parametrize('sizes', SIZES, ids=lambda s: f'{len(s)}x{max(s)}')
+def test_clip_grads(S, sizes, dtype, norm_type):
+    g = torch.Generator().manual_seed(sum(sizes))
+    kinds = [DTYPES[dtype] if dtype != 'mixed' else (torch.float32, torch.bfloat16)[k % 2] for k in range(len(sizes))]
+    host = [torch.randn(n, generator=g).to(d) for n, d in zip(sizes, kinds)]
+    for max_norm in (0.25, 1e6):
+        clip_check(S, [t.cuda() for t in host], max_norm, norm_type)
+    grads = [t.cuda() for t in host]
+    out = [torch.full_like(t, 9.0, dtype=(torch.float32, torch.bfloat16)[(k // 2) % 2]) for k, t in enumerate(grads)]
+    clip_check(S, grads, 0.25, norm_type, out=out)
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(grads, host))         # inputs of an `out` call stay
+
+
+def test_clip_grads_offsets_and_orders(S):
+    """Tensors that begin at odd elements (two bytes off a vector), a transposed one, one of zero dimensions."""
+    g = torch.Generator().manual_seed(4)
+    base = torch.randn(40001, generator=g)
+    for dt in (torch.float32, torch.bfloat16):
+        b = base.to(dt).cuda()
+        grads = [b[1:20000], b[20003:20003 + 60 * 70].view(60, 70).t(), b[30000], b[30001:40001].view(100, 100)]
+        keep = b.clone()
+        clip_check(S, grads, 0.5)
+        for at in (0, 20000, 20001, 20002):
+            assert torch.equal(b[at], keep[at])
+
+
+def test_clip_grads_keeps_the_bits_where_nothing_is_clipped(S):
+    t = torch.randn(5000, generator=torch.Generator().manual_seed(2)).cuda()
+    before = t.clone()
+    S['optim'].clip_grads([t], 1e9)
+    assert torch.equal(t, before)
+    S['optim'].clip_grads([t], math.inf)
+    assert torch.equal(t, before)
+
+
+def test_clip_grads_values_out_of_the_ordinary(S):
+    """Squares beyond fp32's range either way; infinities and NaN as the formula has them."""
+    big = torch.full((1000,), 1e30).cuda()
+    n = S['optim'].clip_grads([big], 1.0)
+    assert abs(float(n) / (1e30 * math.sqrt(1000)) - 1) < 1e-6 and abs(float(big[0]) * math.sqrt(1000) - 1) < 1e-6
+    small = torch.full((1000,), 1e-30).cuda()
+    assert abs(float(S['optim'].clip_grads([small], 1.0)) / (1e-30 * math.sqrt(1000)) - 1) < 1e-6
+    for norm_type in (2.0, math.inf):
+        for at in (0, 16, 999):
+            x = torch.ones(1000)
+            x[at] = float('inf')
+            x = x.cuda()
+            assert float(S['optim'].clip_grads([x], 1.0, norm_type)) == math.inf
+            assert torch.isnan(x[at]) and float(x[(at + 1) % 1000]) == 0.0
+            x = torch.ones(1000)
+            x[at] = float('nan')
+            x = x.cuda()
+            assert math.isnan(float(S['optim'].clip_grads([x], 1.0, norm_type)))
+            assert torch.isnan(x).all()
+    z = torch.zeros(30).cuda()
+    assert float(S['optim'].clip_grads([z], 1.0)) == 0.0 and float(z.abs().max()) == 0.0
+    assert float(S['optim'].clip_grads([torch.zeros(0).cuda()], 1.0)) == 0.0
+
+
+def test_clip_grads_same_tensor_twice_counts_once(S):
+    t = torch.randn(3000, generator=torch.Generator().manual_seed(8))
+    a = t.cuda()
+    n = S['optim'].clip_grads([a, a], 0.5)
+    b = t.cuda()
+    assert float(n) == float(S['optim'].clip_grads([b], 0.5)) and torch.equal(a, b)
+
+
+def test_clip_grad_norm_over_parameters_and_arena(S):
+    g = torch.Generator().manual_seed(6)
+    ps = [torch.nn.Parameter(torch.zeros(*s).cuda()) for s in ((30, 7), (11,), (5, 5))]
+    gr = [torch.randn(p.shape, generator=g) for p in ps]
+    ps[0].grad, ps[2].grad = gr[0].cuda(), gr[2].cuda()
+    norm, f, _ = clip_reference([gr[0], gr[2]], 0.1, 2)
+    n = S['optim'].clip_grad_norm_(ps, 0.1)
+    assert abs(float(n) - norm) <= 2 * U * norm
+    for p, t in ((ps[0], gr[0]), (ps[2], gr[2])):
+        within(p.grad, t.double() * f, t.double().abs() * f * 8 * U)
+    arena = S['optim'].ParamArena(ps)
+    adam = S['optim'].FusedAdam(arena, 1e-3)
+    for p, t in zip(ps, gr):
+        p.grad.copy_(t.cuda())
+    norm, f, _ = clip_reference(gr, 0.1, 2)
+    n = adam.clip_grad_norm(0.1)
+    assert abs(float(n) - norm) <= 2 * U * norm
+    for p, t in zip(ps, gr):
+        within(p.grad, t.double() * f, t.double().abs() * f * 8 * U)
+
+
+def test_clip_grads_refusals(S):
+    f = S['optim'].clip_grads
+    t = torch.zeros(10, 10).cuda()
+    for a, kw, err in [(([], 1.0), {}, ValueError), (([t], -1.0), {}, ValueError), (([t], float('nan')), {}, ValueError), (([t], 1.0, 1.0), {}, ValueError),
+                       (([t.half()], 1.0), {}, TypeError), (([t[:, :5]], 1.0), {}, ValueError), (([t[0].expand(4, 10)], 1.0), {}, ValueError),
+                       (([t, t[2:4]], 1.0), {}, ValueError), (([t], 1.0), dict(out=[]), ValueError), (([t], 1.0), dict(out=[t[:5]]), ValueError),
+                       (([t], 1.0), dict(out=[torch.zeros(10, 10).cuda().t()]), ValueError),
+                       (([t[:5], t[5:]], 1.0), dict(out=[t[5:], t[:5]]), ValueError)]:
+        with pytest.raises(err):
+            f(*a, **kw)
