@@ -169,8 +169,9 @@ struct Product {
     const float* scale;                 // STORE: the factor of all rows
 };
 
-// pairs of pieces, the smallest products first
-__device__ constexpr unsigned char PAIR_R[6] = {0, 1, 2, 0, 1, 0}, PAIR_Q[6] = {2, 1, 0, 1, 0, 0};
+// pairs of pieces, the smallest products first: (0, 2) (1, 1) (2, 0) (0, 1) (1, 0) (0, 0), two bits each
+__device__ __forceinline__ int piece_r(int pair) { return (0x124 >> (2 * pair)) & 3; }
+__device__ __forceinline__ int piece_q(int pair) { return (0x046 >> (2 * pair)) & 3; }
 
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 #define S2AG_LDS_PTR(type, p) ((__attribute__((address_space(3))) type*)(p))
@@ -178,6 +179,11 @@ typedef short s16x4_t __attribute__((ext_vector_type(4)));
 // 16-byte slot of (row, slot) in a stage: the slots of a row are permuted by the row's low bits, so that the 16 rows that a
 // wavefront reads at one slot lie in different banks.
 __device__ __forceinline__ int slot_at(int row, int slot) { return row * BK + ((slot ^ (row & 7)) << 3); }
+
+// 16 bytes a lane from the buffer to LDS: lane l's land at dst + 16 l
+__device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t from, bf16_t* dst, unsigned lane_offset, int offset) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, S2AG_LDS_PTR(void, dst), 16, lane_offset, offset, 0, 0);
+}
 
 template <int BR, int BQ, int WR, int WQ, End END>
 __global__ __launch_bounds__(64 * WR * WQ) void product_k(Product p) {
@@ -197,40 +203,55 @@ __global__ __launch_bounds__(64 * WR * WQ) void product_k(Product p) {
         const int n = gridDim.x, x = blockIdx.x & 7, q8 = n >> 3, r8 = n & 7;
         v = (x < r8 ? x * (q8 + 1) : r8 * (q8 + 1) + (x - r8) * q8) + (blockIdx.x >> 3);
     }
-    const int split = v % p.splits;
-    v /= p.splits;
+    // (whole-number division runs on the vector units: the results are told to be one for the wavefront, so that the operands'
+    // descriptors stay in scalar registers)
+    const int split = __builtin_amdgcn_readfirstlane(v % p.splits);
+    v = __builtin_amdgcn_readfirstlane(v / p.splits);
     constexpr int GROUP = 8;
     const int per = GROUP * p.tiles_q, grp = v / per, first = grp * GROUP;
     const int gsz = min(p.tiles_r - first, GROUP);
-    const int tr = first + (v - grp * per) % gsz, tq = (v - grp * per) / gsz;
+    const int tr = __builtin_amdgcn_readfirstlane(first + (v - grp * per) % gsz), tq = __builtin_amdgcn_readfirstlane((v - grp * per) / gsz);
     const long long r0 = (long long)tr * BR, c0 = (long long)tq * BQ;
-    const long long live = p.r_count ? (long long)*p.r_count : p.r_rows;
+    const long long live = p.r_count ? (long long)__builtin_amdgcn_readfirstlane(*p.r_count) : p.r_rows;
     if (r0 >= live) return;
 
-    const int k = p.k_count ? (*p.k_count + BK - 1) / BK * BK : p.k;
-    const int kt = k / BK, total = kt * p.pairs;
-    const int it0 = (int)((long long)total * split / p.splits), it1 = (int)((long long)total * (split + 1) / p.splits);
+    const int kt = p.k_count ? __builtin_amdgcn_readfirstlane((*p.k_count + BK - 1) / BK) : p.k / BK, total = kt * p.pairs;
+    const int it0 = __builtin_amdgcn_readfirstlane((int)((long long)total * split / p.splits));
+    const int it1 = __builtin_amdgcn_readfirstlane((int)((long long)total * (split + 1) / p.splits));
 
     const long long r_left = p.r_rows - r0, q_left = p.q_rows > c0 ? p.q_rows - c0 : 0;      // (a tile may lie behind the words)
     const int r_bytes = (int)((r_left < BR ? r_left : BR) * p.r.ld * 2), q_bytes = (int)((q_left < BQ ? q_left : BQ) * p.q.ld * 2);
     const int ld_row = tid >> 3, ld_slot = (tid & 7) ^ (ld_row & 7);
-    const unsigned r_off = (unsigned)(ld_row * p.r.ld * 2 + ld_slot * 16), q_off = (unsigned)(ld_row * p.q.ld * 2 + ld_slot * 16);
-    const unsigned r_step = (unsigned)(NT / 8 * p.r.ld * 2), q_step = (unsigned)(NT / 8 * p.q.ld * 2);
+    unsigned r_off[LR], q_off[LQ];
+#pragma unroll
+    for (int i = 0; i < LR; ++i) r_off[i] = (unsigned)((ld_row + i * (NT / 8)) * p.r.ld * 2 + ld_slot * 16);
+#pragma unroll
+    for (int i = 0; i < LQ; ++i) q_off[i] = (unsigned)((ld_row + i * (NT / 8)) * p.q.ld * 2 + ld_slot * 16);
 
-    auto issue = [&](int it, int buf) {
-        const int pair = it / kt, kk = (it - pair * kt) * BK;
-        const bf16_t* rb = p.r.p + PAIR_R[p.pairs == 1 ? 5 : pair] * p.r.plane + r0 * p.r.ld;
-        const bf16_t* qb = p.q.p + PAIR_Q[p.pairs == 1 ? 5 : pair] * p.q.plane + c0 * p.q.ld;
+    // the stage that is loaded next: its pair of pieces, its place along k
+    int pair = __builtin_amdgcn_readfirstlane(it0 / (kt > 0 ? kt : 1)), kk = it0 - pair * kt;
+    const bf16_t *rb, *qb;
+    auto bases = [&]() {
+        rb = p.r.p + piece_r(p.pairs == 1 ? 5 : pair) * p.r.plane + r0 * p.r.ld;
+        qb = p.q.p + piece_q(p.pairs == 1 ? 5 : pair) * p.q.plane + c0 * p.q.ld;
+    };
+    bases();
+    auto issue = [&](int buf) {
         __amdgpu_buffer_rsrc_t rr = __builtin_amdgcn_make_buffer_rsrc((void*)rb, 0, r_bytes, 0x00020000);
         __amdgpu_buffer_rsrc_t qr = __builtin_amdgcn_make_buffer_rsrc((void*)qb, 0, q_bytes, 0x00020000);
         bf16_t* s = lds + buf * STAGE + wave * 512;
+        const int off = kk * (BK * 2);
 #pragma unroll
         for (int i = 0; i < LR; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rr, S2AG_LDS_PTR(void, s + i * NT * 8), 16, r_off + i * r_step, kk * 2, 0, 0);
+            to_lds(rr, s + i * NT * 8, r_off[i], off);
         s += BR * BK;
 #pragma unroll
         for (int i = 0; i < LQ; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(qr, S2AG_LDS_PTR(void, s + i * NT * 8), 16, q_off + i * q_step, kk * 2, 0, 0);
+            to_lds(qr, s + i * NT * 8, q_off[i], off);
+        if (++kk == kt) {
+            kk = 0;
+            if (++pair < p.pairs) bases();
+        }
     };
 
     f32x4 acc[QI][RI];
@@ -240,29 +261,50 @@ __global__ __launch_bounds__(64 * WR * WQ) void product_k(Product p) {
         for (int j = 0; j < RI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     const int fl = lane & 15, fk = lane >> 4;
-    if (it0 < it1) issue(it0, 0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    for (int it = it0; it < it1; ++it) {
-        const int buf = (it - it0) & 1;
-        if (it + 1 < it1) issue(it + 1, buf ^ 1);
-        const bf16_t* rs = lds + buf * STAGE + wr * TR * BK;
-        const bf16_t* qs = lds + buf * STAGE + BR * BK + wq * TQ * BK;
+    const bf16_t* const rs = lds + wr * TR * BK;
+    const bf16_t* const qs = lds + BR * BK + wq * TQ * BK;
+    auto fragments = [&](bf16x8 (&a)[QI], bf16x8 (&b)[RI], int buf, int ks) {
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            bf16x8 a[QI], b[RI];
+        for (int i = 0; i < QI; ++i) a[i] = *reinterpret_cast<const bf16x8*>(qs + buf * STAGE + slot_at(i * 16 + fl, ks * 4 + fk));
 #pragma unroll
-            for (int i = 0; i < QI; ++i) a[i] = *reinterpret_cast<const bf16x8*>(qs + slot_at(i * 16 + fl, ks * 4 + fk));
+        for (int j = 0; j < RI; ++j) b[j] = *reinterpret_cast<const bf16x8*>(rs + buf * STAGE + slot_at(j * 16 + fl, ks * 4 + fk));
+    };
+    auto multiply = [&](const bf16x8 (&a)[QI], const bf16x8 (&b)[RI]) {
 #pragma unroll
-            for (int j = 0; j < RI; ++j) b[j] = *reinterpret_cast<const bf16x8*>(rs + slot_at(j * 16 + fl, ks * 4 + fk));
+        for (int i = 0; i < QI; ++i)
 #pragma unroll
-            for (int i = 0; i < QI; ++i)
-#pragma unroll
-                for (int j = 0; j < RI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], acc[i][j], 0, 0, 0);
-        }
+            for (int j = 0; j < RI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], acc[i][j], 0, 0, 0);
+    };
+
+    // Two stages in LDS, two halves of a stage in registers.  While the first half of a stage is multiplied its second half is
+    // read; then every wavefront is done with the stage's LDS, the next stage (requested a whole stage ago) has landed, and while
+    // the second half is multiplied the first half of the next stage is read and the stage after it is requested.
+    const int stages = it1 - it0;
+    bf16x8 a0[QI], b0[RI], a1[QI], b1[RI];
+    if (stages > 0) {
+        issue(0);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
+        if (stages > 1) issue(1);
+        fragments(a0, b0, 0, 0);
     }
+    for (int n = 0; n < stages; ++n) {
+        const int buf = n & 1;
+        fragments(a1, b1, buf, 1);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(a0, b0);
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // (keeps the reads behind the barrier)
+        if (n + 2 < stages) issue(buf);
+        if (n + 1 < stages) fragments(a0, b0, buf ^ 1, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(a1, b1);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    __syncthreads();
 
     // element e of acc[i][j]: column i * 16 + fk * 4 + e, row j * 16 + fl of the wavefront's part
     const long long wr0 = r0 + wr * TR, wc0 = c0 + wq * TQ;
