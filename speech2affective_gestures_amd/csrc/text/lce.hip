@@ -185,8 +185,16 @@ __device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t from, bf16_t* dst,
     __builtin_amdgcn_raw_ptr_buffer_load_lds(from, S2AG_LDS_PTR(void, dst), 16, lane_offset, offset, 0, 0);
 }
 
+// Matrix instruction with its accumulator in the accumulation registers, where the compiler, left to itself, moves a set that
+// fills all 256 of them to and fro.  The compiler knows no matrix instruction here: `settle` stands between the last of them
+// and the first use of a result, and between the zeros and the first of them.
+__device__ __forceinline__ void mfma_acc(f32x4& c, bf16x8 a, bf16x8 b) {
+    asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
+
 template <int BR, int BQ, int WR, int WQ, End END>
-__global__ __launch_bounds__(64 * WR * WQ) void product_k(Product p) {
+__global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
     constexpr int NT = 64 * WR * WQ;
     constexpr int TR = BR / WR, TQ = BQ / WQ, RI = TR / 16, QI = TQ / 16;      // a wavefront's part
     constexpr int LR = BR * 8 / NT, LQ = BQ * 8 / NT;                          // 16-byte loads per thread and stage
@@ -228,30 +236,34 @@ __global__ __launch_bounds__(64 * WR * WQ) void product_k(Product p) {
 #pragma unroll
     for (int i = 0; i < LQ; ++i) q_off[i] = (unsigned)((ld_row + i * (NT / 8)) * p.q.ld * 2 + ld_slot * 16);
 
-    // the stage that is loaded next: its pair of pieces, its place along k
-    int pair = __builtin_amdgcn_readfirstlane(it0 / (kt > 0 ? kt : 1)), kk = it0 - pair * kt;
-    const bf16_t *rb, *qb;
-    auto bases = [&]() {
-        rb = p.r.p + piece_r(p.pairs == 1 ? 5 : pair) * p.r.plane + r0 * p.r.ld;
-        qb = p.q.p + piece_q(p.pairs == 1 ? 5 : pair) * p.q.plane + c0 * p.q.ld;
+    // the stage that is requested next: its pair of pieces, its place along k; behind the last one the descriptors are empty, so
+    // that the loop has no branch
+    int pair = __builtin_amdgcn_readfirstlane(it0 / (kt > 0 ? kt : 1)), kk = it0 - pair * kt, left = it1 - it0;
+    __amdgpu_buffer_rsrc_t rr, qr;
+    auto descriptors = [&]() {
+        const bf16_t* rb = p.r.p + piece_r(p.pairs == 1 ? 5 : pair) * p.r.plane + r0 * p.r.ld;
+        const bf16_t* qb = p.q.p + piece_q(p.pairs == 1 ? 5 : pair) * p.q.plane + c0 * p.q.ld;
+        rr = __builtin_amdgcn_make_buffer_rsrc((void*)rb, 0, left > 0 ? r_bytes : 0, 0x00020000);
+        qr = __builtin_amdgcn_make_buffer_rsrc((void*)qb, 0, left > 0 ? q_bytes : 0, 0x00020000);
     };
-    bases();
-    auto issue = [&](int buf) {
-        __amdgpu_buffer_rsrc_t rr = __builtin_amdgcn_make_buffer_rsrc((void*)rb, 0, r_bytes, 0x00020000);
-        __amdgpu_buffer_rsrc_t qr = __builtin_amdgcn_make_buffer_rsrc((void*)qb, 0, q_bytes, 0x00020000);
+    descriptors();
+    // requests [from, from + n) of the LR + LQ of a stage
+    auto issue = [&](int buf, int from, int n) {
         bf16_t* s = lds + buf * STAGE + wave * 512;
         const int off = kk * (BK * 2);
 #pragma unroll
-        for (int i = 0; i < LR; ++i)
-            to_lds(rr, s + i * NT * 8, r_off[i], off);
-        s += BR * BK;
-#pragma unroll
-        for (int i = 0; i < LQ; ++i)
-            to_lds(qr, s + i * NT * 8, q_off[i], off);
+        for (int i = from; i < from + n; ++i) {
+            if (i < LR) to_lds(rr, s + i * NT * 8, r_off[i < LR ? i : 0], off);
+            else to_lds(qr, s + BR * BK + (i - LR) * NT * 8, q_off[i < LR ? 0 : i - LR], off);
+        }
+    };
+    auto advance = [&]() {
+        --left;
         if (++kk == kt) {
             kk = 0;
-            if (++pair < p.pairs) bases();
+            pair = pair + 1 < p.pairs ? pair + 1 : pair;
         }
+        descriptors();
     };
 
     f32x4 acc[QI][RI];
@@ -263,47 +275,62 @@ __global__ __launch_bounds__(64 * WR * WQ) void product_k(Product p) {
     const int fl = lane & 15, fk = lane >> 4;
     const bf16_t* const rs = lds + wr * TR * BK;
     const bf16_t* const qs = lds + BR * BK + wq * TQ * BK;
-    auto fragments = [&](bf16x8 (&a)[QI], bf16x8 (&b)[RI], int buf, int ks) {
-#pragma unroll
-        for (int i = 0; i < QI; ++i) a[i] = *reinterpret_cast<const bf16x8*>(qs + buf * STAGE + slot_at(i * 16 + fl, ks * 4 + fk));
-#pragma unroll
-        for (int j = 0; j < RI; ++j) b[j] = *reinterpret_cast<const bf16x8*>(rs + buf * STAGE + slot_at(j * 16 + fl, ks * 4 + fk));
+    // fragment [u] of half ks of a stage: the QI of Q, then the RI of R
+    auto fragment = [&](bf16x8 (&a)[QI], bf16x8 (&b)[RI], int buf, int ks, int u) {
+        if (u < QI) a[u < QI ? u : 0] = *reinterpret_cast<const bf16x8*>(qs + buf * STAGE + slot_at(u * 16 + fl, ks * 4 + fk));
+        else b[u < QI ? 0 : u - QI] = *reinterpret_cast<const bf16x8*>(rs + buf * STAGE + slot_at((u - QI) * 16 + fl, ks * 4 + fk));
     };
-    auto multiply = [&](const bf16x8 (&a)[QI], const bf16x8 (&b)[RI]) {
+    auto multiply = [&](const bf16x8 (&a)[QI], const bf16x8 (&b)[RI], int i) {
 #pragma unroll
-        for (int i = 0; i < QI; ++i)
-#pragma unroll
-            for (int j = 0; j < RI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < RI; ++j) {
+            if constexpr (RI * QI * 4 == 256) mfma_acc(acc[i][j], a[i], b[j]);
+            else acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], acc[i][j], 0, 0, 0);
+        }
     };
 
     // Two stages in LDS, two halves of a stage in registers.  While the first half of a stage is multiplied its second half is
     // read; then every wavefront is done with the stage's LDS, the next stage (requested a whole stage ago) has landed, and while
-    // the second half is multiplied the first half of the next stage is read and the stage after it is requested.
+    // the second half is multiplied the first half of the next stage is read and the stage after it is requested.  Reads and
+    // requests go behind rows of matrix instructions, the reads behind the first ones, so that they run beside the others.
+    constexpr int PER = (QI + RI + QI / 2 - 1) / (QI / 2), LPER = (LR + LQ + QI - 1) / QI;
     const int stages = it1 - it0;
     bf16x8 a0[QI], b0[RI], a1[QI], b1[RI];
-    if (stages > 0) {
-        issue(0);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (stages > 1) issue(1);
-        fragments(a0, b0, 0, 0);
-    }
+    issue(0, 0, LR + LQ);
+    advance();
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    issue(1, 0, LR + LQ);
+    advance();
+#pragma unroll
+    for (int u = 0; u < QI + RI; ++u) fragment(a0, b0, 0, 0, u);
+    settle();
     for (int n = 0; n < stages; ++n) {
         const int buf = n & 1;
-        fragments(a1, b1, buf, 1);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(a0, b0);
-        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < QI; ++i) {
+            multiply(a0, b0, i);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int u = i * PER; u < (i + 1) * PER && u < QI + RI; ++u) fragment(a1, b1, buf, 1, u);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // (keeps the reads behind the barrier)
-        if (n + 2 < stages) issue(buf);
-        if (n + 1 < stages) fragments(a0, b0, buf ^ 1, 0);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(a1, b1);
-        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < QI; ++i) {
+            multiply(a1, b1, i);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int u = i * PER; u < (i + 1) * PER && u < QI + RI; ++u) fragment(a0, b0, buf ^ 1, 0, u);
+            issue(buf, i * LPER, (i + 1) * LPER < LR + LQ ? LPER : LR + LQ - i * LPER);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        advance();
     }
+    settle();
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
 
     // element e of acc[i][j]: column i * 16 + fk * 4 + e, row j * 16 + fl of the wavefront's part
@@ -357,41 +384,36 @@ __global__ __launch_bounds__(64 * WR * WQ) void product_k(Product p) {
         // through LDS as [row][word]: rows are written out from it as they are, columns by the transposing read
         constexpr int SLOTS = BQ / 8;
         auto at = [](int row, int slot) { return row * BQ + ((slot ^ (row & (SLOTS - 1 < 15 ? SLOTS - 1 : 15))) << 3); };
-        float lse[RI], fac[RI];
-        int t[RI];
-#pragma unroll
-        for (int j = 0; j < RI; ++j) {
-            const long long row = wr0 + j * 16 + fl;
-            const bool in = row < live;
-            lse[j] = in ? p.lse[row] : 0.f;
-            fac[j] = in ? (p.factor ? p.factor[row] : 1.f) : 0.f;
-            t[j] = in ? p.tgt[row] : -1;
-#pragma unroll
-            for (int i = 0; i < QI; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const long long c = p.q0 + wc0 + i * 16 + fk * 4 + e;
-                    float g = p.pairs == 1 ? __expf(acc[i][j][e] - lse[j]) : expf(acc[i][j][e] - lse[j]);
-                    if (c == t[j]) g -= 1.f;
-                    acc[i][j][e] = in && c < p.vocab ? g * fac[j] : 0.f;
-                }
-        }
         const int pieces = p.pairs == 1 ? 1 : 3;
-        for (int piece = 0; piece < pieces; ++piece) {
+        for (int piece = 0; piece < pieces; ++piece) {           // (a piece is split off the value formed again: no registers for rests)
             if (piece) __syncthreads();
 #pragma unroll
-            for (int j = 0; j < RI; ++j)
+            for (int j = 0; j < RI; ++j) {
+                const long long row = wr0 + j * 16 + fl;
+                const bool in = row < live;
+                const float lse = in ? p.lse[row] : 0.f, fac = in ? (p.factor ? p.factor[row] : 1.f) : 0.f;
+                const int t = in ? p.tgt[row] : -1;
 #pragma unroll
                 for (int i = 0; i < QI; ++i) {
                     bf16x4 q;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        q[e] = (bf16_t)acc[i][j][e];
-                        acc[i][j][e] -= (float)q[e];             // exact; what the next piece takes
+                        const int c = (int)(p.q0 + wc0) + i * 16 + fk * 4 + e;
+                        float g = p.pairs == 1 ? __expf(acc[i][j][e] - lse) : expf(acc[i][j][e] - lse);
+                        if (c == t) g -= 1.f;
+                        g = in && c < (int)p.vocab ? g * fac : 0.f;
+                        q[e] = (bf16_t)g;
+                        if (piece) {
+                            const float rest = g - (float)q[e];
+                            q[e] = (bf16_t)rest;
+                            if (piece == 2) q[e] = (bf16_t)(rest - (float)q[e]);
+                        }
                     }
-                    const int row = wr * TR + j * 16 + fl, col = wq * TQ + i * 16 + fk * 4;
-                    *reinterpret_cast<bf16x4*>(lds + at(row, col >> 3) + (col & 4)) = q;
+                    const int at_row = wr * TR + j * 16 + fl, col = wq * TQ + i * 16 + fk * 4;
+                    *reinterpret_cast<bf16x4*>(lds + at(at_row, col >> 3) + (col & 4)) = q;
                 }
+                __builtin_amdgcn_sched_barrier(0);               // (rows in turn: all at once would not fit the registers)
+            }
             __syncthreads();
             if (p.g)
                 for (int i = tid; i < BR * SLOTS; i += NT) {
@@ -626,7 +648,7 @@ int launch_tiles(Product& p, long long r_rows, long long q_rows, hipStream_t st)
 template <End END>
 int launch(Product& p, long long r_rows, long long q_rows, hipStream_t st) {
     if (p.splits < 1) p.splits = 1;
-    return big_tiles(r_rows, q_rows) ? launch_tiles<256, 256, 4, 2, END>(p, r_rows, q_rows, st)
+    return big_tiles(r_rows, q_rows) ? launch_tiles<256, 256, 2, 2, END>(p, r_rows, q_rows, st)
                                      : launch_tiles<128, 128, 2, 2, END>(p, r_rows, q_rows, st);
 }
 
