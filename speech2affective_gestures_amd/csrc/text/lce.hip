@@ -151,7 +151,8 @@ struct Product {
     const int* k_count;                 // not null: k is this, rounded up to 64
     const int* r_count;                 // not null: rows of R that matter
     int pairs;                          // 1, or 6 of three pieces
-    int tiles_r, tiles_q, splits;
+    int tiles_q, group;
+    int splits, slots;                  // the most parts of k; workgroups that run at a time
     // STATS: max and sum of exponentials [tile_q][padded rows], logit of the target; GRADS: lse, factor of each row
     const int* tgt;
     long long q0;                       // word number of Q's first row
@@ -162,9 +163,9 @@ struct Product {
     const float *lse, *factor;
     bf16_t *g, *gt;                     // GRADS: [row][word] pitch g_ld, [word][row] pitch gt_ld (either may be null)
     long long g_ld, g_plane, gt_ld, gt_plane;
-    // ACCUM: fp32 [split][row][col] pitch out_ld; STORE: rows of dW
+    // ACCUM: fp32 [split][row, padded to the tile][col] pitch out_ld; STORE: rows of dW
     void* out;
-    long long out_ld, out_split;
+    long long out_ld;
     int cols, add, out_bf16;
     const float* scale;                 // STORE: the factor of all rows
 };
@@ -191,7 +192,32 @@ __device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t from, bf16_t* dst,
 __device__ __forceinline__ void mfma_acc(f32x4& c, bf16x8 a, bf16x8 b) {
     asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
+// One of its values, read where it is used (the compiler would read all 256 at once and not find registers for them).
+__device__ __forceinline__ float acc_read(float a) {
+    float v;
+    asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(a));
+    return v;
+}
 __device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
+
+// exp(d): two terms of the argument's product with log2 e for fp32 operands, one for bf16 ones, whose logits carry more than that
+__device__ __forceinline__ float exp_of(float d, bool precise) {
+    if (!precise) return __expf(d);
+    d = d < -150.f ? -150.f : d;                                 // (0 in fp32 either way; an infinity has no rest)
+    const float t = d * 1.44269504088896340736f;
+    const float rest = fmaf(d, 1.44269504088896340736f, -t) + d * 1.925963033500935e-8f;     // log2 e - its fp32 value
+    const float e = exp2f(t);
+    return fmaf(e * 0.693147180559945f, rest, e);
+}
+
+// The tiles of a launch, in the order in which they are handed out; everything here is one for the workgroup.
+struct Tiles {
+    int n, splits, per, group, tiles_r, kt, total;
+};
+__host__ __device__ inline int splits_of(int tiles, int most, int slots) {       // few tiles: k is split to fill the card
+    const int s = tiles > 0 ? slots / tiles : 1;
+    return s < 1 ? 1 : s > most ? most : s;
+}
 
 template <int BR, int BQ, int WR, int WQ, End END>
 __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
@@ -200,35 +226,48 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
     constexpr int LR = BR * 8 / NT, LQ = BQ * 8 / NT;                          // 16-byte loads per thread and stage
     constexpr int STAGE = (BR + BQ) * BK;
     extern __shared__ __attribute__((aligned(16))) bf16_t lds[];
+    bf16_t* const scratch = lds + 2 * STAGE;                                   // 64 x BQ, for the ends
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave / WQ, wq = wave % WQ;
+    const bool precise = p.pairs > 1;
 
-    // Workgroups are dealt to the eight XCDs in turn; the remap gives each XCD a contiguous range of tiles, and inside it the
-    // tiles go column by column over GROUP row tiles, so that the tiles that run at the same time share operands in its L2.
-    int v;
-    {
-        const int n = gridDim.x, x = blockIdx.x & 7, q8 = n >> 3, r8 = n & 7;
-        v = (x < r8 ? x * (q8 + 1) : r8 * (q8 + 1) + (x - r8) * q8) + (blockIdx.x >> 3);
-    }
     // (whole-number division runs on the vector units: the results are told to be one for the wavefront, so that the operands'
     // descriptors stay in scalar registers)
-    const int split = __builtin_amdgcn_readfirstlane(v % p.splits);
-    v = __builtin_amdgcn_readfirstlane(v / p.splits);
-    constexpr int GROUP = 8;
-    const int per = GROUP * p.tiles_q, grp = v / per, first = grp * GROUP;
-    const int gsz = min(p.tiles_r - first, GROUP);
-    const int tr = __builtin_amdgcn_readfirstlane(first + (v - grp * per) % gsz), tq = __builtin_amdgcn_readfirstlane((v - grp * per) / gsz);
-    const long long r0 = (long long)tr * BR, c0 = (long long)tq * BQ;
-    const long long live = p.r_count ? (long long)__builtin_amdgcn_readfirstlane(*p.r_count) : p.r_rows;
-    if (r0 >= live) return;
+    const int live = p.r_count ? __builtin_amdgcn_readfirstlane(*p.r_count) : (int)p.r_rows;
+    Tiles ts;
+    ts.tiles_r = __builtin_amdgcn_readfirstlane((live + BR - 1) / BR);
+    ts.splits = __builtin_amdgcn_readfirstlane(splits_of(ts.tiles_r * p.tiles_q, p.splits, p.slots));
+    ts.kt = p.k_count ? __builtin_amdgcn_readfirstlane((*p.k_count + BK - 1) / BK) : p.k / BK;
+    ts.total = ts.kt * p.pairs;
+    ts.group = p.group;
+    ts.per = p.group * p.tiles_q;
+    ts.n = ts.tiles_r * p.tiles_q * ts.splits;
 
-    const int kt = p.k_count ? __builtin_amdgcn_readfirstlane((*p.k_count + BK - 1) / BK) : p.k / BK, total = kt * p.pairs;
-    const int it0 = __builtin_amdgcn_readfirstlane((int)((long long)total * split / p.splits));
-    const int it1 = __builtin_amdgcn_readfirstlane((int)((long long)total * (split + 1) / p.splits));
+    // A workgroup takes many tiles, so that the operands of the next one are on their way while this one ends.  Workgroups are
+    // dealt to the eight XCDs in turn; each XCD gets a contiguous range of tiles, and inside it the tiles go column by column
+    // over `group` row tiles, so that the tiles that run at the same time share operands in its L2.
+    const int xcd = blockIdx.x & 7, step = gridDim.x >> 3;
+    const int last = __builtin_amdgcn_readfirstlane((int)((long long)ts.n * (xcd + 1) / 8));
+    const int first = __builtin_amdgcn_readfirstlane((int)((long long)ts.n * xcd / 8)) + (blockIdx.x >> 3);
+    if (first >= last) return;
 
-    const long long r_left = p.r_rows - r0, q_left = p.q_rows > c0 ? p.q_rows - c0 : 0;      // (a tile may lie behind the words)
-    const int r_bytes = (int)((r_left < BR ? r_left : BR) * p.r.ld * 2), q_bytes = (int)((q_left < BQ ? q_left : BQ) * p.q.ld * 2);
+    struct Place {
+        long long r0, c0;
+        int split, it0, it1;
+    };
+    auto place = [&](int v) {
+        Place t;
+        t.split = __builtin_amdgcn_readfirstlane(v % ts.splits);
+        v = __builtin_amdgcn_readfirstlane(v / ts.splits);
+        const int grp = __builtin_amdgcn_readfirstlane(v / ts.per), g0 = grp * ts.group, gsz = min(ts.tiles_r - g0, ts.group);
+        t.r0 = (long long)__builtin_amdgcn_readfirstlane(g0 + (v - grp * ts.per) % gsz) * BR;
+        t.c0 = (long long)__builtin_amdgcn_readfirstlane((v - grp * ts.per) / gsz) * BQ;
+        t.it0 = __builtin_amdgcn_readfirstlane((int)((long long)ts.total * t.split / ts.splits));
+        t.it1 = __builtin_amdgcn_readfirstlane((int)((long long)ts.total * (t.split + 1) / ts.splits));
+        return t;
+    };
+
     const int ld_row = tid >> 3, ld_slot = (tid & 7) ^ (ld_row & 7);
     unsigned r_off[LR], q_off[LQ];
 #pragma unroll
@@ -236,17 +275,42 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
 #pragma unroll
     for (int i = 0; i < LQ; ++i) q_off[i] = (unsigned)((ld_row + i * (NT / 8)) * p.q.ld * 2 + ld_slot * 16);
 
-    // the stage that is requested next: its pair of pieces, its place along k; behind the last one the descriptors are empty, so
-    // that the loop has no branch
-    int pair = __builtin_amdgcn_readfirstlane(it0 / (kt > 0 ? kt : 1)), kk = it0 - pair * kt, left = it1 - it0;
+    // the stage that is requested next: its tile, pair of pieces and place along k; behind the last one the descriptors are
+    // empty, so that the loop has no branch
+    int next = first - step, pair = 0, kk = 0, left = 0;
+    const bf16_t *r_at = p.r.p, *q_at = p.q.p;
+    int r_bytes = 0, q_bytes = 0;
     __amdgpu_buffer_rsrc_t rr, qr;
     auto descriptors = [&]() {
-        const bf16_t* rb = p.r.p + piece_r(p.pairs == 1 ? 5 : pair) * p.r.plane + r0 * p.r.ld;
-        const bf16_t* qb = p.q.p + piece_q(p.pairs == 1 ? 5 : pair) * p.q.plane + c0 * p.q.ld;
-        rr = __builtin_amdgcn_make_buffer_rsrc((void*)rb, 0, left > 0 ? r_bytes : 0, 0x00020000);
-        qr = __builtin_amdgcn_make_buffer_rsrc((void*)qb, 0, left > 0 ? q_bytes : 0, 0x00020000);
+        rr = __builtin_amdgcn_make_buffer_rsrc((void*)(r_at + piece_r(precise ? pair : 5) * p.r.plane), 0, r_bytes, 0x00020000);
+        qr = __builtin_amdgcn_make_buffer_rsrc((void*)(q_at + piece_q(precise ? pair : 5) * p.q.plane), 0, q_bytes, 0x00020000);
     };
-    descriptors();
+    auto next_tile = [&]() {
+        r_bytes = q_bytes = 0;
+        for (next += step; next < last; next += step) {
+            const Place t = place(next);
+            left = t.it1 - t.it0;
+            if (left <= 0) continue;                             // (no stage: nothing to request)
+            pair = __builtin_amdgcn_readfirstlane(t.it0 / ts.kt);
+            kk = t.it0 - pair * ts.kt;
+            const long long r_left = p.r_rows - t.r0, q_left = p.q_rows > t.c0 ? p.q_rows - t.c0 : 0;      // (a tile may lie behind the words)
+            r_bytes = (int)((r_left < BR ? r_left : BR) * p.r.ld * 2);
+            q_bytes = (int)((q_left < BQ ? q_left : BQ) * p.q.ld * 2);
+            r_at = p.r.p + t.r0 * p.r.ld;
+            q_at = p.q.p + t.c0 * p.q.ld;
+            break;
+        }
+        descriptors();
+    };
+    auto advance = [&]() {
+        if (--left <= 0) {
+            next_tile();
+        } else if (++kk == ts.kt) {
+            kk = 0;
+            ++pair;
+            descriptors();
+        }
+    };
     // requests [from, from + n) of the LR + LQ of a stage
     auto issue = [&](int buf, int from, int n) {
         bf16_t* s = lds + buf * STAGE + wave * 512;
@@ -257,28 +321,19 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
             else to_lds(qr, s + BR * BK + (i - LR) * NT * 8, q_off[i < LR ? 0 : i - LR], off);
         }
     };
-    auto advance = [&]() {
-        --left;
-        if (++kk == kt) {
-            kk = 0;
-            pair = pair + 1 < p.pairs ? pair + 1 : pair;
-        }
-        descriptors();
-    };
 
     f32x4 acc[QI][RI];
-#pragma unroll
-    for (int i = 0; i < QI; ++i)
-#pragma unroll
-        for (int j = 0; j < RI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
     const int fl = lane & 15, fk = lane >> 4;
     const bf16_t* const rs = lds + wr * TR * BK;
     const bf16_t* const qs = lds + BR * BK + wq * TQ * BK;
-    // fragment [u] of half ks of a stage: the QI of Q, then the RI of R
-    auto fragment = [&](bf16x8 (&a)[QI], bf16x8 (&b)[RI], int buf, int ks, int u) {
-        if (u < QI) a[u < QI ? u : 0] = *reinterpret_cast<const bf16x8*>(qs + buf * STAGE + slot_at(u * 16 + fl, ks * 4 + fk));
-        else b[u < QI ? 0 : u - QI] = *reinterpret_cast<const bf16x8*>(rs + buf * STAGE + slot_at((u - QI) * 16 + fl, ks * 4 + fk));
+    // fragments [from, to) of half ks of a stage
+    auto read_q = [&](bf16x8 (&a)[QI], int buf, int ks, int from, int to) {
+#pragma unroll
+        for (int i = from; i < to; ++i) a[i] = *reinterpret_cast<const bf16x8*>(qs + buf * STAGE + slot_at(i * 16 + fl, ks * 4 + fk));
+    };
+    auto read_r = [&](bf16x8 (&b)[RI], int buf, int ks, int from, int to) {
+#pragma unroll
+        for (int j = from; j < to; ++j) b[j] = *reinterpret_cast<const bf16x8*>(rs + buf * STAGE + slot_at(j * 16 + fl, ks * 4 + fk));
     };
     auto multiply = [&](const bf16x8 (&a)[QI], const bf16x8 (&b)[RI], int i) {
 #pragma unroll
@@ -288,199 +343,249 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
         }
     };
 
-    // Two stages in LDS, two halves of a stage in registers.  While the first half of a stage is multiplied its second half is
-    // read; then every wavefront is done with the stage's LDS, the next stage (requested a whole stage ago) has landed, and while
-    // the second half is multiplied the first half of the next stage is read and the stage after it is requested.  Reads and
-    // requests go behind rows of matrix instructions, the reads behind the first ones, so that they run beside the others.
-    constexpr int PER = (QI + RI + QI / 2 - 1) / (QI / 2), LPER = (LR + LQ + QI - 1) / QI;
-    const int stages = it1 - it0;
+    auto value = [&](int i, int j, int e) {
+        if constexpr (RI * QI * 4 == 256) return acc_read(acc[i][j][e]);
+        else return acc[i][j][e];
+    };
+
+    // Two stages in LDS, two halves of a stage in registers, matrix instructions in QI groups a half.  While the first half of a
+    // stage is multiplied its second half is read, R before Q: when every wavefront has its part of R, R's place is free and the
+    // R of the stage after the next is requested; in the middle of the stage all of it is read, the next stage (requested a
+    // stage ago) has landed, and while the second half is multiplied the first half of the next stage is read and the Q of the
+    // stage after it is requested.  A request keeps a wavefront's issue busy for as long as eight of its matrix instructions may
+    // take: one or two a group; twice as many at half the places cost a tenth of the rate.
+    constexpr int G = QI, EARLY = G / 2 - 1, RN = G - EARLY, RB = RI / (G / 4), QB = QI / (G / 4);
     bf16x8 a0[QI], b0[RI], a1[QI], b1[RI];
+    next_tile();
     issue(0, 0, LR + LQ);
     advance();
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     issue(1, 0, LR + LQ);
     advance();
+    read_r(b0, 0, 0, 0, RI);
+    read_q(a0, 0, 0, 0, QI);
+    int buf = 0;
+    for (int tile = first; tile < last; tile += step) {
+        const Place t = place(tile);
 #pragma unroll
-    for (int u = 0; u < QI + RI; ++u) fragment(a0, b0, 0, 0, u);
-    settle();
-    for (int n = 0; n < stages; ++n) {
-        const int buf = n & 1;
+        for (int i = 0; i < QI; ++i)
 #pragma unroll
-        for (int i = 0; i < QI; ++i) {
-            multiply(a0, b0, i);
-            __builtin_amdgcn_sched_barrier(0);
+            for (int j = 0; j < RI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        settle();
+        for (int n = t.it0; n < t.it1; ++n) {
 #pragma unroll
-            for (int u = i * PER; u < (i + 1) * PER && u < QI + RI; ++u) fragment(a1, b1, buf, 1, u);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // (keeps the reads behind the barrier)
-#pragma unroll
-        for (int i = 0; i < QI; ++i) {
-            multiply(a1, b1, i);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int u = i * PER; u < (i + 1) * PER && u < QI + RI; ++u) fragment(a0, b0, buf ^ 1, 0, u);
-            issue(buf, i * LPER, (i + 1) * LPER < LR + LQ ? LPER : LR + LQ - i * LPER);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        advance();
-    }
-    settle();
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-
-    // element e of acc[i][j]: column i * 16 + fk * 4 + e, row j * 16 + fl of the wavefront's part
-    const long long wr0 = r0 + wr * TR, wc0 = c0 + wq * TQ;
-    if constexpr (END == STATS) {
-        float2* sm = reinterpret_cast<float2*>(lds);             // [WQ][BR]
-#pragma unroll
-        for (int j = 0; j < RI; ++j) {
-            const long long row = wr0 + j * 16 + fl;
-            const int t = row < live ? p.tgt[row] : -1;
-            float m = -INFINITY;
-            bool mine = false;
-            float tl = 0.f;
-#pragma unroll
-            for (int i = 0; i < QI; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const long long c = p.q0 + wc0 + i * 16 + fk * 4 + e;
-                    if (c == t) {
-                        tl = acc[i][j][e];
-                        mine = true;
-                    }
-                    if (c >= p.vocab) acc[i][j][e] = -INFINITY;
-                    m = fmaxf(m, acc[i][j][e]);
+            for (int i = 0; i < G; ++i) {
+                multiply(a0, b0, i);
+                __builtin_amdgcn_sched_barrier(0);
+                if (i < G / 4) read_r(b1, buf, 1, i * RB, (i + 1) * RB);
+                if (i == EARLY) {
+                    if constexpr (G / 4 < EARLY) asm volatile("s_waitcnt lgkmcnt(4)" ::: "memory");
+                    else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    __builtin_amdgcn_s_barrier();
+                    asm volatile("s_waitcnt lgkmcnt(15)" ::: "memory");      // (keeps the requests behind the barrier)
                 }
-            if (mine) p.target_logit[row] = tl;
-            m = fmaxf(m, __shfl_xor(m, 16));
-            m = fmaxf(m, __shfl_xor(m, 32));
-            const float ms = m == -INFINITY ? 0.f : m;           // a part that lies behind the vocabulary: a sum of 0
-            float s = 0.f;
-#pragma unroll
-            for (int i = 0; i < QI; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s += p.pairs == 1 ? __expf(acc[i][j][e] - ms) : expf(acc[i][j][e] - ms);
-            s += __shfl_xor(s, 16);
-            s += __shfl_xor(s, 32);
-            if (fk == 0) sm[wq * BR + wr * TR + j * 16 + fl] = make_float2(m, s);
-        }
-        __syncthreads();
-        for (int r = tid; r < BR; r += NT) {
-            float2 a = sm[r];
-#pragma unroll
-            for (int w = 1; w < WQ; ++w) {
-                const float2 b = sm[w * BR + r];
-                const float m = fmaxf(a.x, b.x), ms = m == -INFINITY ? 0.f : m;
-                a = make_float2(m, a.y * expf(a.x - ms) + b.y * expf(b.x - ms));
+                if (i >= G / 4 && i < G / 2) read_q(a1, buf, 1, (i - G / 4) * QB, (i - G / 4 + 1) * QB);
+                if (i >= EARLY) issue(buf, (i - EARLY) * LR / RN, (i - EARLY + 1) * LR / RN - (i - EARLY) * LR / RN);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            p.part[tq * p.part_ld + r0 + r] = a;
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if constexpr (LR == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+            else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+            static_assert(LR == 8 || LR == 4, "the requests for R of the stage after the next stay out");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (keeps the reads behind the barrier)
+#pragma unroll
+            for (int i = 0; i < G; ++i) {
+                multiply(a1, b1, i);
+                __builtin_amdgcn_sched_barrier(0);
+                if (i < G / 4) read_r(b0, buf ^ 1, 0, i * RB, (i + 1) * RB);
+                if (i >= G / 4 && i < G / 2) read_q(a0, buf ^ 1, 0, (i - G / 4) * QB, (i - G / 4 + 1) * QB);
+                issue(buf, LR + i * LQ / G, (i + 1) * LQ / G - i * LQ / G);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            advance();
+            buf ^= 1;
         }
-    } else if constexpr (END == GRADS) {
-        // through LDS as [row][word]: rows are written out from it as they are, columns by the transposing read
-        constexpr int SLOTS = BQ / 8;
-        auto at = [](int row, int slot) { return row * BQ + ((slot ^ (row & (SLOTS - 1 < 15 ? SLOTS - 1 : 15))) << 3); };
-        const int pieces = p.pairs == 1 ? 1 : 3;
-        for (int piece = 0; piece < pieces; ++piece) {           // (a piece is split off the value formed again: no registers for rests)
-            if (piece) __syncthreads();
+        settle();
+
+        // element e of acc[i][j]: column i * 16 + fk * 4 + e, row j * 16 + fl of the wavefront's part
+        const long long wr0 = t.r0 + wr * TR, wc0 = t.c0 + wq * TQ;
+        if constexpr (END == STATS || END == GRADS) {
+            const int word0 = (int)(p.q0 + wc0) + fk * 4;        // the lane's first word
+            const int words = (int)p.vocab - word0;              // that it may use, counted from there
+            const bool edge = p.q0 + t.c0 + BQ > p.vocab;
+            if constexpr (END == STATS) {
+                float2* sm = reinterpret_cast<float2*>(scratch);     // [WQ][BR]
+#pragma unroll
+                for (int j = 0; j < RI; ++j) {
+                    const int row = (int)wr0 + j * 16 + fl;
+                    const unsigned at = (unsigned)((row < live ? p.tgt[row] : -1) - word0);     // the target's place, if it is the lane's
+                    float z[QI * 4], m4[4], s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int i = 0; i < QI * 4; ++i) z[i] = value(i / 4, j, i % 4);
+                    if (edge) {
+#pragma unroll
+                        for (int i = 0; i < QI * 4; ++i)
+                            if (i / 4 * 16 + i % 4 >= words) z[i] = -INFINITY;
+                    }
+                    if (at < (unsigned)TQ) {
+#pragma unroll
+                        for (int i = 0; i < QI * 4; ++i)
+                            if (at == (unsigned)(i / 4 * 16 + i % 4)) p.target_logit[row] = z[i];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) m4[e] = z[e];
+#pragma unroll
+                    for (int i = 4; i < QI * 4; ++i) m4[i % 4] = fmaxf(m4[i % 4], z[i]);
+                    float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                    m = fmaxf(m, __shfl_xor(m, 16));
+                    m = fmaxf(m, __shfl_xor(m, 32));
+                    const float ms = m == -INFINITY ? 0.f : m;   // a part that lies behind the vocabulary: a sum of 0
+#pragma unroll
+                    for (int i = 0; i < QI * 4; ++i) s4[i % 4] += exp_of(z[i] - ms, precise);
+                    float s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+                    s += __shfl_xor(s, 16);
+                    s += __shfl_xor(s, 32);
+                    if (fk == 0) sm[wq * BR + wr * TR + j * 16 + fl] = make_float2(m, s);
+                    __builtin_amdgcn_sched_barrier(0);           // (rows in turn: all at once would not fit the registers)
+                }
+                __syncthreads();
+                for (int r = tid; r < BR; r += NT) {
+                    float2 a = sm[r];
+#pragma unroll
+                    for (int w = 1; w < WQ; ++w) {
+                        const float2 b = sm[w * BR + r];
+                        const float m = fmaxf(a.x, b.x), ms = m == -INFINITY ? 0.f : m;
+                        a = make_float2(m, a.y * expf(a.x - ms) + b.y * expf(b.x - ms));
+                    }
+                    p.part[t.c0 / BQ * p.part_ld + t.r0 + r] = a;
+                }
+            } else {
+                // Through LDS as [row][word], 32 rows of each of the WR parts at a time: rows are written out from it as they
+                // are, columns by the transposing read.
+                constexpr int SLOTS = BQ / 8;
+                auto at = [](int row, int slot) { return row * BQ + ((slot ^ (row & 15)) << 3); };
+                const int pieces = precise ? 3 : 1;
+                for (int piece = 0; piece < pieces; ++piece) {   // (a piece is split off the value formed again: no registers for rests)
+#pragma unroll
+                    for (int jj = 0; jj < RI; jj += 2) {
+#pragma unroll
+                        for (int j = jj; j < jj + 2; ++j) {
+                            const int row = (int)wr0 + j * 16 + fl;
+                            const bool in = row < live;          // (rows behind are zeros: a factor of 0 keeps them so)
+                            const float lse = in ? p.lse[row] : 0.f, fac = in ? (p.factor ? p.factor[row] : 1.f) : 0.f;
+                            const unsigned tgt = (unsigned)((in ? p.tgt[row] : -1) - word0);
+#pragma unroll
+                            for (int i = 0; i < QI; ++i) {
+                                float g[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) g[e] = exp_of(value(i, j, e) - lse, precise);
+                                if (tgt - i * 16 < 4u) {
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) g[e] -= tgt - i * 16 == (unsigned)e ? 1.f : 0.f;
+                                }
+                                if (edge) {
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e)
+                                        if (i * 16 + e >= words) g[e] = 0.f;
+                                }
+                                bf16x4 q;
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    g[e] *= fac;
+                                    q[e] = (bf16_t)g[e];
+                                    if (piece) {
+                                        const float rest = g[e] - (float)q[e];
+                                        q[e] = (bf16_t)rest;
+                                        if (piece == 2) q[e] = (bf16_t)(rest - (float)q[e]);
+                                    }
+                                }
+                                const int lrow = wr * 32 + (j - jj) * 16 + fl, col = wq * TQ + i * 16 + fk * 4;
+                                *reinterpret_cast<bf16x4*>(scratch + at(lrow, col >> 3) + (col & 4)) = q;
+                            }
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                        __syncthreads();
+                        if (p.g)
+                            for (int i = tid; i < WR * 32 * SLOTS; i += NT) {
+                                const int lrow = i / SLOTS, slot = i % SLOTS;
+                                const long long row = t.r0 + (lrow >> 5) * TR + jj * 16 + (lrow & 31);
+                                *reinterpret_cast<bf16x8*>(p.g + piece * p.g_plane + row * p.g_ld + t.c0 + slot * 8) =
+                                    *reinterpret_cast<const bf16x8*>(scratch + at(lrow, slot));
+                            }
+                        if (p.gt)
+                            // a wavefront takes 16 words x 32 rows: its four groups of 16 lanes eight rows each, in two reads of four
+                            for (int u = wave; u < (BQ / 16) * WR; u += NT / 64) {
+                                const int w0 = (u % (BQ / 16)) * 16, part = u / (BQ / 16);
+                                bf16x8 q;
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    const int lrow = part * 32 + fk * 8 + h * 4 + (fl >> 2), col = w0 + (fl & 3) * 4;
+                                    const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                        S2AG_LDS_PTR(s16x4_t, scratch + at(lrow, col >> 3) + (col & 4)));
+                                    const bf16x4 y = __builtin_bit_cast(bf16x4, x);
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) q[h * 4 + e] = y[e];
+                                }
+                                *reinterpret_cast<bf16x8*>(p.gt + piece * p.gt_plane + (t.c0 + w0 + fl) * p.gt_ld + t.r0 + part * TR + jj * 16 +
+                                                           fk * 8) = q;
+                            }
+                        __syncthreads();
+                    }
+                }
+            }
+        } else if constexpr (END == ACCUM) {
+            float* out = static_cast<float*>(p.out) + (long long)t.split * ts.tiles_r * BR * p.out_ld;
 #pragma unroll
             for (int j = 0; j < RI; ++j) {
                 const long long row = wr0 + j * 16 + fl;
-                const bool in = row < live;
-                const float lse = in ? p.lse[row] : 0.f, fac = in ? (p.factor ? p.factor[row] : 1.f) : 0.f;
-                const int t = in ? p.tgt[row] : -1;
 #pragma unroll
                 for (int i = 0; i < QI; ++i) {
-                    bf16x4 q;
+                    const long long c = wc0 + i * 16 + fk * 4;
+                    if (row >= live || c >= p.cols) continue;    // (out_ld is a multiple of 4)
+                    f32x4* o = reinterpret_cast<f32x4*>(out + row * p.out_ld + c);
+                    f32x4 x;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int c = (int)(p.q0 + wc0) + i * 16 + fk * 4 + e;
-                        float g = p.pairs == 1 ? __expf(acc[i][j][e] - lse) : expf(acc[i][j][e] - lse);
-                        if (c == t) g -= 1.f;
-                        g = in && c < (int)p.vocab ? g * fac : 0.f;
-                        q[e] = (bf16_t)g;
-                        if (piece) {
-                            const float rest = g - (float)q[e];
-                            q[e] = (bf16_t)rest;
-                            if (piece == 2) q[e] = (bf16_t)(rest - (float)q[e]);
+                    for (int e = 0; e < 4; ++e) x[e] = value(i, j, e);
+                    if (p.add) x += *o;
+                    *o = x;
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            const float f = p.scale ? *p.scale : 1.f;
+#pragma unroll
+            for (int j = 0; j < RI; ++j) {
+                const long long row = wr0 + j * 16 + fl;
+#pragma unroll
+                for (int i = 0; i < QI; ++i) {
+                    const long long c = wc0 + i * 16 + fk * 4;
+                    if (row >= p.r_rows || c >= p.cols) continue;
+                    f32x4 x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = value(i, j, e) * f;
+                    if (p.out_bf16) {
+                        bf16_t* o = static_cast<bf16_t*>(p.out) + row * p.out_ld + c;
+                        if ((p.out_ld & 3) == 0) {
+                            bf16x4 q;
+                            for (int e = 0; e < 4; ++e) q[e] = (bf16_t)x[e];
+                            *reinterpret_cast<bf16x4*>(o) = q;
+                        } else {
+                            for (int e = 0; e < 4; ++e)
+                                if (c + e < p.cols) o[e] = (bf16_t)x[e];
                         }
-                    }
-                    const int at_row = wr * TR + j * 16 + fl, col = wq * TQ + i * 16 + fk * 4;
-                    *reinterpret_cast<bf16x4*>(lds + at(at_row, col >> 3) + (col & 4)) = q;
-                }
-                __builtin_amdgcn_sched_barrier(0);               // (rows in turn: all at once would not fit the registers)
-            }
-            __syncthreads();
-            if (p.g)
-                for (int i = tid; i < BR * SLOTS; i += NT) {
-                    const int row = i / SLOTS, slot = i % SLOTS;
-                    *reinterpret_cast<bf16x8*>(p.g + piece * p.g_plane + (r0 + row) * p.g_ld + c0 + slot * 8) =
-                        *reinterpret_cast<const bf16x8*>(lds + at(row, slot));
-                }
-            if (p.gt)
-                // a wavefront takes 16 words x 32 rows: its four groups of 16 lanes eight rows each, in two reads of four
-                for (int u = wave; u < (BQ / 16) * (BR / 32); u += NT / 64) {
-                    const int w0 = (u % (BQ / 16)) * 16, rr = (u / (BQ / 16)) * 32 + fk * 8;
-                    bf16x8 q;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int row = rr + h * 4 + (fl >> 2), col = w0 + (fl & 3) * 4;
-                        const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            S2AG_LDS_PTR(s16x4_t, lds + at(row, col >> 3) + (col & 4)));
-                        const bf16x4 y = __builtin_bit_cast(bf16x4, x);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) q[h * 4 + e] = y[e];
-                    }
-                    *reinterpret_cast<bf16x8*>(p.gt + piece * p.gt_plane + (c0 + w0 + fl) * p.gt_ld + r0 + rr) = q;
-                }
-        }
-    } else if constexpr (END == ACCUM) {
-        float* out = static_cast<float*>(p.out) + split * p.out_split;
-#pragma unroll
-        for (int j = 0; j < RI; ++j) {
-            const long long row = wr0 + j * 16 + fl;
-#pragma unroll
-            for (int i = 0; i < QI; ++i) {
-                const long long c = wc0 + i * 16 + fk * 4;
-                if (row >= live || c >= p.cols) continue;        // (out_ld is a multiple of 4)
-                f32x4* o = reinterpret_cast<f32x4*>(out + row * p.out_ld + c);
-                f32x4 x = acc[i][j];
-                if (p.add) x += *o;
-                *o = x;
-            }
-        }
-    } else {
-        const float f = p.scale ? *p.scale : 1.f;
-#pragma unroll
-        for (int j = 0; j < RI; ++j) {
-            const long long row = wr0 + j * 16 + fl;
-#pragma unroll
-            for (int i = 0; i < QI; ++i) {
-                const long long c = wc0 + i * 16 + fk * 4;
-                if (row >= p.r_rows || c >= p.cols) continue;
-                const f32x4 x = acc[i][j] * f;
-                if (p.out_bf16) {
-                    bf16_t* o = static_cast<bf16_t*>(p.out) + row * p.out_ld + c;
-                    if ((p.out_ld & 3) == 0) {
-                        bf16x4 q;
-                        for (int e = 0; e < 4; ++e) q[e] = (bf16_t)x[e];
-                        *reinterpret_cast<bf16x4*>(o) = q;
                     } else {
+                        float* o = static_cast<float*>(p.out) + row * p.out_ld + c;
                         for (int e = 0; e < 4; ++e)
-                            if (c + e < p.cols) o[e] = (bf16_t)x[e];
+                            if (c + e < p.cols) o[e] = p.add ? o[e] + x[e] : x[e];
                     }
-                } else {
-                    float* o = static_cast<float*>(p.out) + row * p.out_ld + c;
-                    for (int e = 0; e < 4; ++e)
-                        if (c + e < p.cols) o[e] = p.add ? o[e] + x[e] : x[e];
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // (requests with empty descriptors may still be out)
 }
 
 // ---- joins -------------------------------------------------------------------------------------------------------------------
@@ -542,17 +647,25 @@ __global__ __launch_bounds__(256) void factors_k(const float* __restrict__ grad_
 
 // dx[r] = factor * sum over the splits of the packed row, zeros for rows that were ignored
 template <typename T>
-__global__ __launch_bounds__(256) void finish_dx_k(const float* __restrict__ acc, long long ld, long long split, int splits, State s,
-                                                   const float* __restrict__ scale, long long rows, int dim, T* __restrict__ dx) {
+__global__ __launch_bounds__(256) void finish_dx_k(const float* __restrict__ acc, long long ld, int tile, int tiles_q, int most, int slots,
+                                                   State s, const float* __restrict__ scale, long long rows, int dim, T* __restrict__ dx) {
     const float f = scale ? *scale : 1.f;
-    const int groups = (dim + 3) / 4;
+    const int groups = (dim + 3) / 4, tiles_r = (*s.count + tile - 1) / tile, splits = splits_of(tiles_r * tiles_q, most, slots);
+    const long long split = (long long)tiles_r * tile * ld;
     const long long total = rows * groups;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
         const long long r = i / groups;
         const int c = (int)(i - r * groups) * 4, at = s.inv[r];
         f32x4 x = {0.f, 0.f, 0.f, 0.f};
         if (at >= 0) {
-            for (int k = 0; k < splits; ++k) x += *reinterpret_cast<const f32x4*>(acc + k * split + at * ld + c);
+            const float* q = acc + at * ld + c;
+            int k = 0;
+            for (; k + 8 <= splits; k += 8) {                    // eight loads in flight
+                f32x4 v[8];
+                for (int u = 0; u < 8; ++u) v[u] = *reinterpret_cast<const f32x4*>(q + (k + u) * split);
+                for (int u = 0; u < 8; ++u) x += v[u];
+            }
+            for (; k < splits; ++k) x += *reinterpret_cast<const f32x4*>(q + k * split);
             x *= f;
         }
         T* o = dx + r * dim + c;
@@ -570,7 +683,7 @@ struct Plan {
     // bytes from the workspace's start
     long long xp, wp, part, tl, row_loss, xt, wt, factor, acc, g, gt, bytes;
     long long piece;                    // words of a piece of the vocabulary
-    int splits, acc_ld;
+    int acc_tile, splits, acc_ld;       // of the product that dX is
 };
 
 constexpr long long PIECE_VALUES = 1LL << 27;   // of G in a piece: 256 MB each way in bf16, beside which the fp32 sums of dX are small
@@ -580,6 +693,8 @@ bool valid(const s2ag_lce_args* a) {
     return a && a->rows >= 0 && a->rows <= (1 << 21) && a->vocab > 0 && a->vocab <= (1 << 21) && a->dim > 0 && a->dim <= (1 << 20) &&
            a->ldx >= a->dim && a->ldw >= a->dim && a->reduction >= 0 && a->reduction <= 2 && !(a->bf16 && a->dw_accumulate);
 }
+
+constexpr int SLOTS = 256;              // large tiles: one workgroup on a compute unit; small ones: two
 
 // 256 x 256 tiles where they fill the 256 compute units, else 128 x 128
 bool big_tiles(long long r, long long q) { return cdiv(r, 256) * (long long)cdiv(q, 256) >= 256; }
@@ -610,17 +725,15 @@ Plan plan(const s2ag_lce_args* a, bool backward) {
         p.piece = round_up(cdiv(p.vp, pieces), 256);
         const bool dx = a->dx != nullptr, dw = a->dw != nullptr;
         p.acc_ld = (int)round_up(a->dim, 4);
-        // few tiles: the words of a piece are split, down to 16 stages each
-        const bool big = big_tiles(p.np, a->dim);
-        const long long tiles = (long long)cdiv(p.np, big ? 256 : 128) * cdiv(a->dim, big ? 256 : 128);
-        long long s = cdiv(512, tiles ? tiles : 1);
+        // dX has few tiles: the words of a piece are split, down to eight stages each
+        p.acc_tile = 256;
         const long long stages = p.piece / BK * p.pairs;
-        if (s > stages / 16) s = stages / 16;
-        p.splits = big || s < 1 ? 1 : (int)s;
+        p.splits = (int)(stages / 8 < 1 ? 1 : stages / 8 > SLOTS ? SLOTS : stages / 8);
         p.xt = take(dw ? 2 * p.planes * a->dim * p.np : 0);
         p.wt = take(dx ? 2 * p.planes * a->dim * p.vp : 0);
         p.factor = take(4 * (a->reduction == S2AG_LCE_NONE ? p.np : 1));
-        p.acc = take(dx ? 4 * p.splits * p.np * p.acc_ld : 0);
+        // (what fills the card with splits is no more than its tiles hold)
+        p.acc = take(dx ? 4 * (p.np * p.acc_ld + (long long)SLOTS * 256 * 256) : 0);
         p.g = take(dx ? 2 * p.planes * p.np * p.piece : 0);
         p.gt = take(dw ? 2 * p.planes * p.np * p.piece : 0);
     }
@@ -630,26 +743,29 @@ Plan plan(const s2ag_lce_args* a, bool backward) {
 
 template <int BR, int BQ, int WR, int WQ, End END>
 int launch_tiles(Product& p, long long r_rows, long long q_rows, hipStream_t st) {
-    constexpr int LDS = 2 * (BR + BQ) * BK * 2;
-    static_assert(LDS >= BR * BQ * 2 && LDS >= WQ * BR * 8, "the ends reuse the stages");
+    constexpr int LDS = (2 * (BR + BQ) * BK + 64 * BQ) * 2, PER_CU = BR == 256 ? 1 : 2;
+    static_assert(LDS * PER_CU <= 160 * 1024 && WR == 2 && 64 * BQ * 2 >= WQ * BR * 8, "the ends' scratch");
     // (every time: the attribute belongs to the current device)
     if (hipFuncSetAttribute((const void*)product_k<BR, BQ, WR, WQ, END>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess)
         return S2AG_E_UNSUPPORTED;
-    p.tiles_r = cdiv(r_rows, BR);
+    // The rows of R of a group stay in an XCD's 4 MB L2 while the columns pass, if half of it holds them (k of 1024: 4 row tiles
+    // 816 TFLOP/s, 8 of them 560; of 2048: 2 row tiles 1023, 8 of them 841); where not two fit, the 8 x 4 tiles that run at a time
+    // share what they can.
+    const long long fit = (2LL << 20) / (2LL * BR * (p.k_count ? p.r.ld : p.k));
+    p.group = fit >= 8 || fit < 2 ? 8 : fit >= 4 ? 4 : 2;
     p.tiles_q = cdiv(q_rows, BQ);
-    const long long n = (long long)p.tiles_r * p.tiles_q * p.splits;
-    if (n > 0x7fffffffLL) return S2AG_E_UNSUPPORTED;
-    if (n == 0) return 0;
-    hipLaunchKernelGGL((product_k<BR, BQ, WR, WQ, END>), dim3((unsigned)n), dim3(64 * WR * WQ), LDS, st, p);
+    p.slots = SLOTS * PER_CU;
+    if (p.splits < 1) p.splits = 1;
+    if ((long long)cdiv(r_rows, BR) * p.tiles_q * p.splits > 0x3fffffffLL) return S2AG_E_UNSUPPORTED;
+    if (r_rows == 0 || q_rows == 0) return 0;
+    hipLaunchKernelGGL((product_k<BR, BQ, WR, WQ, END>), dim3(p.slots), dim3(64 * WR * WQ), LDS, st, p);
     S2AG_LAUNCH_CHECK();
     return 0;
 }
 
 template <End END>
-int launch(Product& p, long long r_rows, long long q_rows, hipStream_t st) {
-    if (p.splits < 1) p.splits = 1;
-    return big_tiles(r_rows, q_rows) ? launch_tiles<256, 256, 2, 2, END>(p, r_rows, q_rows, st)
-                                     : launch_tiles<128, 128, 2, 2, END>(p, r_rows, q_rows, st);
+int launch(Product& p, bool big, long long r_rows, long long q_rows, hipStream_t st) {
+    return big ? launch_tiles<256, 256, 2, 2, END>(p, r_rows, q_rows, st) : launch_tiles<128, 128, 2, 2, END>(p, r_rows, q_rows, st);
 }
 
 unsigned grid_of(long long work) {
@@ -723,7 +839,7 @@ extern "C" int s2ag_lce_fwd(const s2ag_lce_args* a, void* stream) {
         q.part = reinterpret_cast<float2*>(ws + p.part);
         q.part_ld = p.np;
         q.target_logit = reinterpret_cast<float*>(ws + p.tl);
-        if (int rc = launch<STATS>(q, p.np, a->vocab, st)) return rc;
+        if (int rc = launch<STATS>(q, big_tiles(p.np, a->vocab), p.np, a->vocab, st)) return rc;
         hipLaunchKernelGGL(join_stats_k, dim3((unsigned)(p.np / 64)), dim3(1024), 0, st, q.part, q.part_ld, q.tiles_q, s, q.target_logit,
                            a->reduction, a->loss, row_loss);
         S2AG_LAUNCH_CHECK();
@@ -787,7 +903,7 @@ extern "C" int s2ag_lce_bwd(const s2ag_lce_args* a, void* stream) {
         q.gt = a->dw ? gt : nullptr;
         q.gt_ld = p.np;
         q.gt_plane = p.piece * p.np;
-        if (int rc = launch<GRADS>(q, p.np, wide, st)) return rc;
+        if (int rc = launch<GRADS>(q, big_tiles(p.np, wide), p.np, wide, st)) return rc;
         if (a->dx) {
             Product d{};
             d.r = Operand{g, q.g_plane, p.piece};
@@ -800,9 +916,8 @@ extern "C" int s2ag_lce_bwd(const s2ag_lce_args* a, void* stream) {
             d.splits = p.splits;
             d.out = acc;
             d.out_ld = p.acc_ld;
-            d.out_split = p.np * p.acc_ld;
             d.add = v0 > 0;
-            if (int rc = launch<ACCUM>(d, p.np, a->dim, st)) return rc;
+            if (int rc = launch<ACCUM>(d, true, p.np, a->dim, st)) return rc;
         }
         if (a->dw) {
             Product d{};
@@ -817,16 +932,16 @@ extern "C" int s2ag_lce_bwd(const s2ag_lce_args* a, void* stream) {
             d.out_bf16 = a->bf16;
             d.add = a->dw_accumulate;
             d.scale = each ? nullptr : factor;
-            if (int rc = launch<STORE>(d, words, a->dim, st)) return rc;
+            if (int rc = launch<STORE>(d, big_tiles(words, a->dim), words, a->dim, st)) return rc;
         }
     }
     if (a->dx && a->rows) {
         const unsigned gx = grid_of(a->rows * ((a->dim + 3) / 4));
         if (a->bf16)
-            hipLaunchKernelGGL(finish_dx_k<bf16_t>, dim3(gx), dim3(256), 0, st, acc, (long long)p.acc_ld, p.np * p.acc_ld, p.splits, s,
+            hipLaunchKernelGGL(finish_dx_k<bf16_t>, dim3(gx), dim3(256), 0, st, acc, (long long)p.acc_ld, p.acc_tile, cdiv(a->dim, p.acc_tile), p.splits, SLOTS, s,
                                each ? nullptr : factor, a->rows, a->dim, static_cast<bf16_t*>(a->dx));
         else
-            hipLaunchKernelGGL(finish_dx_k<float>, dim3(gx), dim3(256), 0, st, acc, (long long)p.acc_ld, p.np * p.acc_ld, p.splits, s,
+            hipLaunchKernelGGL(finish_dx_k<float>, dim3(gx), dim3(256), 0, st, acc, (long long)p.acc_ld, p.acc_tile, cdiv(a->dim, p.acc_tile), p.splits, SLOTS, s,
                                each ? nullptr : factor, a->rows, a->dim, static_cast<float*>(a->dx));
         S2AG_LAUNCH_CHECK();
     }
