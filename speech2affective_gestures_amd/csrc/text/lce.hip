@@ -219,6 +219,62 @@ __host__ __device__ inline int splits_of(int tiles, int most, int slots) {      
     return s < 1 ? 1 : s > most ? most : s;
 }
 
+// A tile of values to out[row][column], rows below `live` and columns below p.cols.
+template <typename T, int BR, int BQ, int WR, int WQ, typename F>
+__device__ __forceinline__ void write_out(bf16_t* scratch, T* out, const Product& p, long long r0, long long c0, int live, float f, F value) {
+    constexpr int NT = 64 * WR * WQ, TR = BR / WR, TQ = BQ / WQ, RI = TR / 16, QI = TQ / 16;
+    constexpr int V = Vec<T>::N, SLOTS = BQ / V, JS = 4 / (int)sizeof(T);         // 32 or 16 rows of each part at a time
+    T* const lds = reinterpret_cast<T*>(scratch);
+    auto at = [](int row, int slot) { return row * BQ + ((slot ^ (row & 15)) * V); };
+    const int lane = threadIdx.x & 63, fl = lane & 15, fk = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / WQ, wq = wave % WQ;
+    const bool vectors = (p.out_ld % V == 0) && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+#pragma unroll
+    for (int jj = 0; jj < RI; jj += JS) {
+#pragma unroll
+        for (int j = jj; j < jj + JS; ++j) {
+#pragma unroll
+            for (int i = 0; i < QI; ++i) {
+                const int lrow = wr * 16 * JS + (j - jj) * 16 + fl, col = wq * TQ + i * 16 + fk * 4;
+                T* o = lds + at(lrow, col / V) + col % V;
+                if constexpr (sizeof(T) == 2) {
+                    bf16x4 q;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) q[e] = (bf16_t)(value(i, j, e) * f);
+                    *reinterpret_cast<bf16x4*>(o) = q;
+                } else {
+                    f32x4 q;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) q[e] = value(i, j, e) * f;
+                    *reinterpret_cast<f32x4*>(o) = q;
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < WR * 16 * JS * SLOTS; i += NT) {
+            const int lrow = i / SLOTS, slot = i % SLOTS;
+            const long long row = r0 + lrow / (16 * JS) * TR + jj * 16 + lrow % (16 * JS), c = c0 + slot * V;
+            if (row >= live || c >= p.cols) continue;
+            float v[V];
+            Vec<T>::load(lds + at(lrow, slot), v);
+            T* o = out + row * p.out_ld + c;
+            if (vectors && c + V <= p.cols) {
+                if (sizeof(T) == 4 && p.add) {
+                    float w[V];
+                    Vec<T>::load(o, w);
+                    for (int e = 0; e < V; ++e) v[e] += w[e];
+                }
+                Vec<T>::store(o, v);
+            } else {
+                for (int e = 0; e < V; ++e)
+                    if (c + e < p.cols) o[e] = (T)(p.add ? (float)o[e] + v[e] : v[e]);
+            }
+        }
+        __syncthreads();
+    }
+}
+
 template <int BR, int BQ, int WR, int WQ, End END>
 __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
     constexpr int NT = 64 * WR * WQ;
@@ -231,6 +287,8 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave / WQ, wq = wave % WQ;
     const bool precise = p.pairs > 1;
+    // (read here: a load that is still out behind the end of a tile would be waited for in every stage of the next one)
+    const float f = END == STORE && p.scale ? __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(*p.scale))) : 1.f;
 
     // (whole-number division runs on the vector units: the results are told to be one for the wavefront, so that the operands'
     // descriptors stay in scalar registers)
@@ -535,53 +593,14 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
                     }
                 }
             }
-        } else if constexpr (END == ACCUM) {
-            float* out = static_cast<float*>(p.out) + (long long)t.split * ts.tiles_r * BR * p.out_ld;
-#pragma unroll
-            for (int j = 0; j < RI; ++j) {
-                const long long row = wr0 + j * 16 + fl;
-#pragma unroll
-                for (int i = 0; i < QI; ++i) {
-                    const long long c = wc0 + i * 16 + fk * 4;
-                    if (row >= live || c >= p.cols) continue;    // (out_ld is a multiple of 4)
-                    f32x4* o = reinterpret_cast<f32x4*>(out + row * p.out_ld + c);
-                    f32x4 x;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = value(i, j, e);
-                    if (p.add) x += *o;
-                    *o = x;
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
         } else {
-            const float f = p.scale ? *p.scale : 1.f;
-#pragma unroll
-            for (int j = 0; j < RI; ++j) {
-                const long long row = wr0 + j * 16 + fl;
-#pragma unroll
-                for (int i = 0; i < QI; ++i) {
-                    const long long c = wc0 + i * 16 + fk * 4;
-                    if (row >= p.r_rows || c >= p.cols) continue;
-                    f32x4 x;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = value(i, j, e) * f;
-                    if (p.out_bf16) {
-                        bf16_t* o = static_cast<bf16_t*>(p.out) + row * p.out_ld + c;
-                        if ((p.out_ld & 3) == 0) {
-                            bf16x4 q;
-                            for (int e = 0; e < 4; ++e) q[e] = (bf16_t)x[e];
-                            *reinterpret_cast<bf16x4*>(o) = q;
-                        } else {
-                            for (int e = 0; e < 4; ++e)
-                                if (c + e < p.cols) o[e] = (bf16_t)x[e];
-                        }
-                    } else {
-                        float* o = static_cast<float*>(p.out) + row * p.out_ld + c;
-                        for (int e = 0; e < 4; ++e)
-                            if (c + e < p.cols) o[e] = p.add ? o[e] + x[e] : x[e];
-                    }
-                }
-                __builtin_amdgcn_sched_barrier(0);
+            // Through LDS too, as many rows at a time as it holds: a wavefront then writes whole rows of the tile.  (From the
+            // registers it would write 32 or 64 bytes of sixteen rows at a time, at 1.6 TB/s.)
+            if (END == STORE && p.out_bf16) {
+                write_out<bf16_t, BR, BQ, WR, WQ>(scratch, static_cast<bf16_t*>(p.out), p, t.r0, t.c0, live, f, value);
+            } else {
+                float* out = static_cast<float*>(p.out) + (long long)t.split * ts.tiles_r * BR * p.out_ld;
+                write_out<float, BR, BQ, WR, WQ>(scratch, out, p, t.r0, t.c0, live, f, value);
             }
         }
     }
