@@ -18,6 +18,7 @@
 // own rounding: still more than twice the rate of the f32 matrix instructions.  bf16 operands need one product; there G is
 // rounded to bf16 (2^-9 of each value; sums stay in fp32), without its factor g where that is one number for all rows.
 #include "text_common.h"
+#include <type_traits>
 
 namespace {
 using namespace s2ag;
@@ -201,8 +202,9 @@ __device__ __forceinline__ float acc_read(float a) {
 __device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
 // exp(d): two terms of the argument's product with log2 e for fp32 operands, one for bf16 ones, whose logits carry more than that
-__device__ __forceinline__ float exp_of(float d, bool precise) {
-    if (!precise) return __expf(d);
+template <bool PRECISE>
+__device__ __forceinline__ float exp_of(float d) {
+    if constexpr (!PRECISE) return __expf(d);
     d = d < -150.f ? -150.f : d;                                 // (0 in fp32 either way; an infinity has no rest)
     const float t = d * 1.44269504088896340736f;
     const float rest = fmaf(d, 1.44269504088896340736f, -t) + d * 1.925963033500935e-8f;     // log2 e - its fp32 value
@@ -219,6 +221,15 @@ __host__ __device__ inline int splits_of(int tiles, int most, int slots) {      
     return s < 1 ? 1 : s > most ? most : s;
 }
 
+// f(0), f(STEP), ... below N, with the index as a constant: the accumulators are registers, which no loop can index.
+template <int I, int N, int STEP, typename F>
+__device__ __forceinline__ void each(F f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        each<I + STEP, N, STEP>(f);
+    }
+}
+
 // A tile of values to out[row][column], rows below `live` and columns below p.cols.
 template <typename T, int BR, int BQ, int WR, int WQ, typename F>
 __device__ __forceinline__ void write_out(bf16_t* scratch, T* out, const Product& p, long long r0, long long c0, int live, float f, F value) {
@@ -229,8 +240,8 @@ __device__ __forceinline__ void write_out(bf16_t* scratch, T* out, const Product
     const int lane = threadIdx.x & 63, fl = lane & 15, fk = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / WQ, wq = wave % WQ;
     const bool vectors = (p.out_ld % V == 0) && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-#pragma unroll
-    for (int jj = 0; jj < RI; jj += JS) {
+    each<0, RI, JS>([&](auto at_j) {
+        constexpr int jj = decltype(at_j)::value;
 #pragma unroll
         for (int j = jj; j < jj + JS; ++j) {
 #pragma unroll
@@ -272,10 +283,10 @@ __device__ __forceinline__ void write_out(bf16_t* scratch, T* out, const Product
             }
         }
         __syncthreads();
-    }
+    });
 }
 
-template <int BR, int BQ, int WR, int WQ, End END>
+template <int BR, int BQ, int WR, int WQ, End END, bool PRECISE>
 __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
     constexpr int NT = 64 * WR * WQ;
     constexpr int TR = BR / WR, TQ = BQ / WQ, RI = TR / 16, QI = TQ / 16;      // a wavefront's part
@@ -286,7 +297,7 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave / WQ, wq = wave % WQ;
-    const bool precise = p.pairs > 1;
+    constexpr int pairs = PRECISE ? 6 : 1;
     // (read here: a load that is still out behind the end of a tile would be waited for in every stage of the next one)
     const float f = END == STORE && p.scale ? __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(*p.scale))) : 1.f;
 
@@ -297,7 +308,7 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
     ts.tiles_r = __builtin_amdgcn_readfirstlane((live + BR - 1) / BR);
     ts.splits = __builtin_amdgcn_readfirstlane(splits_of(ts.tiles_r * p.tiles_q, p.splits, p.slots));
     ts.kt = p.k_count ? __builtin_amdgcn_readfirstlane((*p.k_count + BK - 1) / BK) : p.k / BK;
-    ts.total = ts.kt * p.pairs;
+    ts.total = ts.kt * pairs;
     ts.group = p.group;
     ts.per = p.group * p.tiles_q;
     ts.n = ts.tiles_r * p.tiles_q * ts.splits;
@@ -340,8 +351,8 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
     int r_bytes = 0, q_bytes = 0;
     __amdgpu_buffer_rsrc_t rr, qr;
     auto descriptors = [&]() {
-        rr = __builtin_amdgcn_make_buffer_rsrc((void*)(r_at + piece_r(precise ? pair : 5) * p.r.plane), 0, r_bytes, 0x00020000);
-        qr = __builtin_amdgcn_make_buffer_rsrc((void*)(q_at + piece_q(precise ? pair : 5) * p.q.plane), 0, q_bytes, 0x00020000);
+        rr = __builtin_amdgcn_make_buffer_rsrc((void*)(r_at + piece_r(PRECISE ? pair : 5) * p.r.plane), 0, r_bytes, 0x00020000);
+        qr = __builtin_amdgcn_make_buffer_rsrc((void*)(q_at + piece_q(PRECISE ? pair : 5) * p.q.plane), 0, q_bytes, 0x00020000);
     };
     auto next_tile = [&]() {
         r_bytes = q_bytes = 0;
@@ -475,10 +486,13 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
             const bool edge = p.q0 + t.c0 + BQ > p.vocab;
             if constexpr (END == STATS) {
                 float2* sm = reinterpret_cast<float2*>(scratch);     // [WQ][BR]
+                int tgt[RI];
+#pragma unroll
+                for (int j = 0; j < RI; ++j) tgt[j] = wr0 + j * 16 + fl < live ? p.tgt[wr0 + j * 16 + fl] : -1;
 #pragma unroll
                 for (int j = 0; j < RI; ++j) {
                     const int row = (int)wr0 + j * 16 + fl;
-                    const unsigned at = (unsigned)((row < live ? p.tgt[row] : -1) - word0);     // the target's place, if it is the lane's
+                    const unsigned at = (unsigned)(tgt[j] - word0);  // the target's place, if it is the lane's
                     float z[QI * 4], m4[4], s4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int i = 0; i < QI * 4; ++i) z[i] = value(i / 4, j, i % 4);
@@ -501,7 +515,7 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
                     m = fmaxf(m, __shfl_xor(m, 32));
                     const float ms = m == -INFINITY ? 0.f : m;   // a part that lies behind the vocabulary: a sum of 0
 #pragma unroll
-                    for (int i = 0; i < QI * 4; ++i) s4[i % 4] += exp_of(z[i] - ms, precise);
+                    for (int i = 0; i < QI * 4; ++i) s4[i % 4] += exp_of<PRECISE>(z[i] - ms);
                     float s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
                     s += __shfl_xor(s, 16);
                     s += __shfl_xor(s, 32);
@@ -524,37 +538,45 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
                 // are, columns by the transposing read.
                 constexpr int SLOTS = BQ / 8;
                 auto at = [](int row, int slot) { return row * BQ + ((slot ^ (row & 15)) << 3); };
-                const int pieces = precise ? 3 : 1;
-                for (int piece = 0; piece < pieces; ++piece) {   // (a piece is split off the value formed again: no registers for rests)
+                constexpr int pieces = PRECISE ? 3 : 1;
+                float lse[RI], fac[RI];
+                int tgt[RI];
 #pragma unroll
-                    for (int jj = 0; jj < RI; jj += 2) {
+                for (int j = 0; j < RI; ++j) {
+                    const long long row = wr0 + j * 16 + fl;
+                    const bool in = row < live;                  // (rows behind are zeros: a factor of 0 keeps them so)
+                    lse[j] = in ? p.lse[row] : 0.f;
+                    fac[j] = in ? (p.factor ? p.factor[row] : 1.f) : 0.f;
+                    tgt[j] = in ? p.tgt[row] : -1;
+                }
+                for (int piece = 0; piece < pieces; ++piece) {   // (a piece is split off the value formed again: no registers for rests)
+                    each<0, RI, 2>([&](auto at_j) {
+                        constexpr int jj = decltype(at_j)::value;
 #pragma unroll
                         for (int j = jj; j < jj + 2; ++j) {
-                            const int row = (int)wr0 + j * 16 + fl;
-                            const bool in = row < live;          // (rows behind are zeros: a factor of 0 keeps them so)
-                            const float lse = in ? p.lse[row] : 0.f, fac = in ? (p.factor ? p.factor[row] : 1.f) : 0.f;
-                            const unsigned tgt = (unsigned)((in ? p.tgt[row] : -1) - word0);
+                            const unsigned place = (unsigned)(tgt[j] - word0);       // the target's, if it is the lane's
+                            float g[QI * 4];
+#pragma unroll
+                            for (int i = 0; i < QI * 4; ++i) g[i] = exp_of<PRECISE>(value(i / 4, j, i % 4) - lse[j]);
+                            if (place < (unsigned)TQ) {
+#pragma unroll
+                                for (int i = 0; i < QI * 4; ++i)
+                                    if (place == (unsigned)(i / 4 * 16 + i % 4)) g[i] -= 1.f;
+                            }
+                            if (edge) {
+#pragma unroll
+                                for (int i = 0; i < QI * 4; ++i)
+                                    if (i / 4 * 16 + i % 4 >= words) g[i] = 0.f;
+                            }
 #pragma unroll
                             for (int i = 0; i < QI; ++i) {
-                                float g[4];
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) g[e] = exp_of(value(i, j, e) - lse, precise);
-                                if (tgt - i * 16 < 4u) {
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) g[e] -= tgt - i * 16 == (unsigned)e ? 1.f : 0.f;
-                                }
-                                if (edge) {
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e)
-                                        if (i * 16 + e >= words) g[e] = 0.f;
-                                }
                                 bf16x4 q;
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
-                                    g[e] *= fac;
-                                    q[e] = (bf16_t)g[e];
-                                    if (piece) {
-                                        const float rest = g[e] - (float)q[e];
+                                    const float v = g[i * 4 + e] * fac[j];
+                                    q[e] = (bf16_t)v;
+                                    if (PRECISE && piece) {
+                                        const float rest = v - (float)q[e];
                                         q[e] = (bf16_t)rest;
                                         if (piece == 2) q[e] = (bf16_t)(rest - (float)q[e]);
                                     }
@@ -590,7 +612,7 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
                                                            fk * 8) = q;
                             }
                         __syncthreads();
-                    }
+                    });
                 }
             }
         } else {
@@ -760,12 +782,12 @@ Plan plan(const s2ag_lce_args* a, bool backward) {
     return p;
 }
 
-template <int BR, int BQ, int WR, int WQ, End END>
+template <int BR, int BQ, int WR, int WQ, End END, bool PRECISE>
 int launch_tiles(Product& p, long long r_rows, long long q_rows, hipStream_t st) {
     constexpr int LDS = (2 * (BR + BQ) * BK + 64 * BQ) * 2, PER_CU = BR == 256 ? 1 : 2;
     static_assert(LDS * PER_CU <= 160 * 1024 && WR == 2 && 64 * BQ * 2 >= WQ * BR * 8, "the ends' scratch");
     // (every time: the attribute belongs to the current device)
-    if (hipFuncSetAttribute((const void*)product_k<BR, BQ, WR, WQ, END>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess)
+    if (hipFuncSetAttribute((const void*)product_k<BR, BQ, WR, WQ, END, PRECISE>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess)
         return S2AG_E_UNSUPPORTED;
     // The rows of R of a group stay in an XCD's 4 MB L2 while the columns pass, if half of it holds them (k of 1024: 4 row tiles
     // 816 TFLOP/s, 8 of them 560; of 2048: 2 row tiles 1023, 8 of them 841); where not two fit, the 8 x 4 tiles that run at a time
@@ -777,14 +799,16 @@ int launch_tiles(Product& p, long long r_rows, long long q_rows, hipStream_t st)
     if (p.splits < 1) p.splits = 1;
     if ((long long)cdiv(r_rows, BR) * p.tiles_q * p.splits > 0x3fffffffLL) return S2AG_E_UNSUPPORTED;
     if (r_rows == 0 || q_rows == 0) return 0;
-    hipLaunchKernelGGL((product_k<BR, BQ, WR, WQ, END>), dim3(p.slots), dim3(64 * WR * WQ), LDS, st, p);
+    hipLaunchKernelGGL((product_k<BR, BQ, WR, WQ, END, PRECISE>), dim3(p.slots), dim3(64 * WR * WQ), LDS, st, p);
     S2AG_LAUNCH_CHECK();
     return 0;
 }
 
 template <End END>
 int launch(Product& p, bool big, long long r_rows, long long q_rows, hipStream_t st) {
-    return big ? launch_tiles<256, 256, 2, 2, END>(p, r_rows, q_rows, st) : launch_tiles<128, 128, 2, 2, END>(p, r_rows, q_rows, st);
+    if (p.pairs > 1)
+        return big ? launch_tiles<256, 256, 2, 2, END, true>(p, r_rows, q_rows, st) : launch_tiles<128, 128, 2, 2, END, true>(p, r_rows, q_rows, st);
+    return big ? launch_tiles<256, 256, 2, 2, END, false>(p, r_rows, q_rows, st) : launch_tiles<128, 128, 2, 2, END, false>(p, r_rows, q_rows, st);
 }
 
 unsigned grid_of(long long work) {
