@@ -156,7 +156,9 @@ __global__ __launch_bounds__(256) void scale_k(Table t, const double* __restrict
     f = f > 1.f ? 1.f : f;                                        // (NaN stays NaN)
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
     const unsigned chunks = t.first[t.tensors];
-    for (unsigned c = blockIdx.x; c < chunks; c += gridDim.x) {
+    // backwards: what the norm read last is still in the memory-side cache
+    for (unsigned i = blockIdx.x; i < chunks; i += gridDim.x) {
+        const unsigned c = chunks - 1 - i;
         const int k = tensor_of(t, c);
         if (!t.dst[k] || (f == 1.f && t.dst[k] == t.src[k])) continue;
         const long long off = (long long)(c - t.first[k]) * CHUNK, left = (t.n[k] & COUNT) - off;
@@ -212,7 +214,7 @@ int run(const s2ag_clip_tensor* a, int tensors, float max_norm, double* partials
         count = 1;
     }
     float* out = norm;
-    at = 0;
+    at = tensors > 0 ? (tensors - 1) / GROUP * GROUP : 0;
     do {
         const unsigned chunks = fill(t, a, at, tensors);
         bool any = out != nullptr;
@@ -226,8 +228,8 @@ int run(const s2ag_clip_tensor* a, int tensors, float max_norm, double* partials
             S2AG_LAUNCH_CHECK();
         }
         out = nullptr;
-        at += GROUP;
-    } while (at < tensors);
+        at -= GROUP;
+    } while (at >= 0);
     return 0;
 }
 }  // namespace

@@ -17,25 +17,33 @@ using namespace s2ag;
 using namespace s2ag::text;
 
 // ---- lookup ----------------------------------------------------------------------------------------------------------------
-// A row is read by 2^tx_log lanes, 16 bytes each where every row starts at a multiple of 16 bytes.
-template <typename T, bool ALIGNED>
+// A row is read by 2^tx_log lanes, 16 bytes each, four rows in flight: with one, a workgroup waits for an id and then for a row
+// for every 4 KB that it writes.
+template <typename T>
 __global__ __launch_bounds__(256) void lookup_k(const void* __restrict__ ids, int ids_i32, const T* __restrict__ table, long long n,
                                                 int dim, long long n_entries, float scale, T* __restrict__ out, int tx_log) {
-    constexpr int V = ALIGNED ? Vec<T>::N : 1;
+    constexpr int V = Vec<T>::N, R = 4;
     const int tx = threadIdx.x & ((1 << tx_log) - 1), ty = threadIdx.x >> tx_log, rows = 256 >> tx_log;
-    for (long long r = (long long)blockIdx.x * rows + ty; r < n; r += (long long)gridDim.x * rows) {
-        const long long id = load_id(ids, ids_i32, r);
-        const bool in = id >= 0 && id < n_entries;
-        const T* src = table + (in ? id : 0) * dim;
-        T* dst = out + r * dim;
+    for (long long r0 = (long long)blockIdx.x * rows * R + ty; r0 < n; r0 += (long long)gridDim.x * rows * R) {
+        const T* src[R];
+        bool in[R];
+        for (int u = 0; u < R; ++u) {
+            const long long r = r0 + u * rows, id = r < n ? load_id(ids, ids_i32, r) : -1;
+            in[u] = id >= 0 && id < n_entries;
+            src[u] = table + (in[u] ? id : 0) * dim;
+        }
         for (int c = tx * V; c < dim; c += V << tx_log) {
-            if constexpr (ALIGNED) {
-                float v[V];
-                Vec<T>::load(src + c, v);
-                for (int j = 0; j < V; ++j) v[j] = in ? v[j] * scale : 0.f;
-                Vec<T>::store(dst + c, v);
+            if (c + V <= dim) {
+                float v[R][V];
+                for (int u = 0; u < R; ++u) Vec<T>::load_any(src[u] + c, v[u]);
+                for (int u = 0; u < R; ++u) {
+                    for (int j = 0; j < V; ++j) v[u][j] = in[u] ? v[u][j] * scale : 0.f;
+                    if (r0 + u * rows < n) Vec<T>::store_any(out + (r0 + u * rows) * dim + c, v[u]);
+                }
             } else {
-                dst[c] = in ? (T)((float)src[c] * scale) : (T)0.f;
+                for (int u = 0; u < R; ++u)
+                    for (int j = c; j < dim; ++j)
+                        if (r0 + u * rows < n) out[(r0 + u * rows) * dim + j] = in[u] ? (T)((float)src[u][j] * scale) : (T)0.f;
             }
         }
     }
@@ -71,18 +79,19 @@ __device__ __forceinline__ unsigned key_of(const void* ids, int ids_i32, long lo
 // Up to SMALL positions: one workgroup sorts them in LDS, 8 bits a pass.  Items go by wavefront, round and lane, which is their
 // order; a wavefront counts its items per digit while it ranks them, so that a pass reads its items once.
 constexpr int SMALL = 8192;
-constexpr int SB = 8, SBINS = 1 << SB, SWAVES = 16, SROUNDS = SMALL / 1024;
+constexpr int SB = 8, SBINS = 1 << SB, SWAVES = 16;
+template <int SROUNDS>
 __global__ __launch_bounds__(1024) void sort_small_k(const void* __restrict__ ids, int ids_i32, int n, long long n_entries,
                                                      long long padding_idx, int passes, int clear_flags,
                                                      unsigned* __restrict__ keys, int* __restrict__ pos,
                                                      unsigned char* __restrict__ touched) {
-    __shared__ unsigned k_s[SMALL];
-    __shared__ unsigned short p_s[SMALL];
+    __shared__ unsigned k_s[SROUNDS * 1024];
+    __shared__ unsigned short p_s[SROUNDS * 1024];
     __shared__ unsigned short cnt[SWAVES][SBINS];
     __shared__ int base[SBINS];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     if (touched && clear_flags)
-        for (long long i = tid; i < n_entries; i += 1024) touched[i] = 0;
+        for (long long i = tid; i < (n_entries + 15) / 16; i += 1024) reinterpret_cast<u32x4*>(touched)[i] = u32x4{0, 0, 0, 0};      // (padded)
     const int items = wave * (SROUNDS * 64) + lane;
     unsigned key[SROUNDS];
     int at[SROUNDS], rank[SROUNDS];
@@ -152,9 +161,9 @@ __global__ __launch_bounds__(1024) void sort_small_k(const void* __restrict__ id
     }
 }
 
-// More: per pass of LB bits one launch counts the digits of every tile of LTILE items, one adds the counts up over the tiles
-// (a workgroup per digit), one moves the items.
-constexpr int LB = 9, LBINS = 1 << LB, LTILE = 4096, LWAVES = 4, LROUNDS = LTILE / 256;
+// More: per pass of LB bits one launch counts the digits of every tile of LTILE items and one moves the items.  Up to DIRECT
+// tiles the second adds the counts of the tiles itself; more are added up by a launch between the two (a workgroup per digit).
+constexpr int LB = 9, LBINS = 1 << LB, LTILE = 2048, LWAVES = 4, LROUNDS = LTILE / 256, DIRECT = 64;
 struct SortIn {
     const void* ids;                    // first pass: the keys come from the ids, the positions count up
     int ids_i32;
@@ -166,18 +175,29 @@ struct SortIn {
 __device__ __forceinline__ unsigned sort_key(const SortIn& in, int i) {
     return in.ids ? key_of(in.ids, in.ids_i32, i, in.n_entries, in.padding_idx) : in.keys[i];
 }
+// counts: [tile][digit] for the direct sums, [digit][tile] for the launch between
+__device__ __forceinline__ long long count_at(int tile, int digit, int tiles) {
+    return tiles <= DIRECT ? (long long)tile * LBINS + digit : (long long)digit * tiles + tile;
+}
 
-__global__ __launch_bounds__(256) void sort_count_k(SortIn in, int shift, int tiles, int* __restrict__ counts) {
+__global__ __launch_bounds__(256) void sort_count_k(SortIn in, int shift, int tiles, int* __restrict__ counts,
+                                                    unsigned char* __restrict__ clear) {
     __shared__ int c[LBINS];
+    if (clear)                                                   // the flags that the last pass sets (padded to 16)
+        for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (in.n_entries + 15) / 16; i += (long long)gridDim.x * 256)
+            reinterpret_cast<u32x4*>(clear)[i] = u32x4{0, 0, 0, 0};
     for (int i = threadIdx.x; i < LBINS; i += 256) c[i] = 0;
     __syncthreads();
     const int t0 = blockIdx.x * LTILE;
+    unsigned key[LROUNDS];
     for (int r = 0; r < LROUNDS; ++r) {
         const int i = t0 + r * 256 + threadIdx.x;
-        if (i < in.n) atomicAdd(&c[(sort_key(in, i) >> shift) & (LBINS - 1)], 1);     // (whole numbers: any order, one sum)
+        key[r] = i < in.n ? sort_key(in, i) : 0u;
     }
+    for (int r = 0; r < LROUNDS; ++r)
+        if (t0 + r * 256 + (int)threadIdx.x < in.n) atomicAdd(&c[(key[r] >> shift) & (LBINS - 1)], 1);     // (whole numbers: any order, one sum)
     __syncthreads();
-    for (int i = threadIdx.x; i < LBINS; i += 256) counts[(long long)i * tiles + blockIdx.x] = c[i];
+    for (int i = threadIdx.x; i < LBINS; i += 256) counts[count_at(blockIdx.x, i, tiles)] = c[i];
 }
 
 __global__ __launch_bounds__(256) void sort_scan_k(int tiles, int* __restrict__ counts, int* __restrict__ totals) {
@@ -207,28 +227,42 @@ __global__ __launch_bounds__(256) void sort_move_k(SortIn in, int shift, int til
     __shared__ unsigned short cnt[LWAVES][LBINS];
     __shared__ int base[LBINS];
     __shared__ int sm[LWAVES];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (int i = tid; i < LWAVES * LBINS; i += 256) (&cnt[0][0])[i] = 0;
-    // where each digit's items of this tile begin: totals of the lower digits, counts of the tiles before
-    {
-        const int a = totals[2 * tid], b = totals[2 * tid + 1];
-        const int inc = wave_scan(a + b, lane);
-        if (lane == 63) sm[wave] = inc;
-        __syncthreads();
-        int e = inc - a - b;
-        for (int w = 0; w < wave; ++w) e += sm[w];
-        base[2 * tid] = e + counts[(long long)(2 * tid) * tiles + blockIdx.x];
-        base[2 * tid + 1] = e + a + counts[(long long)(2 * tid + 1) * tiles + blockIdx.x];
-    }
-    const int first = blockIdx.x * LTILE + wave * (LROUNDS * 64) + lane;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, me = blockIdx.x;
+    const int first = me * LTILE + wave * (LROUNDS * 64) + lane;
     unsigned key[LROUNDS];
-    int rank[LROUNDS];
+    int at[LROUNDS], rank[LROUNDS];
     for (int r = 0; r < LROUNDS; ++r) {
         const int i = first + r * 64;
         key[r] = i < in.n ? sort_key(in, i) : ~0u;
+        at[r] = in.ids || i >= in.n ? i : in.pos[i];
     }
-    __syncthreads();
-    for (int r = 0; r < LROUNDS; ++r) {
+    for (int i = tid; i < LWAVES * LBINS; i += 256) (&cnt[0][0])[i] = 0;
+    // where each digit's items of this tile begin: totals of the lower digits, counts of the tiles before
+    {
+        int total[2] = {0, 0}, before[2] = {0, 0};
+        if (tiles <= DIRECT) {
+#pragma unroll 8
+            for (int t = 0; t < tiles; ++t)
+                for (int h = 0; h < 2; ++h) {
+                    const int c = counts[(long long)t * LBINS + 2 * tid + h];
+                    total[h] += c;
+                    if (t < me) before[h] += c;
+                }
+        } else {
+            for (int h = 0; h < 2; ++h) {
+                total[h] = totals[2 * tid + h];
+                before[h] = counts[count_at(me, 2 * tid + h, tiles)];
+            }
+        }
+        const int inc = wave_scan(total[0] + total[1], lane);
+        if (lane == 63) sm[wave] = inc;
+        __syncthreads();
+        int e = inc - total[0] - total[1];
+        for (int w = 0; w < wave; ++w) e += sm[w];
+        base[2 * tid] = e + before[0];
+        base[2 * tid + 1] = e + total[0] + before[1];
+    }
+    for (int r = 0; r < LROUNDS; ++r) {                          // (a wavefront's counters are its own)
         const unsigned d = (key[r] >> shift) & (LBINS - 1);
         int total;
         const int low = lower_peers<LB>(d, lane, &total);
@@ -249,12 +283,11 @@ __global__ __launch_bounds__(256) void sort_move_k(SortIn in, int shift, int til
     }
     __syncthreads();
     for (int r = 0; r < LROUNDS; ++r) {
-        const int i = first + r * 64;
-        if (i < in.n) {                                          // (the items behind the last rank behind all others: no gap)
+        if (first + r * 64 < in.n) {                             // (the items behind the last rank behind all others: no gap)
             const unsigned d = (key[r] >> shift) & (LBINS - 1);
             const int to = base[d] + cnt[wave][d] + rank[r];
             keys_out[to] = key[r];
-            pos_out[to] = in.ids ? i : in.pos[i];
+            pos_out[to] = at[r];
             if (touched && key[r] < (unsigned)in.n_entries) touched[key[r]] = 1;
         }
     }
@@ -263,41 +296,40 @@ __global__ __launch_bounds__(256) void sort_move_k(SortIn in, int shift, int til
 // ---- sums ------------------------------------------------------------------------------------------------------------------
 constexpr int UNROLL = 8;               // rows in flight per wavefront: 8 KB, 128 KB on a compute unit with 16 wavefronts
 
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ int column(int chunk, int lane, int j) {
+// A lane's V columns of a row: one 16-byte access at any alignment, element by element at the row's end.
+template <typename T>
+__device__ __forceinline__ void load_cols(const T* row, int c, int dim, float* v) {
     constexpr int V = Vec<T>::N;
-    return chunk * 64 * V + (ALIGNED ? lane * V + j : j * 64 + lane);
-}
-
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ void load_cols(const T* row, int chunk, int lane, int dim, float* v) {
-    constexpr int V = Vec<T>::N;
-    if constexpr (ALIGNED) {
-        const int c = column<T, true>(chunk, lane, 0);
-        if (c < dim) Vec<T>::load(row + c, v);
+    if (c + V <= dim) {
+        Vec<T>::load_any(row + c, v);
     } else {
-        for (int j = 0; j < V; ++j) {
-            const int c = column<T, false>(chunk, lane, j);
-            v[j] = c < dim ? (float)row[c] : 0.f;
-        }
+        for (int j = 0; j < V; ++j) v[j] = c + j < dim ? (float)row[c + j] : 0.f;
     }
 }
 
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ void write_row(T* row, int chunk, int lane, int dim, const float* acc, float scale, int accumulate) {
+template <typename T>
+__device__ __forceinline__ void write_cols(T* row, int c, int dim, const float* acc, float scale, int accumulate) {
     constexpr int V = Vec<T>::N;
     float v[V];
-    if (accumulate) load_cols<T, ALIGNED>(row, chunk, lane, dim, v);
+    if (accumulate) load_cols<T>(row, c, dim, v);
     for (int j = 0; j < V; ++j) v[j] = accumulate ? v[j] + scale * acc[j] : scale * acc[j];
-    if constexpr (ALIGNED) {
-        const int c = column<T, true>(chunk, lane, 0);
-        if (c < dim) Vec<T>::store(row + c, v);
+    if (c + V <= dim) {
+        Vec<T>::store_any(row + c, v);
     } else {
-        for (int j = 0; j < V; ++j) {
-            const int c = column<T, false>(chunk, lane, j);
-            if (c < dim) row[c] = (T)v[j];
-        }
+        for (int j = 0; j < V; ++j)
+            if (c + j < dim) row[c + j] = (T)v[j];
     }
+}
+
+// A wavefront writes zeros to n elements: rows that follow each other are one piece of memory.
+template <typename T>
+__device__ __forceinline__ void write_zeros(T* p, long long n, int lane) {
+    constexpr int V = Vec<T>::N;
+    const long long head = min((long long)(((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T)), n), body = (n - head) / V;
+    if (lane < head) p[lane] = (T)0.f;
+    u32x4* q = reinterpret_cast<u32x4*>(p + head);
+    for (long long i = lane; i < body; i += 64) q[i] = u32x4{0, 0, 0, 0};
+    if (lane < n - head - body * V) p[head + body * V + lane] = (T)0.f;
 }
 
 // pieces of the runs that cross a border: [tile][0: began before the tile, 1: goes on behind it][chunk][j][lane]
@@ -306,19 +338,25 @@ __device__ __forceinline__ float* piece(float* pieces, int tile, int which, int 
     return pieces + (((long long)tile * 2 + which) * chunks + chunk) * (64 * V);
 }
 
-template <typename T, bool ALIGNED>
+template <typename T>
 __global__ __launch_bounds__(256) void sum_k(const unsigned* __restrict__ keys, const int* __restrict__ pos, int n,
                                              const T* __restrict__ dy, long long ldy, int dim, long long n_entries, float scale,
                                              T* __restrict__ dtable, int accumulate, int tile_len, int tiles, int chunks,
-                                             float* __restrict__ pieces, const unsigned char* __restrict__ touched, int sum_blocks) {
+                                             float* __restrict__ pieces, const unsigned char* __restrict__ touched, int sum_blocks,
+                                             int zero_rows) {
     constexpr int V = Vec<T>::N;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if ((int)blockIdx.x >= sum_blocks) {                          // rows without an id
-        const float zero[V] = {};
-        const long long step = (long long)(gridDim.x - sum_blocks) * 4;
-        for (long long v = (long long)(blockIdx.x - sum_blocks) * 4 + wave; v < n_entries; v += step)
-            if (!touched[v])
-                for (int c = 0; c < chunks; ++c) write_row<T, ALIGNED>(dtable + v * dim, c, lane, dim, zero, 0.f, 0);
+    if ((int)blockIdx.x >= sum_blocks) {                          // rows without an id, zero_rows to a wavefront
+        const long long v0 = ((long long)(blockIdx.x - sum_blocks) * 4 + wave) * zero_rows;
+        const bool mine = lane < zero_rows && v0 + lane < n_entries && !touched[v0 + lane];
+        unsigned long long left = __ballot(mine);
+        while (left) {
+            const int at = __ffsll(left) - 1;
+            const unsigned long long rest = ~(left >> at);
+            const int run = rest ? __ffsll(rest) - 1 : 64;
+            write_zeros<T>(dtable + (v0 + at) * dim, (long long)run * dim, lane);
+            left = at + run >= 64 ? 0 : left & ~(((1ULL << run) - 1) << at);
+        }
         return;
     }
     const long long item = (long long)blockIdx.x * 4 + wave;
@@ -331,6 +369,7 @@ __global__ __launch_bounds__(256) void sum_k(const unsigned* __restrict__ keys, 
     if (cnt == 0) return;
     unsigned cur = (unsigned)__builtin_amdgcn_readlane((int)key_l, 0);
     bool head = t0 > 0 && keys[t0 - 1] == cur;
+    const int c = (chunk * 64 + lane) * V;
     float acc[V];
     for (int j = 0; j < V; ++j) acc[j] = 0.f;
     auto leave = [&](int which) {
@@ -340,31 +379,34 @@ __global__ __launch_bounds__(256) void sum_k(const unsigned* __restrict__ keys, 
     for (int j0 = 0; j0 < cnt; j0 += UNROLL) {
         float v[UNROLL][V];
         unsigned k[UNROLL];
+#pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
             const int i = min(j0 + u, cnt - 1);
-            k[u] = j0 + u < cnt ? (unsigned)__builtin_amdgcn_readlane((int)key_l, i) : ~0u;
+            k[u] = (unsigned)__builtin_amdgcn_readlane((int)key_l, i);
             const int p = __builtin_amdgcn_readlane(pos_l, i);
-            load_cols<T, ALIGNED>(dy + (long long)p * ldy, chunk, lane, dim, v[u]);
+            load_cols<T>(dy + (long long)p * ldy, c, dim, v[u]);
         }
+#pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
-            if (j0 + u >= cnt) break;
-            if (k[u] != cur) {
-                if (head) leave(0);
-                else write_row<T, ALIGNED>(dtable + (long long)cur * dim, chunk, lane, dim, acc, scale, accumulate);
-                cur = k[u];
-                head = false;
-                for (int j = 0; j < V; ++j) acc[j] = 0.f;
+            if (j0 + u < cnt) {
+                if (k[u] != cur) {
+                    if (head) leave(0);
+                    else write_cols<T>(dtable + (long long)cur * dim, c, dim, acc, scale, accumulate);
+                    cur = k[u];
+                    head = false;
+                    for (int j = 0; j < V; ++j) acc[j] = 0.f;
+                }
+                for (int j = 0; j < V; ++j) acc[j] += v[u][j];
             }
-            for (int j = 0; j < V; ++j) acc[j] += v[u][j];
         }
     }
     if (head) leave(0);
     else if (t0 + cnt < n && keys[t0 + cnt] == cur) leave(1);
-    else write_row<T, ALIGNED>(dtable + (long long)cur * dim, chunk, lane, dim, acc, scale, accumulate);
+    else write_cols<T>(dtable + (long long)cur * dim, c, dim, acc, scale, accumulate);
 }
 
 // A workgroup per (tile, chunk) that a crossing run begins in: eight wavefronts add every eighth piece, then each other's sums.
-template <typename T, bool ALIGNED>
+template <typename T>
 __global__ __launch_bounds__(512) void join_k(const unsigned* __restrict__ keys, int n, int dim, long long n_entries, float scale,
                                               T* __restrict__ dtable, int accumulate, int tile_len, int chunks,
                                               float* __restrict__ pieces) {
@@ -386,6 +428,7 @@ __global__ __launch_bounds__(512) void join_k(const unsigned* __restrict__ keys,
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float acc[V];
     for (int j = 0; j < V; ++j) acc[j] = 0.f;
+#pragma unroll 4
     for (int t = tile + wave; t <= last; t += 8) {
         const float* q = piece<V>(pieces, t, t == tile ? 1 : 0, chunk, chunks);
         for (int j = 0; j < V; ++j) acc[j] += q[j * 64 + lane];
@@ -395,7 +438,7 @@ __global__ __launch_bounds__(512) void join_k(const unsigned* __restrict__ keys,
     if (wave == 0) {
         for (int w = 1; w < 8; ++w)
             for (int j = 0; j < V; ++j) acc[j] += sm[w][j * 64 + lane];
-        write_row<T, ALIGNED>(dtable + (long long)cur * dim, chunk, lane, dim, acc, scale, accumulate);
+        write_cols<T>(dtable + (long long)cur * dim, (chunk * 64 + lane) * V, dim, acc, scale, accumulate);
     }
 }
 
@@ -422,7 +465,7 @@ Layout layout(long long n, int dim, long long n_entries) {
     l.counts = take(small ? 0 : 4 * LBINS * tiles);
     l.totals = take(4 * LBINS);
     l.pieces = take(4 * 2 * cols * cdiv(n, tile_len_of(n)));
-    l.touched = take(n_entries);
+    l.touched = take(n_entries);        // (a multiple of 256: cleared in 16-byte steps)
     l.bytes = at;
     return l;
 }
@@ -431,22 +474,21 @@ bool valid_sizes(long long n, int dim, long long n_entries) {
     return n >= 0 && n < (1LL << 31) - 65536 && dim > 0 && dim <= (1 << 24) && n_entries > 0 && n_entries < (1LL << 30);
 }
 
-template <typename T, bool ALIGNED>
+template <typename T>
 int launch_sums(const unsigned* keys, const int* pos, int n, const void* dy, long long ldy, int dim, long long n_entries, float scale,
                 void* dtable, int accumulate, float* pieces, const unsigned char* touched, hipStream_t st) {
     const int tl = tile_len_of(n), tiles = cdiv(n, tl), chunks = cdiv(dim, 64 * Vec<T>::N);
     const long long blocks = ((long long)tiles * chunks + 3) / 4;
-    if (blocks + 4096 > 0x7fffffffLL) return S2AG_E_UNSUPPORTED;
-    long long zero = 0;
-    if (touched) zero = n_entries / 4 + 1 < 4096 ? n_entries / 4 + 1 : 4096;
+    const int zero_rows = n_entries < 65536 ? 16 : 64;            // a small table: more wavefronts
+    const long long zero = touched ? (n_entries + 4 * zero_rows - 1) / (4 * zero_rows) : 0;
+    if (blocks + zero > 0x7fffffffLL) return S2AG_E_UNSUPPORTED;
     if (blocks + zero)
-        hipLaunchKernelGGL((sum_k<T, ALIGNED>), dim3((unsigned)(blocks + zero)), dim3(256), 0, st, keys, pos, n,
-                           static_cast<const T*>(dy), ldy, dim, n_entries, scale, static_cast<T*>(dtable), accumulate, tl, tiles,
-                           chunks, pieces, touched, (int)blocks);
+        hipLaunchKernelGGL(sum_k<T>, dim3((unsigned)(blocks + zero)), dim3(256), 0, st, keys, pos, n, static_cast<const T*>(dy), ldy, dim,
+                           n_entries, scale, static_cast<T*>(dtable), accumulate, tl, tiles, chunks, pieces, touched, (int)blocks, zero_rows);
     S2AG_LAUNCH_CHECK();
     if (tiles > 1) {
-        hipLaunchKernelGGL((join_k<T, ALIGNED>), dim3((unsigned)((long long)(tiles - 1) * chunks)), dim3(512), 0, st, keys, n, dim, n_entries,
-                           scale, static_cast<T*>(dtable), accumulate, tl, chunks, pieces);
+        hipLaunchKernelGGL(join_k<T>, dim3((unsigned)((long long)(tiles - 1) * chunks)), dim3(512), 0, st, keys, n, dim, n_entries, scale,
+                           static_cast<T*>(dtable), accumulate, tl, chunks, pieces);
         S2AG_LAUNCH_CHECK();
     }
     return 0;
@@ -455,20 +497,14 @@ int launch_sums(const unsigned* keys, const int* pos, int n, const void* dy, lon
 template <typename T>
 int launch_lookup(const void* ids, int ids_i32, const void* table, long long n, int dim, long long n_entries, float scale, void* out,
                   hipStream_t st) {
-    constexpr int V = Vec<T>::N;
-    const bool al = dim % V == 0 && aligned16(table) && aligned16(out);
-    const int per_row = al ? dim / V : dim;
+    const int per_row = cdiv(dim, Vec<T>::N);
     int tx = 0;
     while (tx < 8 && (1 << tx) < per_row) ++tx;
-    const long long rows = 256 >> tx;
+    const long long rows = 4 * (256 >> tx);
     long long blocks = (n + rows - 1) / rows;
-    if (blocks > 8192) blocks = 8192;
-    if (al)
-        hipLaunchKernelGGL((lookup_k<T, true>), dim3((unsigned)blocks), dim3(256), 0, st, ids, ids_i32, static_cast<const T*>(table), n, dim,
-                           n_entries, scale, static_cast<T*>(out), tx);
-    else
-        hipLaunchKernelGGL((lookup_k<T, false>), dim3((unsigned)blocks), dim3(256), 0, st, ids, ids_i32, static_cast<const T*>(table), n, dim,
-                           n_entries, scale, static_cast<T*>(out), tx);
+    if (blocks > (1 << 20)) blocks = 1 << 20;
+    hipLaunchKernelGGL(lookup_k<T>, dim3((unsigned)blocks), dim3(256), 0, st, ids, ids_i32, static_cast<const T*>(table), n, dim, n_entries,
+                       scale, static_cast<T*>(out), tx);
     S2AG_LAUNCH_CHECK();
     return 0;
 }
@@ -502,12 +538,19 @@ extern "C" int s2ag_emb_grad(const void* ids, int ids_i32, const void* dy, long 
     int bits = 1;
     while ((n_entries >> bits) != 0) ++bits;                       // the keys 0 .. n_entries
     const bool small = n <= SMALL;
-    const bool clear_inside = small && n > 0 && n_entries <= 131072;
+    const bool clear_inside = n > 0 && (!small || n_entries <= 131072);        // by the sort's first launch
     if (touched && !clear_inside)
         if (hipError_t e = zero_async(touched, (size_t)round_up(n_entries, 4), st)) return (int)e;
     if (n > 0 && small) {
-        hipLaunchKernelGGL(sort_small_k, dim3(1), dim3(1024), 0, st, ids, ids_i32, (int)n, n_entries, padding_idx, cdiv(bits, SB),
-                           (int)clear_inside, keys, pos, touched);
+#define S2AG_SORT(R) \
+    hipLaunchKernelGGL(sort_small_k<R>, dim3(1), dim3(1024), 0, st, ids, ids_i32, (int)n, n_entries, padding_idx, cdiv(bits, SB), \
+                       (int)clear_inside, keys, pos, touched)
+        if (n <= 1024) S2AG_SORT(1);
+        else if (n <= 2048) S2AG_SORT(2);
+        else if (n <= 4096) S2AG_SORT(4);
+        else if (n <= 6144) S2AG_SORT(6);
+        else S2AG_SORT(8);
+#undef S2AG_SORT
         S2AG_LAUNCH_CHECK();
     } else if (n > 0) {
         const int tiles = cdiv(n, LTILE), passes = cdiv(bits, LB);
@@ -518,10 +561,12 @@ extern "C" int s2ag_emb_grad(const void* ids, int ids_i32, const void* dy, long 
             const int to = (passes - 1 - p) & 1;                   // the last pass ends in the first pair of buffers
             unsigned* ko = reinterpret_cast<unsigned*>(ws + l.keys[to]);
             int* po = reinterpret_cast<int*>(ws + l.pos[to]);
-            hipLaunchKernelGGL(sort_count_k, dim3(tiles), dim3(256), 0, st, in, p * LB, tiles, counts);
+            hipLaunchKernelGGL(sort_count_k, dim3(tiles), dim3(256), 0, st, in, p * LB, tiles, counts, p == 0 ? touched : nullptr);
             S2AG_LAUNCH_CHECK();
-            hipLaunchKernelGGL(sort_scan_k, dim3(LBINS), dim3(256), 0, st, tiles, counts, totals);
-            S2AG_LAUNCH_CHECK();
+            if (tiles > DIRECT) {
+                hipLaunchKernelGGL(sort_scan_k, dim3(LBINS), dim3(256), 0, st, tiles, counts, totals);
+                S2AG_LAUNCH_CHECK();
+            }
             hipLaunchKernelGGL(sort_move_k, dim3(tiles), dim3(256), 0, st, in, p * LB, tiles, counts, totals, ko, po,
                                p == passes - 1 ? touched : nullptr);
             S2AG_LAUNCH_CHECK();
@@ -531,10 +576,6 @@ extern "C" int s2ag_emb_grad(const void* ids, int ids_i32, const void* dy, long 
         }
     }
     float* pieces = reinterpret_cast<float*>(ws + l.pieces);
-    const int V = bf16 ? 8 : 4;
-    const bool al = dim % V == 0 && ldy % V == 0 && aligned16(dy) && aligned16(dtable);
-#define S2AG_SUMS(T, AL) launch_sums<T, AL>(keys, pos, (int)n, dy, ldy, dim, n_entries, scale, dtable, accumulate, pieces, touched, st)
-    if (bf16) return al ? S2AG_SUMS(bf16_t, true) : S2AG_SUMS(bf16_t, false);
-    return al ? S2AG_SUMS(float, true) : S2AG_SUMS(float, false);
-#undef S2AG_SUMS
+    return bf16 ? launch_sums<bf16_t>(keys, pos, (int)n, dy, ldy, dim, n_entries, scale, dtable, accumulate, pieces, touched, st)
+                : launch_sums<float>(keys, pos, (int)n, dy, ldy, dim, n_entries, scale, dtable, accumulate, pieces, touched, st);
 }

@@ -13,17 +13,29 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 // The elements that 16 bytes hold, widened to fp32 (exact) and rounded back (to nearest even, the one rounding of a result).
+// `_any`: at any multiple of the element's size; one 16-byte access all the same.
+typedef bf16x8 bf16x8_any __attribute__((aligned(2)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
 template <typename T> struct Vec;
 template <> struct Vec<float> {
     static constexpr int N = 4;
     static __device__ __forceinline__ void load(const float* p, float* v) {
         const f32x4 q = *reinterpret_cast<const f32x4*>(p);
-        for (int i = 0; i < 4; ++i) v[i] = q[i];
+        for (int i = 0; i < 4; ++i) v[i] = (float)q[i];
     }
     static __device__ __forceinline__ void store(float* p, const float* v) {
         f32x4 q;
-        for (int i = 0; i < 4; ++i) q[i] = v[i];
+        for (int i = 0; i < 4; ++i) q[i] = (float)v[i];
         *reinterpret_cast<f32x4*>(p) = q;
+    }
+    static __device__ __forceinline__ void load_any(const float* p, float* v) {
+        const f32x4 q = *reinterpret_cast<const f32x4_any*>(p);
+        for (int i = 0; i < 4; ++i) v[i] = (float)q[i];
+    }
+    static __device__ __forceinline__ void store_any(float* p, const float* v) {
+        f32x4 q;
+        for (int i = 0; i < 4; ++i) q[i] = (float)v[i];
+        *reinterpret_cast<f32x4_any*>(p) = q;
     }
 };
 template <> struct Vec<bf16_t> {
@@ -36,6 +48,15 @@ template <> struct Vec<bf16_t> {
         bf16x8 q;
         for (int i = 0; i < 8; ++i) q[i] = (bf16_t)v[i];
         *reinterpret_cast<bf16x8*>(p) = q;
+    }
+    static __device__ __forceinline__ void load_any(const bf16_t* p, float* v) {
+        const bf16x8 q = *reinterpret_cast<const bf16x8_any*>(p);
+        for (int i = 0; i < 8; ++i) v[i] = (float)q[i];
+    }
+    static __device__ __forceinline__ void store_any(bf16_t* p, const float* v) {
+        bf16x8 q;
+        for (int i = 0; i < 8; ++i) q[i] = (bf16_t)v[i];
+        *reinterpret_cast<bf16x8_any*>(p) = q;
     }
 };
 

@@ -6,7 +6,9 @@ kernel launch per optimizer (s2ag_adam_step), and the data-parallel gradient exc
 all-reduce over the arena (parallel.py) instead of one collective per tensor.
 """
 import ctypes as C
+import itertools
 import math
+import operator
 from typing import Iterable, List, Optional, Sequence, Union
 
 import torch
@@ -101,6 +103,8 @@ class FusedAdam:
 
 
 _CLIP_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+_CLIP_BYTES = (4, 2)
+_DEVICE, _DTYPE = operator.attrgetter('device'), operator.attrgetter('dtype')
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -134,48 +138,43 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float 
         raise ValueError(f'clip_grads: max_norm must not be negative, got {max_norm}')
     if not grads:
         raise ValueError('clip_grads: no gradients')
+    results = grads
     if out is not None:
-        out = list(out)
-        if len(out) != len(grads):
-            raise ValueError(f'clip_grads: {len(grads)} gradients and {len(out)} outputs')
+        results = list(out)
+        if len(results) != len(grads):
+            raise ValueError(f'clip_grads: {len(grads)} gradients and {len(results)} outputs')
+    # (whole lists at a time: a call is as long as its Python code for tensors that the kernels take some us for)
+    tensors = grads if out is None else grads + results
     dev = grads[0].device
-    table = (L.ClipTensor * len(grads))()
-    spans, seen, k = [], {}, 0
-    for i, g in enumerate(grads):
-        o = g if out is None else out[i]
-        for t in (g,) if o is g else (g, o):
-            if not t.is_cuda:
-                raise RuntimeError('clip_grads: got a CPU tensor; the S2AG ops run on MI355X only and there is no CPU fallback')
-            if t.device != dev:
-                raise ValueError(f'clip_grads: tensors on {dev} and {t.device}')
-            if t.dtype not in _CLIP_DTYPES:
-                raise TypeError(f'clip_grads: tensors must be float32 or bfloat16, got {t.dtype}')
-            if t.layout != torch.strided or not _dense(t):
+    if not grads[0].is_cuda:
+        raise RuntimeError('clip_grads: got a CPU tensor; the S2AG ops run on MI355X only and there is no CPU fallback')
+    if any(d != dev for d in map(_DEVICE, tensors)):
+        raise ValueError(f'clip_grads: tensors on {sorted(set(map(str, map(_DEVICE, tensors))))}')
+    kinds = list(map(_CLIP_DTYPES.get, map(_DTYPE, tensors)))
+    if None in kinds:
+        raise TypeError(f'clip_grads: tensors must be float32 or bfloat16, got {tensors[kinds.index(None)].dtype}')
+    contiguous = all(map(torch.Tensor.is_contiguous, tensors))
+    if not contiguous:
+        for t in tensors:
+            if not _dense(t):
                 raise ValueError(f'clip_grads: a tensor of shape {tuple(t.shape)} and strides {tuple(t.stride())} is not dense in memory')
-        if o is not g and (o.shape != g.shape or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()))):
-            raise ValueError(f'clip_grads: output {tuple(o.shape)} / {tuple(o.stride())} for a gradient {tuple(g.shape)} / {tuple(g.stride())}')
-        n = g.numel()
-        if n == 0:
-            continue
-        src, dst = g.data_ptr(), o.data_ptr()
-        key = (src, n, g.dtype)
-        if key in seen:
-            if seen[key] != dst:
-                raise ValueError('clip_grads: a gradient that is listed twice has two outputs')
-            continue
-        seen[key] = dst
-        q = table[k]
-        q.src, q.dst, q.n, q.src_bf16, q.dst_bf16 = src, dst, n, _CLIP_DTYPES[g.dtype], _CLIP_DTYPES[o.dtype]
-        spans.append((src, src + n * g.element_size()))
-        if dst != src:
-            spans.append((dst, dst + n * o.element_size()))
-        elif o.dtype != g.dtype:
-            raise ValueError('clip_grads: an output overlaps a gradient of another type')
-        k += 1
+    if out is not None:
+        for g, o in zip(grads, results):
+            if o.shape != g.shape or not contiguous and o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()):
+                raise ValueError(f'clip_grads: output {tuple(o.shape)} / {tuple(o.stride())} for a gradient {tuple(g.shape)} / {tuple(g.stride())}')
+    # rows of s2ag_clip_tensor: src, dst, elements, (src is bf16) + 2^32 (dst is bf16); one that is listed again has the same row
+    src, counts = list(map(torch.Tensor.data_ptr, grads)), list(map(torch.Tensor.numel, grads))
+    dst = src if out is None else list(map(torch.Tensor.data_ptr, results))
+    rows = [r for r in dict.fromkeys(zip(src, dst, counts, (a + (b << 32) for a, b in zip(kinds, kinds[-len(grads):])))) if r[2]]
+    spans = [(r[0], r[0] + r[2] * _CLIP_BYTES[r[3] & 1]) for r in rows]
+    if out is not None:
+        spans += [(r[1], r[1] + r[2] * _CLIP_BYTES[r[3] >> 32]) for r in rows if r[0] != r[1] or (r[3] & 1) != r[3] >> 32]
     spans.sort()
-    for (_, end), (begin, _) in zip(spans, spans[1:]):
-        if begin < end:
-            raise ValueError('clip_grads: two of the tensors share memory')
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise ValueError('clip_grads: two of the tensors share memory, or one that is listed twice has two outputs')
+    rows = list(itertools.chain.from_iterable(rows))
+    k = len(rows) // 4
+    table = C.cast((C.c_longlong * max(len(rows), 1))(*rows), C.POINTER(L.ClipTensor))
     lib = L.load()
     with torch.cuda.device(dev):
         partials = torch.empty(lib.s2ag_clip_partials(table, k), dtype=torch.float64, device=dev)

@@ -6,6 +6,7 @@ stream of their tensors' device, can be captured into a graph (kernels only, mem
 bits for the same inputs."""
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from typing import Optional
 
@@ -21,14 +22,29 @@ MAX_ROWS = MAX_WORDS = 1 << 21         # linear_cross_entropy: rows of x, rows o
 
 
 def _p(t: Optional[Tensor]):
-    return None if t is None else C.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
-def _stream():
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+_NOTHING = contextlib.nullcontext()
 
 
-def _check_tensors(what: str, **ts) -> torch.device:
+def _on(t: Tensor):
+    """Context in which ``t``'s device is the current one (nothing to do where it is: the usual case)."""
+    dev = t.device
+    return _NOTHING if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _stream(t: Tensor) -> int:
+    return torch._C._cuda_getCurrentRawStream(t.device.index)      # (torch.cuda.current_stream builds an object: some us a call)
+
+
+def _once(backward):
+    """once_differentiable, whose bookkeeping is only wanted where a second derivative might be."""
+    full = torch.autograd.function.once_differentiable(backward)
+    return lambda ctx, *grads: (full if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+
+def _check_tensors(what: str, **ts) -> None:
     dev = None
     for name, t in ts.items():
         if not isinstance(t, Tensor):
@@ -39,7 +55,6 @@ def _check_tensors(what: str, **ts) -> torch.device:
             dev = t.device
         elif t.device != dev:
             raise ValueError(f'{what}: tensors on {dev} and {t.device}')
-    return dev
 
 
 def _check_ids(what: str, name: str, t: Tensor) -> None:
@@ -58,6 +73,8 @@ def _rows(t: Tensor):
     """(tensor, row pitch): ``t`` as a matrix with unit column stride; a copy only if its rows do not lie at one pitch."""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
+    if t.is_contiguous():
+        return t, t.shape[1]
     if t.numel() and (t.stride(1) != 1 and t.shape[1] > 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
         t = t.contiguous()
     return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
@@ -65,8 +82,10 @@ def _rows(t: Tensor):
 
 def _arena_slot(p: Tensor) -> Optional[Tensor]:
     """The gradient of a parameter that lives in an optim.ParamArena: the kernels add to it in place."""
+    if getattr(p, '_s2ag_arena', None) is None:
+        return None
     from .ops import _grad_slot
-    return _grad_slot(p) if getattr(p, '_s2ag_arena', None) is not None else None
+    return _grad_slot(p)
 
 
 # ----------------------------------------------------------------------------------------------------
@@ -75,32 +94,33 @@ def _arena_slot(p: Tensor) -> Optional[Tensor]:
 class _EmbeddingSorted(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, table, scale, padding_idx):
-        with torch.cuda.device(table.device):
+        lib = L.load()
+        with _on(table):
             ids = ids.contiguous()
             data = table.contiguous()
             n, (entries, dim) = ids.numel(), data.shape
+            i32, bf16 = ids.dtype == torch.int32, data.dtype == torch.bfloat16
             out = torch.empty(*ids.shape, dim, dtype=data.dtype, device=data.device)
-            L.check(L.load().s2ag_emb_lookup(_p(ids), int(ids.dtype == torch.int32), _p(data), int(data.dtype == torch.bfloat16), n, dim,
-                                             entries, scale, _p(out), _stream()), 'emb_lookup')
-        ctx.save_for_backward(ids)
-        ctx.table, ctx.scale, ctx.padding_idx = table, scale, padding_idx
+            L.check(lib.s2ag_emb_lookup(ids.data_ptr(), i32, data.data_ptr(), bf16, n, dim, entries, scale, out.data_ptr(), _stream(out)),
+                    'emb_lookup')
+        if ctx.needs_input_grad[1]:
+            ctx.save_for_backward(ids)
+            # (all that the backward pass needs to know: its thread runs Python code slowly)
+            ctx.plan = (lib, table, i32, bf16, n, dim, entries, padding_idx, scale, lib.s2ag_emb_grad_workspace_bytes(n, dim, entries))
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy):
         (ids,) = ctx.saved_tensors
-        table = ctx.table
-        entries, dim = table.shape
-        n, lib = ids.numel(), L.load()
-        with torch.cuda.device(table.device):
+        lib, table, i32, bf16, n, dim, entries, padding_idx, scale, ws_bytes = ctx.plan
+        with _on(dy):
             dy, ld = _rows(dy)
             slot = _arena_slot(table)
-            dt = torch.empty(entries, dim, dtype=table.dtype, device=table.device) if slot is None else slot
-            ws_bytes = lib.s2ag_emb_grad_workspace_bytes(n, dim, entries)
-            ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=table.device)
-            L.check(lib.s2ag_emb_grad(_p(ids), int(ids.dtype == torch.int32), _p(dy), ld, int(table.dtype == torch.bfloat16), n, dim, entries,
-                                      ctx.padding_idx, ctx.scale, _p(dt), int(slot is not None), _p(ws), ws.numel(), _stream()), 'emb_grad')
+            dt = torch.empty(entries, dim, dtype=dy.dtype, device=dy.device) if slot is None else slot
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dy.device)
+            L.check(lib.s2ag_emb_grad(ids.data_ptr(), i32, dy.data_ptr(), ld, bf16, n, dim, entries, padding_idx, scale, dt.data_ptr(),
+                                      slot is not None, ws.data_ptr(), ws_bytes, _stream(dy)), 'emb_grad')
         return None, (dt if slot is None else None), None, None
 
 
@@ -151,7 +171,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, target, ignore_index, reduction):
         lib = L.load()
-        with torch.cuda.device(x.device):
+        with _on(x):
             xr, ldx = _rows(x)
             w, ldw = _rows(weight)
             t = target.contiguous().view(-1)
@@ -160,19 +180,19 @@ class _LinearCrossEntropy(torch.autograd.Function):
             a = _lce_args(xr, w, t, ldx, ldw, ignore_index, reduction, state)
             a.loss = loss.data_ptr() or state.data_ptr()          # (no rows, no reduction: nothing is written)
             ws = _lce_workspace(a, False, x.device)
-            L.check(lib.s2ag_lce_fwd(C.byref(a), _stream()), 'lce_fwd')
+            L.check(lib.s2ag_lce_fwd(C.byref(a), _stream(x)), 'lce_fwd')
             del ws
         ctx.save_for_backward(x, weight, t, state)
         ctx.weight_leaf, ctx.meta = weight, (ignore_index, reduction)
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dloss):
         x, weight, t, state = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[:2]
         lib = L.load()
-        with torch.cuda.device(x.device):
+        with _on(x):
             slot = _arena_slot(ctx.weight_leaf) if need_w else None
             dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
             dw = None
@@ -189,7 +209,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
                 a.grad_out = g.data_ptr()
                 a.dx, a.dw, a.dw_accumulate = (None if dx is None else dx.data_ptr()), (None if dw is None else dw.data_ptr()), int(slot is not None)
                 ws = _lce_workspace(a, True, x.device)
-                L.check(lib.s2ag_lce_bwd(C.byref(a), _stream()), 'lce_bwd')
+                L.check(lib.s2ag_lce_bwd(C.byref(a), _stream(x)), 'lce_bwd')
                 del ws
         return dx, (dw if slot is None else None), None, None, None
 
