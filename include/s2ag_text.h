@@ -57,6 +57,7 @@ typedef struct {
     long long rows, vocab, ldx, ldw, ignore_index;
     int dim, reduction;
     float* loss;             /* forward: one word, or `rows` of them with S2AG_LCE_NONE */
+    int keep;                /* forward: a backward call will follow (its operands stay in `state`) */
     void* state;             /* s2ag_lce_state_bytes: written by the forward call, read by the backward call */
     const float* grad_out;   /* backward: one word, or `rows` of them */
     void *dx, *dw;           /* backward: contiguous, either may be null */
@@ -64,7 +65,7 @@ typedef struct {
     void* workspace;
     long long workspace_bytes;
 } s2ag_lce_args;
-long long s2ag_lce_state_bytes(long long rows);
+long long s2ag_lce_state_bytes(const s2ag_lce_args* a /*host*/);
 long long s2ag_lce_workspace_bytes(const s2ag_lce_args* a /*host*/, int backward);
 int s2ag_lce_fwd(const s2ag_lce_args* a /*host*/, void* stream);
 int s2ag_lce_bwd(const s2ag_lce_args* a /*host*/, void* stream);

@@ -89,7 +89,7 @@ class ClipTensor(C.Structure):    # s2ag_clip_tensor
 
 class LceArgs(C.Structure):       # s2ag_lce_args
     _fields_ = [('x', vp), ('w', vp), ('target', vp), ('target_i32', ci), ('bf16', ci), ('rows', cll), ('vocab', cll), ('ldx', cll),
-                ('ldw', cll), ('ignore_index', cll), ('dim', ci), ('reduction', ci), ('loss', vp), ('state', vp), ('grad_out', vp),
+                ('ldw', cll), ('ignore_index', cll), ('dim', ci), ('reduction', ci), ('loss', vp), ('keep', ci), ('state', vp), ('grad_out', vp),
                 ('dx', vp), ('dw', vp), ('dw_accumulate', ci), ('workspace', vp), ('workspace_bytes', cll)]
 
 
@@ -256,7 +256,7 @@ TEXT_SIGNATURES = {
     's2ag_emb_lookup': [vp, ci, vp, ci, cll, ci, cll, cf, vp, vp],
     's2ag_emb_grad_workspace_bytes': [cll, ci, cll],
     's2ag_emb_grad': [vp, ci, vp, cll, ci, cll, ci, cll, cll, cf, vp, ci, vp, cll, vp],
-    's2ag_lce_state_bytes': [cll],
+    's2ag_lce_state_bytes': [C.POINTER(LceArgs)],
     's2ag_lce_workspace_bytes': [C.POINTER(LceArgs), ci],
     's2ag_lce_fwd': [C.POINTER(LceArgs), vp],
     's2ag_lce_bwd': [C.POINTER(LceArgs), vp],

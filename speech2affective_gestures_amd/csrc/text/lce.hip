@@ -6,10 +6,10 @@
 // Bound by the matrix pipe: 2 N V D operations for the loss, 8 N V D with the gradient (the logits are formed twice: keeping
 // them would be N V values, the largest tensor of a training step by far).
 //
-// All four products are ONE tiled product out[r][c] = sum_k R[r][k] Q[c][k] of two bf16 matrices whose rows run along k, with
-// four ends: (1) max and sum of exponentials of each row of a tile of logits, joined over the tiles by a small launch;
-// (2) G of a piece of the vocabulary, stored as [row][word] and as [word][row]; (3) dX += G W over that piece in fp32;
-// (4) dW of that piece.  Operands whose rows do not run along k are transposed once (X^T, W^T: small beside the products).
+// All four products are ONE tiled product out[r][c] = sum_k R[r][k] Q[c][k] on bf16 matrix instructions with four ends: (1) max
+// and sum of exponentials of each row of a tile of logits, joined over the tiles by a small launch; (2) G of a piece of the
+// vocabulary, stored; (3) dX += G W over that piece in fp32; (4) dW of that piece.  Where k runs down the columns of an operand
+// as it lies in memory (W in (3), G and X in (4)) its fragments come by the transposing LDS read: nothing is transposed in memory.
 //
 // The rows that are ignored are left out of every product: the others are packed in front (rowmap), their number stays on the
 // device, and the tiles behind it end at once.
@@ -76,7 +76,7 @@ __global__ __launch_bounds__(1024) void select_rows_k(const void* __restrict__ t
     if (threadIdx.x == 0) *s.count = base;
 }
 
-// ---- operands: rows along k, padded with zeros to a multiple of 64, fp32 as three bf16 pieces --------------------------------
+// ---- operands: rows of features, padded with zeros to a multiple of 64, fp32 as three bf16 pieces --------------------------------
 struct Operand {
     const bf16_t* p;
     long long plane, ld;                // elements
@@ -105,40 +105,22 @@ __global__ __launch_bounds__(256) void pack_k(const T* __restrict__ src, long lo
         const bool in = r < live;
         const T* s = src + (in ? (rowmap ? (long long)rowmap[r] : r) : 0) * ld;
         bf16x8 q[3];
+        float v[8];
+        if (in && c + 8 <= dim) {
+            for (int j = 0; j < 8; j += Vec<T>::N) Vec<T>::load_any(s + c + j, v + j);
+        } else {
+            for (int j = 0; j < 8; ++j) v[j] = in && c + j < dim ? (float)s[c + j] : 0.f;
+        }
         for (int j = 0; j < 8; ++j) {
-            const float v = in && c + j < dim ? (float)s[c + j] : 0.f;
             if constexpr (sizeof(T) == 2) {
-                q[0][j] = (bf16_t)v;
+                q[0][j] = (bf16_t)v[j];
             } else {
                 bf16_t p[3];
-                split3(v, p);
+                split3(v[j], p);
                 for (int k = 0; k < 3; ++k) q[k][j] = p[k];
             }
         }
         for (int k = 0; k < (sizeof(T) == 2 ? 1 : 3); ++k) *reinterpret_cast<bf16x8*>(dst + k * plane + r * kp + c) = q[k];
-    }
-}
-
-// dst[c][r] = src[r][c] for r < rows (zeros behind, up to the multiple of 64 that holds rows_end), c < cols; 64 x 64 a workgroup
-__global__ __launch_bounds__(256) void transpose_k(Operand src, long long rows, const int* __restrict__ count, int cols,
-                                                   bf16_t* __restrict__ dst, long long ld_dst, long long plane_dst) {
-    __shared__ bf16_t sm[64][66];
-    const long long r0 = (long long)blockIdx.x * 64;
-    const int c0 = blockIdx.y * 64;
-    if (count && r0 >= (long long)*count) return;                // (packed rows are zero up to a multiple of 256)
-    const bf16_t* s = src.p + blockIdx.z * src.plane;
-    bf16_t* d = dst + blockIdx.z * plane_dst;
-    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-        const int r = i >> 6, c = i & 63;
-        sm[r][c] = r0 + r < rows && c0 + c < cols ? s[(r0 + r) * src.ld + c0 + c] : (bf16_t)0.f;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 64 * 8; i += 256) {
-        const int c = i >> 3, r = (i & 7) * 8;
-        if (c0 + c >= cols) continue;
-        bf16x8 q;
-        for (int j = 0; j < 8; ++j) q[j] = sm[r + j][c];
-        *reinterpret_cast<bf16x8*>(d + (long long)(c0 + c) * ld_dst + r0 + r) = q;
     }
 }
 
@@ -147,28 +129,34 @@ enum End { STATS, GRADS, ACCUM, STORE };
 
 struct Product {
     Operand r, q;
-    long long r_rows, q_rows;           // rows that exist
+    long long r_rows, q_rows;           // rows of out, columns of out that exist; what lies behind reads as zeros
+    // an operand whose k runs down its columns: its rows (k) and columns that exist
+    long long r_deep, q_deep;
+    int r_cols, q_cols;
     int k;                              // of one pair of pieces, a multiple of 64
     const int* k_count;                 // not null: k is this, rounded up to 64
     const int* r_count;                 // not null: rows of R that matter
     int pairs;                          // 1, or 6 of three pieces
     int tiles_q, group;
     int splits, slots;                  // the most parts of k; workgroups that run at a time
-    // STATS: max and sum of exponentials [tile_q][padded rows], logit of the target; GRADS: lse, factor of each row
+    // STATS: max and sum of exponentials [tile_q][padded rows], logit of the target
     const int* tgt;
     long long q0;                       // word number of Q's first row
     long long vocab;
     float2* part;
     long long part_ld;
     float* target_logit;
-    const float *lse, *factor;
-    bf16_t *g, *gt;                     // GRADS: [row][word] pitch g_ld, [word][row] pitch gt_ld (either may be null)
-    long long g_ld, g_plane, gt_ld, gt_plane;
+    // GRADS: [row][word] pitch g_ld; the factor of each row is grad_out[rowmap[row]], if it is not one for all
+    const float *lse, *grad_out;
+    const int* rowmap;
+    bf16_t* g;
+    long long g_ld, g_plane;
     // ACCUM: fp32 [split][row, padded to the tile][col] pitch out_ld; STORE: rows of dW
     void* out;
     long long out_ld;
     int cols, add, out_bf16;
-    const float* scale;                 // STORE: the factor of all rows
+    const float* scale;                 // STORE: not null: the factor of all rows, over their number with `mean`
+    int mean;
 };
 
 // pairs of pieces, the smallest products first: (0, 2) (1, 1) (2, 0) (0, 1) (1, 0) (0, 0), two bits each
@@ -182,9 +170,17 @@ typedef short s16x4_t __attribute__((ext_vector_type(4)));
 // wavefront reads at one slot lie in different banks.
 __device__ __forceinline__ int slot_at(int row, int slot) { return row * BK + ((slot ^ (row & 7)) << 3); }
 
-// 16 bytes a lane from the buffer to LDS: lane l's land at dst + 16 l
-__device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t from, bf16_t* dst, unsigned lane_offset, int offset) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, S2AG_LDS_PTR(void, dst), 16, lane_offset, offset, 0, 0);
+// A raw buffer descriptor: base address, no stride, bytes behind which a lane reads zeros.
+__device__ __forceinline__ u32x4 buffer(const void* p, unsigned bytes) {
+    const unsigned long long a = reinterpret_cast<unsigned long long>(p);
+    return u32x4{(unsigned)a, (unsigned)(a >> 32), bytes, 0x00020000u};
+}
+
+// 16 bytes a lane from the buffer to LDS: lane l's land at dst + 16 l.  Written out, because behind the builtin the compiler lets
+// every transposing read wait for all requests that are out; no register is loaded, and the waits for LDS are the kernel's own.
+__device__ __forceinline__ void to_lds(u32x4 from, bf16_t* dst, unsigned lane_offset, int offset) {
+    const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)S2AG_LDS_PTR(void, dst));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "s"(at), "v"(lane_offset), "s"(from), "s"(offset) : "memory");
 }
 
 // Matrix instruction with its accumulator in the accumulation registers, where the compiler, left to itself, moves a set that
@@ -198,6 +194,12 @@ __device__ __forceinline__ float acc_read(float a) {
     float v;
     asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(a));
     return v;
+}
+// A barrier for LDS alone: stores to memory stay out (__syncthreads would wait for them).
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // (keeps what follows behind the barrier)
 }
 __device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
@@ -262,7 +264,7 @@ __device__ __forceinline__ void write_out(bf16_t* scratch, T* out, const Product
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-        __syncthreads();
+        lds_barrier();
         for (int i = threadIdx.x; i < WR * 16 * JS * SLOTS; i += NT) {
             const int lrow = i / SLOTS, slot = i % SLOTS;
             const long long row = r0 + lrow / (16 * JS) * TR + jj * 16 + lrow % (16 * JS), c = c0 + slot * V;
@@ -282,8 +284,46 @@ __device__ __forceinline__ void write_out(bf16_t* scratch, T* out, const Product
                     if (c + e < p.cols) o[e] = (T)(p.add ? (float)o[e] + v[e] : v[e]);
             }
         }
-        __syncthreads();
+        lds_barrier();
     });
+}
+
+// An operand's tile in LDS.  k along its rows: [row][64 k], slots of 16 bytes permuted by slot_at.  k down its columns: [k][B
+// columns], pairs of slots (the 16 columns of a fragment) permuted by four bits of k, so that the 16 rows that a transposing read
+// touches lie in different banks.
+template <int B>
+__device__ __forceinline__ int pair_at(int k, int pair) { return k * B + ((pair ^ (((k & 3) | ((k >> 3) & 3) << 2) & (B / 16 - 1))) << 4); }
+
+// byte offset in the operand of the 16 bytes that a thread brings with request i
+template <int B, bool DOWN, int NT>
+__device__ __forceinline__ unsigned request_at(int i, int tid, long long ld) {
+    const int at = i * NT + tid;                                 // 16-byte place in the tile
+    if constexpr (DOWN) {
+        const int k = at / (B / 8), slot = at % (B / 8);
+        return (unsigned)(k * ld * 2 + (pair_at<B>(k, slot >> 1) - k * B + (slot & 1) * 8) * 2);
+    } else {
+        const int row = at >> 3;
+        return (unsigned)(row * ld * 2 + ((at & 7) ^ (row & 7)) * 16);
+    }
+}
+
+// the operand's 16 rows (or columns) from x on, k = 32 ks + 8 fk + 0..7
+template <int B, bool DOWN>
+__device__ __forceinline__ bf16x8 fragment(const bf16_t* tile, int x, int ks, int fl, int fk) {
+    if constexpr (!DOWN) {
+        return *reinterpret_cast<const bf16x8*>(tile + slot_at(x + fl, ks * 4 + fk));
+    } else {
+        bf16x8 v;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int k = ks * 32 + fk * 8 + h * 4 + (fl >> 2);
+            const bf16x4 y = __builtin_bit_cast(
+                bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(S2AG_LDS_PTR(s16x4_t, tile + pair_at<B>(k, x >> 4) + (fl & 3) * 4)));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[h * 4 + e] = y[e];
+        }
+        return v;
+    }
 }
 
 template <int BR, int BQ, int WR, int WQ, End END, bool PRECISE>
@@ -292,6 +332,7 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
     constexpr int TR = BR / WR, TQ = BQ / WQ, RI = TR / 16, QI = TQ / 16;      // a wavefront's part
     constexpr int LR = BR * 8 / NT, LQ = BQ * 8 / NT;                          // 16-byte loads per thread and stage
     constexpr int STAGE = (BR + BQ) * BK;
+    constexpr bool RK = END == STORE, QK = END == STORE || END == ACCUM;       // k runs down the operand's columns
     extern __shared__ __attribute__((aligned(16))) bf16_t lds[];
     bf16_t* const scratch = lds + 2 * STAGE;                                   // 64 x BQ, for the ends
     const int tid = threadIdx.x, lane = tid & 63;
@@ -299,7 +340,11 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
     const int wr = wave / WQ, wq = wave % WQ;
     constexpr int pairs = PRECISE ? 6 : 1;
     // (read here: a load that is still out behind the end of a tile would be waited for in every stage of the next one)
-    const float f = END == STORE && p.scale ? __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(*p.scale))) : 1.f;
+    float f = 1.f;
+    if constexpr (END == STORE) {
+        if (p.scale) f = p.mean ? *p.scale / (float)max(1, *p.k_count) : *p.scale;
+        f = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(f)));
+    }
 
     // (whole-number division runs on the vector units: the results are told to be one for the wavefront, so that the operands'
     // descriptors stay in scalar registers)
@@ -337,36 +382,46 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
         return t;
     };
 
-    const int ld_row = tid >> 3, ld_slot = (tid & 7) ^ (ld_row & 7);
     unsigned r_off[LR], q_off[LQ];
 #pragma unroll
-    for (int i = 0; i < LR; ++i) r_off[i] = (unsigned)((ld_row + i * (NT / 8)) * p.r.ld * 2 + ld_slot * 16);
+    for (int i = 0; i < LR; ++i) r_off[i] = request_at<BR, RK, NT>(i, tid, p.r.ld);
 #pragma unroll
-    for (int i = 0; i < LQ; ++i) q_off[i] = (unsigned)((ld_row + i * (NT / 8)) * p.q.ld * 2 + ld_slot * 16);
+    for (int i = 0; i < LQ; ++i) q_off[i] = request_at<BQ, QK, NT>(i, tid, p.q.ld);
 
     // the stage that is requested next: its tile, pair of pieces and place along k; behind the last one the descriptors are
     // empty, so that the loop has no branch
     int next = first - step, pair = 0, kk = 0, left = 0;
-    const bf16_t *r_at = p.r.p, *q_at = p.q.p;
-    int r_bytes = 0, q_bytes = 0;
-    __amdgpu_buffer_rsrc_t rr, qr;
+    long long r0_next = 0, c0_next = 0;
+    u32x4 rr, qr;
+    // an operand's part of that stage: from row x of R or Q, or from its column x on
+    auto descriptor = [&](const Operand& o, int piece, bool down, long long x, long long rows, int tile, long long deep, int cols) {
+        const bf16_t* at = o.p + piece * o.plane;
+        long long bytes;
+        if (down) {
+            const long long k0 = (long long)kk * BK, n = deep - k0 < BK ? deep - k0 : BK;
+            at += k0 * o.ld + x;
+            bytes = n > 0 ? ((n - 1) * o.ld + cols - x) * 2 : 0;
+        } else {
+            const long long n = rows - x < tile ? rows - x : tile;
+            at += x * o.ld;
+            bytes = n > 0 ? n * o.ld * 2 : 0;                    // (a tile may lie behind the words)
+        }
+        return buffer(at, left > 0 ? (unsigned)bytes : 0u);
+    };
     auto descriptors = [&]() {
-        rr = __builtin_amdgcn_make_buffer_rsrc((void*)(r_at + piece_r(PRECISE ? pair : 5) * p.r.plane), 0, r_bytes, 0x00020000);
-        qr = __builtin_amdgcn_make_buffer_rsrc((void*)(q_at + piece_q(PRECISE ? pair : 5) * p.q.plane), 0, q_bytes, 0x00020000);
+        rr = descriptor(p.r, piece_r(PRECISE ? pair : 5), RK, r0_next, p.r_rows, BR, p.r_deep, p.r_cols);
+        qr = descriptor(p.q, piece_q(PRECISE ? pair : 5), QK, c0_next, p.q_rows, BQ, p.q_deep, p.q_cols);
     };
     auto next_tile = [&]() {
-        r_bytes = q_bytes = 0;
+        left = 0;
         for (next += step; next < last; next += step) {
             const Place t = place(next);
             left = t.it1 - t.it0;
             if (left <= 0) continue;                             // (no stage: nothing to request)
             pair = __builtin_amdgcn_readfirstlane(t.it0 / ts.kt);
             kk = t.it0 - pair * ts.kt;
-            const long long r_left = p.r_rows - t.r0, q_left = p.q_rows > t.c0 ? p.q_rows - t.c0 : 0;      // (a tile may lie behind the words)
-            r_bytes = (int)((r_left < BR ? r_left : BR) * p.r.ld * 2);
-            q_bytes = (int)((q_left < BQ ? q_left : BQ) * p.q.ld * 2);
-            r_at = p.r.p + t.r0 * p.r.ld;
-            q_at = p.q.p + t.c0 * p.q.ld;
+            r0_next = t.r0;
+            c0_next = t.c0;
             break;
         }
         descriptors();
@@ -374,35 +429,36 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
     auto advance = [&]() {
         if (--left <= 0) {
             next_tile();
-        } else if (++kk == ts.kt) {
-            kk = 0;
-            ++pair;
-            descriptors();
+        } else {
+            const bool wrap = ++kk == ts.kt;
+            if (wrap) {
+                kk = 0;
+                ++pair;
+            }
+            if (RK || QK || wrap) descriptors();
         }
     };
     // requests [from, from + n) of the LR + LQ of a stage
     auto issue = [&](int buf, int from, int n) {
         bf16_t* s = lds + buf * STAGE + wave * 512;
-        const int off = kk * (BK * 2);
+        const int off = kk * (BK * 2);                           // (down the columns the descriptor moves)
 #pragma unroll
         for (int i = from; i < from + n; ++i) {
-            if (i < LR) to_lds(rr, s + i * NT * 8, r_off[i < LR ? i : 0], off);
-            else to_lds(qr, s + BR * BK + (i - LR) * NT * 8, q_off[i < LR ? 0 : i - LR], off);
+            if (i < LR) to_lds(rr, s + i * NT * 8, r_off[i < LR ? i : 0], RK ? 0 : off);
+            else to_lds(qr, s + BR * BK + (i - LR) * NT * 8, q_off[i < LR ? 0 : i - LR], QK ? 0 : off);
         }
     };
 
     f32x4 acc[QI][RI];
     const int fl = lane & 15, fk = lane >> 4;
-    const bf16_t* const rs = lds + wr * TR * BK;
-    const bf16_t* const qs = lds + BR * BK + wq * TQ * BK;
     // fragments [from, to) of half ks of a stage
     auto read_q = [&](bf16x8 (&a)[QI], int buf, int ks, int from, int to) {
 #pragma unroll
-        for (int i = from; i < to; ++i) a[i] = *reinterpret_cast<const bf16x8*>(qs + buf * STAGE + slot_at(i * 16 + fl, ks * 4 + fk));
+        for (int i = from; i < to; ++i) a[i] = fragment<BQ, QK>(lds + buf * STAGE + BR * BK, wq * TQ + i * 16, ks, fl, fk);
     };
     auto read_r = [&](bf16x8 (&b)[RI], int buf, int ks, int from, int to) {
 #pragma unroll
-        for (int j = from; j < to; ++j) b[j] = *reinterpret_cast<const bf16x8*>(rs + buf * STAGE + slot_at(j * 16 + fl, ks * 4 + fk));
+        for (int j = from; j < to; ++j) b[j] = fragment<BR, RK>(lds + buf * STAGE, wr * TR + j * 16, ks, fl, fk);
     };
     auto multiply = [&](const bf16x8 (&a)[QI], const bf16x8 (&b)[RI], int i) {
 #pragma unroll
@@ -449,7 +505,8 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
                 __builtin_amdgcn_sched_barrier(0);
                 if (i < G / 4) read_r(b1, buf, 1, i * RB, (i + 1) * RB);
                 if (i == EARLY) {
-                    if constexpr (G / 4 < EARLY) asm volatile("s_waitcnt lgkmcnt(4)" ::: "memory");
+                    if constexpr (G / 4 < EARLY && !QK) asm volatile("s_waitcnt lgkmcnt(4)" ::: "memory");      // (Q's reads so far)
+                    else if constexpr (G / 4 < EARLY) asm volatile("s_waitcnt lgkmcnt(8)" ::: "memory");
                     else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                     __builtin_amdgcn_s_barrier();
                     asm volatile("s_waitcnt lgkmcnt(15)" ::: "memory");      // (keeps the requests behind the barrier)
@@ -522,7 +579,7 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
                     if (fk == 0) sm[wq * BR + wr * TR + j * 16 + fl] = make_float2(m, s);
                     __builtin_amdgcn_sched_barrier(0);           // (rows in turn: all at once would not fit the registers)
                 }
-                __syncthreads();
+                lds_barrier();
                 for (int r = tid; r < BR; r += NT) {
                     float2 a = sm[r];
 #pragma unroll
@@ -534,11 +591,10 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
                     p.part[t.c0 / BQ * p.part_ld + t.r0 + r] = a;
                 }
             } else {
-                // Through LDS as [row][word], 32 rows of each of the WR parts at a time: rows are written out from it as they
-                // are, columns by the transposing read.
-                constexpr int SLOTS = BQ / 8;
+                // Through LDS, 32 rows of each of the WR parts at a time (16 where there are three pieces of each value to hold): whole
+                // rows of the tile are written out.
+                constexpr int SLOTS = BQ / 8, pieces = PRECISE ? 3 : 1, JS = PRECISE ? 1 : 2;
                 auto at = [](int row, int slot) { return row * BQ + ((slot ^ (row & 15)) << 3); };
-                constexpr int pieces = PRECISE ? 3 : 1;
                 float lse[RI], fac[RI];
                 int tgt[RI];
 #pragma unroll
@@ -546,74 +602,56 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
                     const long long row = wr0 + j * 16 + fl;
                     const bool in = row < live;                  // (rows behind are zeros: a factor of 0 keeps them so)
                     lse[j] = in ? p.lse[row] : 0.f;
-                    fac[j] = in ? (p.factor ? p.factor[row] : 1.f) : 0.f;
+                    fac[j] = in ? (p.grad_out ? p.grad_out[p.rowmap[row]] : 1.f) : 0.f;
                     tgt[j] = in ? p.tgt[row] : -1;
                 }
-                for (int piece = 0; piece < pieces; ++piece) {   // (a piece is split off the value formed again: no registers for rests)
-                    each<0, RI, 2>([&](auto at_j) {
-                        constexpr int jj = decltype(at_j)::value;
+                each<0, RI, JS>([&](auto at_j) {
+                    constexpr int jj = decltype(at_j)::value;
+                    float g[JS][QI * 4];
 #pragma unroll
-                        for (int j = jj; j < jj + 2; ++j) {
-                            const unsigned place = (unsigned)(tgt[j] - word0);       // the target's, if it is the lane's
-                            float g[QI * 4];
+                    for (int j = 0; j < JS; ++j) {
+                        const unsigned place = (unsigned)(tgt[jj + j] - word0);      // the target's, if it is the lane's
 #pragma unroll
-                            for (int i = 0; i < QI * 4; ++i) g[i] = exp_of<PRECISE>(value(i / 4, j, i % 4) - lse[j]);
-                            if (place < (unsigned)TQ) {
+                        for (int i = 0; i < QI * 4; ++i) g[j][i] = exp_of<PRECISE>(value(i / 4, jj + j, i % 4) - lse[jj + j]);
+                        if (place < (unsigned)TQ) {
 #pragma unroll
-                                for (int i = 0; i < QI * 4; ++i)
-                                    if (place == (unsigned)(i / 4 * 16 + i % 4)) g[i] -= 1.f;
-                            }
-                            if (edge) {
+                            for (int i = 0; i < QI * 4; ++i)
+                                if (place == (unsigned)(i / 4 * 16 + i % 4)) g[j][i] -= 1.f;
+                        }
+                        if (edge) {
 #pragma unroll
-                                for (int i = 0; i < QI * 4; ++i)
-                                    if (i / 4 * 16 + i % 4 >= words) g[i] = 0.f;
-                            }
+                            for (int i = 0; i < QI * 4; ++i)
+                                if (i / 4 * 16 + i % 4 >= words) g[j][i] = 0.f;
+                        }
+#pragma unroll
+                        for (int i = 0; i < QI * 4; ++i) g[j][i] *= fac[jj + j];
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    each<0, pieces, 1>([&](auto at_piece) {
+                        constexpr int piece = decltype(at_piece)::value;
+#pragma unroll
+                        for (int j = 0; j < JS; ++j)
 #pragma unroll
                             for (int i = 0; i < QI; ++i) {
                                 bf16x4 q;
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
-                                    const float v = g[i * 4 + e] * fac[j];
-                                    q[e] = (bf16_t)v;
-                                    if (PRECISE && piece) {
-                                        const float rest = v - (float)q[e];
-                                        q[e] = (bf16_t)rest;
-                                        if (piece == 2) q[e] = (bf16_t)(rest - (float)q[e]);
-                                    }
+                                    q[e] = (bf16_t)g[j][i * 4 + e];
+                                    if (piece + 1 < pieces) g[j][i * 4 + e] -= (float)q[e];      // exact; what the next piece takes
                                 }
-                                const int lrow = wr * 32 + (j - jj) * 16 + fl, col = wq * TQ + i * 16 + fk * 4;
+                                const int lrow = wr * 16 * JS + j * 16 + fl, col = wq * TQ + i * 16 + fk * 4;
                                 *reinterpret_cast<bf16x4*>(scratch + at(lrow, col >> 3) + (col & 4)) = q;
                             }
-                            __builtin_amdgcn_sched_barrier(0);
+                        lds_barrier();
+                        for (int i = tid; i < WR * 16 * JS * SLOTS; i += NT) {
+                            const int lrow = i / SLOTS, slot = i % SLOTS;
+                            const long long row = t.r0 + lrow / (16 * JS) * TR + jj * 16 + lrow % (16 * JS);
+                            *reinterpret_cast<bf16x8*>(p.g + piece * p.g_plane + row * p.g_ld + t.c0 + slot * 8) =
+                                *reinterpret_cast<const bf16x8*>(scratch + at(lrow, slot));
                         }
-                        __syncthreads();
-                        if (p.g)
-                            for (int i = tid; i < WR * 32 * SLOTS; i += NT) {
-                                const int lrow = i / SLOTS, slot = i % SLOTS;
-                                const long long row = t.r0 + (lrow >> 5) * TR + jj * 16 + (lrow & 31);
-                                *reinterpret_cast<bf16x8*>(p.g + piece * p.g_plane + row * p.g_ld + t.c0 + slot * 8) =
-                                    *reinterpret_cast<const bf16x8*>(scratch + at(lrow, slot));
-                            }
-                        if (p.gt)
-                            // a wavefront takes 16 words x 32 rows: its four groups of 16 lanes eight rows each, in two reads of four
-                            for (int u = wave; u < (BQ / 16) * WR; u += NT / 64) {
-                                const int w0 = (u % (BQ / 16)) * 16, part = u / (BQ / 16);
-                                bf16x8 q;
-#pragma unroll
-                                for (int h = 0; h < 2; ++h) {
-                                    const int lrow = part * 32 + fk * 8 + h * 4 + (fl >> 2), col = w0 + (fl & 3) * 4;
-                                    const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                        S2AG_LDS_PTR(s16x4_t, scratch + at(lrow, col >> 3) + (col & 4)));
-                                    const bf16x4 y = __builtin_bit_cast(bf16x4, x);
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) q[h * 4 + e] = y[e];
-                                }
-                                *reinterpret_cast<bf16x8*>(p.gt + piece * p.gt_plane + (t.c0 + w0 + fl) * p.gt_ld + t.r0 + part * TR + jj * 16 +
-                                                           fk * 8) = q;
-                            }
-                        __syncthreads();
+                        lds_barrier();
                     });
-                }
+                });
             }
         } else {
             // Through LDS too, as many rows at a time as it holds: a wavefront then writes whole rows of the tile.  (From the
@@ -676,21 +714,12 @@ __global__ __launch_bounds__(1024) void sum_loss_k(const float* __restrict__ row
     *loss = (float)(reduction == S2AG_LCE_MEAN ? s / (n > 0 ? n : 1) : s);
 }
 
-// factor[0]: of all rows (mean, sum), or factor[r]: of each packed row
-__global__ __launch_bounds__(256) void factors_k(const float* __restrict__ grad_out, State s, int reduction, float* __restrict__ factor) {
-    const int n = *s.count;
-    if (reduction != S2AG_LCE_NONE) {
-        if (blockIdx.x == 0 && threadIdx.x == 0) *factor = reduction == S2AG_LCE_MEAN ? *grad_out / (float)(n > 0 ? n : 1) : *grad_out;
-        return;
-    }
-    for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) factor[i] = grad_out[s.rowmap[i]];
-}
-
 // dx[r] = factor * sum over the splits of the packed row, zeros for rows that were ignored
 template <typename T>
 __global__ __launch_bounds__(256) void finish_dx_k(const float* __restrict__ acc, long long ld, int tile, int tiles_q, int most, int slots,
-                                                   State s, const float* __restrict__ scale, long long rows, int dim, T* __restrict__ dx) {
-    const float f = scale ? *scale : 1.f;
+                                                   State s, const float* __restrict__ scale, int mean, long long rows, int dim,
+                                                   T* __restrict__ dx) {
+    const float f = scale ? (mean ? *scale / (float)max(1, *s.count) : *scale) : 1.f;
     const int groups = (dim + 3) / 4, tiles_r = (*s.count + tile - 1) / tile, splits = splits_of(tiles_r * tiles_q, most, slots);
     const long long split = (long long)tiles_r * tile * ld;
     const long long total = rows * groups;
@@ -721,13 +750,16 @@ struct Plan {
     long long np, vp;                   // rows and words, padded
     int kp;
     bool pack_w;
+    // bytes from the state's start (kept) or the workspace's
+    long long xp, wp;
+    bool kept;
     // bytes from the workspace's start
-    long long xp, wp, part, tl, row_loss, xt, wt, factor, acc, g, gt, bytes;
+    long long part, tl, row_loss, acc, g, bytes, state_bytes;
     long long piece;                    // words of a piece of the vocabulary
     int acc_tile, splits, acc_ld;       // of the product that dX is
 };
 
-constexpr long long PIECE_VALUES = 1LL << 27;   // of G in a piece: 256 MB each way in bf16, beside which the fp32 sums of dX are small
+constexpr long long PIECE_VALUES = 1LL << 27;   // of G in a piece: 256 MB in bf16, beside which the fp32 sums of dX are small
 
 bool valid(const s2ag_lce_args* a) {
     // 2^21: a tile's rows stay within a 31-bit byte offset whichever way they run
@@ -754,8 +786,17 @@ Plan plan(const s2ag_lce_args* a, bool backward) {
         at += round_up(b, 256);
         return here;
     };
-    p.xp = take(2 * p.planes * p.np * p.kp);
-    p.wp = take(p.pack_w ? 2 * p.planes * a->vocab * p.kp : 0);
+    p.kept = backward || a->keep;
+    const long long x_bytes = round_up(2 * p.planes * p.np * p.kp, 256), w_bytes = p.pack_w ? round_up(2 * p.planes * a->vocab * p.kp, 256) : 0;
+    if (p.kept) {
+        p.xp = round_up(4 * state_words(a->rows), 256);
+        p.wp = p.xp + x_bytes;
+        p.state_bytes = p.wp + w_bytes;
+    } else {
+        p.xp = take(x_bytes);
+        p.wp = take(w_bytes);
+        p.state_bytes = 4 * state_words(a->rows);
+    }
     if (!backward) {
         p.part = take(8 * p.np * cdiv(a->vocab, 128));
         p.tl = take(4 * p.np);
@@ -764,19 +805,15 @@ Plan plan(const s2ag_lce_args* a, bool backward) {
         const long long most = PIECE_VALUES / p.planes / (p.np ? p.np : 1) / 256 * 256;
         const long long pieces = cdiv(p.vp, most < 1024 ? 1024 : most);
         p.piece = round_up(cdiv(p.vp, pieces), 256);
-        const bool dx = a->dx != nullptr, dw = a->dw != nullptr;
+        const bool dx = a->dx != nullptr;
         p.acc_ld = (int)round_up(a->dim, 4);
         // dX has few tiles: the words of a piece are split, down to eight stages each
         p.acc_tile = 256;
         const long long stages = p.piece / BK * p.pairs;
         p.splits = (int)(stages / 8 < 1 ? 1 : stages / 8 > SLOTS ? SLOTS : stages / 8);
-        p.xt = take(dw ? 2 * p.planes * a->dim * p.np : 0);
-        p.wt = take(dx ? 2 * p.planes * a->dim * p.vp : 0);
-        p.factor = take(4 * (a->reduction == S2AG_LCE_NONE ? p.np : 1));
         // (what fills the card with splits is no more than its tiles hold)
         p.acc = take(dx ? 4 * (p.np * p.acc_ld + (long long)SLOTS * 256 * 256) : 0);
-        p.g = take(dx ? 2 * p.planes * p.np * p.piece : 0);
-        p.gt = take(dw ? 2 * p.planes * p.np * p.piece : 0);
+        p.g = take(2 * p.planes * p.np * p.piece);
     }
     p.bytes = at;
     return p;
@@ -792,7 +829,7 @@ int launch_tiles(Product& p, long long r_rows, long long q_rows, hipStream_t st)
     // The rows of R of a group stay in an XCD's 4 MB L2 while the columns pass, if half of it holds them (k of 1024: 4 row tiles
     // 816 TFLOP/s, 8 of them 560; of 2048: 2 row tiles 1023, 8 of them 841); where not two fit, the 8 x 4 tiles that run at a time
     // share what they can.
-    const long long fit = (2LL << 20) / (2LL * BR * (p.k_count ? p.r.ld : p.k));
+    const long long fit = (2LL << 20) / (2LL * BR * (p.k_count ? p.r_deep : p.k));
     p.group = fit >= 8 || fit < 2 ? 8 : fit >= 4 ? 4 : 2;
     p.tiles_q = cdiv(q_rows, BQ);
     p.slots = SLOTS * PER_CU;
@@ -816,31 +853,24 @@ unsigned grid_of(long long work) {
     return (unsigned)(b < 1 ? 1 : b > 4096 ? 4096 : b);
 }
 
-int pack(const s2ag_lce_args* a, const Plan& p, const State& s, char* ws, Operand* x, Operand* w, hipStream_t st) {
-    bf16_t* xp = reinterpret_cast<bf16_t*>(ws + p.xp);
-    *x = Operand{xp, p.np * p.kp, p.kp};
-    const unsigned g = grid_of(p.np * (p.kp / 8));
-    if (a->bf16)
-        hipLaunchKernelGGL(pack_k<bf16_t>, dim3(g), dim3(256), 0, st, static_cast<const bf16_t*>(a->x), a->ldx, a->dim, s.rowmap, s.count,
-                           p.np, xp, p.kp, p.np * p.kp);
-    else
-        hipLaunchKernelGGL(pack_k<float>, dim3(g), dim3(256), 0, st, static_cast<const float*>(a->x), a->ldx, a->dim, s.rowmap, s.count, p.np,
-                           xp, p.kp, p.np * p.kp);
+// where the packed operands are, or the caller's W as it is
+void operands(const s2ag_lce_args* a, const Plan& p, Operand* x, Operand* w) {
+    char* at = static_cast<char*>(p.kept ? a->state : a->workspace);
+    *x = Operand{reinterpret_cast<bf16_t*>(at + p.xp), p.np * p.kp, p.kp};
+    if (p.pack_w) *w = Operand{reinterpret_cast<bf16_t*>(at + p.wp), a->vocab * p.kp, p.kp};
+    else *w = Operand{static_cast<const bf16_t*>(a->w), 0, a->ldw};
+}
+
+template <typename T>
+int pack(const s2ag_lce_args* a, const Plan& p, const State& s, const Operand& x, const Operand& w, hipStream_t st) {
+    hipLaunchKernelGGL(pack_k<T>, dim3(grid_of(p.np * (p.kp / 8))), dim3(256), 0, st, static_cast<const T*>(a->x), a->ldx, a->dim, s.rowmap,
+                       s.count, p.np, const_cast<bf16_t*>(x.p), p.kp, x.plane);
     S2AG_LAUNCH_CHECK();
-    if (!p.pack_w) {
-        *w = Operand{static_cast<const bf16_t*>(a->w), 0, a->ldw};
-        return 0;
+    if (p.pack_w) {
+        hipLaunchKernelGGL(pack_k<T>, dim3(grid_of(a->vocab * (p.kp / 8))), dim3(256), 0, st, static_cast<const T*>(a->w), a->ldw, a->dim,
+                           (const int*)nullptr, (const int*)nullptr, a->vocab, const_cast<bf16_t*>(w.p), p.kp, w.plane);
+        S2AG_LAUNCH_CHECK();
     }
-    bf16_t* wp = reinterpret_cast<bf16_t*>(ws + p.wp);
-    *w = Operand{wp, a->vocab * p.kp, p.kp};
-    const unsigned gw = grid_of(a->vocab * (p.kp / 8));
-    if (a->bf16)
-        hipLaunchKernelGGL(pack_k<bf16_t>, dim3(gw), dim3(256), 0, st, static_cast<const bf16_t*>(a->w), a->ldw, a->dim, (const int*)nullptr,
-                           (const int*)nullptr, a->vocab, wp, p.kp, a->vocab * p.kp);
-    else
-        hipLaunchKernelGGL(pack_k<float>, dim3(gw), dim3(256), 0, st, static_cast<const float*>(a->w), a->ldw, a->dim, (const int*)nullptr,
-                           (const int*)nullptr, a->vocab, wp, p.kp, a->vocab * p.kp);
-    S2AG_LAUNCH_CHECK();
     return 0;
 }
 
@@ -849,9 +879,9 @@ bool ready(const s2ag_lce_args* a, const Plan& p) {
 }
 }  // namespace
 
-extern "C" long long s2ag_lce_state_bytes(long long rows) {
-    if (rows < 0 || rows > (1 << 21)) return S2AG_E_BADARG;
-    return 4 * state_words(rows);
+extern "C" long long s2ag_lce_state_bytes(const s2ag_lce_args* a) {
+    if (!valid(a)) return S2AG_E_BADARG;
+    return plan(a, false).state_bytes;
 }
 
 extern "C" long long s2ag_lce_workspace_bytes(const s2ag_lce_args* a, int backward) {
@@ -872,7 +902,8 @@ extern "C" int s2ag_lce_fwd(const s2ag_lce_args* a, void* stream) {
     S2AG_LAUNCH_CHECK();
     if (a->rows) {
         Product q{};
-        if (int rc = pack(a, p, s, ws, &q.r, &q.q, st)) return rc;
+        operands(a, p, &q.r, &q.q);
+        if (int rc = a->bf16 ? pack<bf16_t>(a, p, s, q.r, q.q, st) : pack<float>(a, p, s, q.r, q.q, st)) return rc;
         q.r_rows = p.np;
         q.q_rows = q.vocab = a->vocab;
         q.k = p.kp;
@@ -902,26 +933,10 @@ extern "C" int s2ag_lce_bwd(const s2ag_lce_args* a, void* stream) {
     if (!a->dx && !a->dw) return 0;
     const State s = state_of(a->state, a->rows);
     char* ws = static_cast<char*>(a->workspace);
-    float* factor = reinterpret_cast<float*>(ws + p.factor);
-    const bool each = a->reduction == S2AG_LCE_NONE;
-    hipLaunchKernelGGL(factors_k, dim3(each ? grid_of(a->rows) : 1), dim3(256), 0, st, a->grad_out, s, a->reduction, factor);
-    S2AG_LAUNCH_CHECK();
+    const bool each = a->reduction == S2AG_LCE_NONE, mean = a->reduction == S2AG_LCE_MEAN;
     Operand x, w;
-    if (int rc = pack(a, p, s, ws, &x, &w, st)) return rc;
-    bf16_t* xt = reinterpret_cast<bf16_t*>(ws + p.xt);
-    bf16_t* wt = reinterpret_cast<bf16_t*>(ws + p.wt);
-    if (a->dw && p.np) {
-        hipLaunchKernelGGL(transpose_k, dim3((unsigned)(p.np / 64), cdiv(a->dim, 64), p.planes), dim3(256), 0, st, x, p.np, s.count, a->dim, xt,
-                           p.np, a->dim * p.np);
-        S2AG_LAUNCH_CHECK();
-    }
-    if (a->dx && p.np) {
-        hipLaunchKernelGGL(transpose_k, dim3((unsigned)(p.vp / 64), cdiv(a->dim, 64), p.planes), dim3(256), 0, st, w, a->vocab,
-                           (const int*)nullptr, a->dim, wt, p.vp, a->dim * p.vp);
-        S2AG_LAUNCH_CHECK();
-    }
+    operands(a, p, &x, &w);
     bf16_t* g = reinterpret_cast<bf16_t*>(ws + p.g);
-    bf16_t* gt = reinterpret_cast<bf16_t*>(ws + p.gt);
     float* acc = reinterpret_cast<float*>(ws + p.acc);
     for (long long v0 = 0; v0 < p.vp; v0 += p.piece) {
         const long long words = a->vocab - v0 < p.piece ? a->vocab - v0 : p.piece;     // that exist
@@ -939,20 +954,20 @@ extern "C" int s2ag_lce_bwd(const s2ag_lce_args* a, void* stream) {
         q.q0 = v0;
         q.vocab = a->vocab;
         q.lse = s.lse;
-        q.factor = each ? factor : nullptr;
-        q.g = a->dx ? g : nullptr;
+        q.grad_out = each ? a->grad_out : nullptr;
+        q.rowmap = s.rowmap;
+        q.g = g;
         q.g_ld = p.piece;
         q.g_plane = p.np * p.piece;
-        q.gt = a->dw ? gt : nullptr;
-        q.gt_ld = p.np;
-        q.gt_plane = p.piece * p.np;
         if (int rc = launch<GRADS>(q, big_tiles(p.np, wide), p.np, wide, st)) return rc;
         if (a->dx) {
             Product d{};
             d.r = Operand{g, q.g_plane, p.piece};
-            d.q = Operand{wt + v0, a->dim * p.vp, p.vp};
+            d.q = Operand{w.p + v0 * w.ld, w.plane, w.ld};
             d.r_rows = p.np;
             d.q_rows = d.cols = a->dim;
+            d.q_deep = words;
+            d.q_cols = p.pack_w ? p.kp : a->dim;
             d.k = (int)wide;
             d.pairs = p.pairs;
             d.r_count = s.count;
@@ -964,17 +979,21 @@ extern "C" int s2ag_lce_bwd(const s2ag_lce_args* a, void* stream) {
         }
         if (a->dw) {
             Product d{};
-            d.r = Operand{gt, q.gt_plane, p.np};
-            d.q = Operand{xt, a->dim * p.np, p.np};
+            d.r = Operand{g, q.g_plane, p.piece};
+            d.q = x;
             d.r_rows = words;
             d.q_rows = d.cols = a->dim;
+            d.r_deep = d.q_deep = p.np;
+            d.r_cols = (int)p.piece;
+            d.q_cols = p.kp;
             d.k_count = s.count;
             d.pairs = p.pairs;
             d.out = a->bf16 ? (void*)(static_cast<bf16_t*>(a->dw) + v0 * a->dim) : (void*)(static_cast<float*>(a->dw) + v0 * a->dim);
             d.out_ld = a->dim;
             d.out_bf16 = a->bf16;
             d.add = a->dw_accumulate;
-            d.scale = each ? nullptr : factor;
+            d.scale = each ? nullptr : a->grad_out;
+            d.mean = mean;
             if (int rc = launch<STORE>(d, big_tiles(words, a->dim), words, a->dim, st)) return rc;
         }
     }
@@ -982,10 +1001,10 @@ extern "C" int s2ag_lce_bwd(const s2ag_lce_args* a, void* stream) {
         const unsigned gx = grid_of(a->rows * ((a->dim + 3) / 4));
         if (a->bf16)
             hipLaunchKernelGGL(finish_dx_k<bf16_t>, dim3(gx), dim3(256), 0, st, acc, (long long)p.acc_ld, p.acc_tile, cdiv(a->dim, p.acc_tile), p.splits, SLOTS, s,
-                               each ? nullptr : factor, a->rows, a->dim, static_cast<bf16_t*>(a->dx));
+                               each ? nullptr : a->grad_out, (int)mean, a->rows, a->dim, static_cast<bf16_t*>(a->dx));
         else
             hipLaunchKernelGGL(finish_dx_k<float>, dim3(gx), dim3(256), 0, st, acc, (long long)p.acc_ld, p.acc_tile, cdiv(a->dim, p.acc_tile), p.splits, SLOTS, s,
-                               each ? nullptr : factor, a->rows, a->dim, static_cast<float*>(a->dx));
+                               each ? nullptr : a->grad_out, (int)mean, a->rows, a->dim, static_cast<float*>(a->dx));
         S2AG_LAUNCH_CHECK();
     }
     return 0;

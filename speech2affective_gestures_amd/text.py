@@ -149,68 +149,59 @@ def embedding_sorted(ids: Tensor, table: Tensor, scale: float = 1.0, padding_idx
 # ----------------------------------------------------------------------------------------------------
 # linear + softmax cross entropy
 # ----------------------------------------------------------------------------------------------------
-def _lce_args(x, w, target, ldx, ldw, ignore_index, reduction, state) -> 'L.LceArgs':
-    a = L.LceArgs()
-    a.x, a.w, a.target, a.state = x.data_ptr(), w.data_ptr(), target.data_ptr(), state.data_ptr()
-    a.target_i32, a.bf16 = int(target.dtype == torch.int32), int(x.dtype == torch.bfloat16)
-    a.rows, a.dim, a.vocab, a.ldx, a.ldw = x.shape[0], x.shape[1], w.shape[0], ldx, ldw
-    a.ignore_index, a.reduction = ignore_index, reduction
-    return a
-
-
-def _lce_workspace(a, backward: bool, device) -> Tensor:
-    n = L.load().s2ag_lce_workspace_bytes(C.byref(a), int(backward))
+def _lce_workspace(lib, a, backward: bool, device) -> Tensor:
+    n = lib.s2ag_lce_workspace_bytes(a, backward)
     if n < 0:
         raise RuntimeError(f'linear_cross_entropy: sizes refused ({n})')
-    ws = torch.empty(max(n, 16), dtype=torch.uint8, device=device)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    ws = torch.empty(n, dtype=torch.uint8, device=device)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), n
     return ws
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, target, ignore_index, reduction):
-        lib = L.load()
+        lib, a = L.load(), L.LceArgs()
         with _on(x):
-            xr, ldx = _rows(x)
-            w, ldw = _rows(weight)
-            t = target.contiguous().view(-1)
-            state = torch.empty(lib.s2ag_lce_state_bytes(xr.shape[0]) // 4, dtype=torch.int32, device=x.device)
+            xr, a.ldx = _rows(x)
+            w, a.ldw = _rows(weight)
+            t = target.contiguous()
+            a.x, a.w, a.target = xr.data_ptr(), w.data_ptr(), t.data_ptr()
+            a.target_i32, a.bf16 = t.dtype == torch.int32, x.dtype == torch.bfloat16
+            (a.rows, a.dim), a.vocab = xr.shape, w.shape[0]
+            a.ignore_index, a.reduction, a.keep = ignore_index, reduction, any(ctx.needs_input_grad)
+            state = torch.empty(lib.s2ag_lce_state_bytes(a), dtype=torch.uint8, device=x.device)
             loss = torch.empty(target.shape if reduction == 2 else (), dtype=torch.float32, device=x.device)
-            a = _lce_args(xr, w, t, ldx, ldw, ignore_index, reduction, state)
-            a.loss = loss.data_ptr() or state.data_ptr()          # (no rows, no reduction: nothing is written)
-            ws = _lce_workspace(a, False, x.device)
-            L.check(lib.s2ag_lce_fwd(C.byref(a), _stream(x)), 'lce_fwd')
-            del ws
-        ctx.save_for_backward(x, weight, t, state)
-        ctx.weight_leaf, ctx.meta = weight, (ignore_index, reduction)
+            a.state = state.data_ptr()
+            a.loss = loss.data_ptr() or a.state                   # (no rows, no reduction: nothing is written)
+            ws = _lce_workspace(lib, a, False, x.device)
+            L.check(lib.s2ag_lce_fwd(a, _stream(ws)), 'lce_fwd')
+        if a.keep:
+            ctx.save_for_backward(x, weight, t, state)
+            ctx.plan = (lib, a, w, weight)       # (w: the rows that a.w points at, where weight's own do not lie at one pitch)
         return loss
 
     @staticmethod
     @_once
     def backward(ctx, dloss):
         x, weight, t, state = ctx.saved_tensors
+        lib, a, w, leaf = ctx.plan
         need_x, need_w = ctx.needs_input_grad[:2]
-        lib = L.load()
         with _on(x):
-            slot = _arena_slot(ctx.weight_leaf) if need_w else None
+            slot = _arena_slot(leaf) if need_w else None
             dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-            dw = None
-            if need_w:
-                dw = slot if slot is not None else torch.empty(weight.shape, dtype=weight.dtype, device=x.device)
-            xr, ldx = _rows(x)
-            w, ldw = _rows(weight)
-            if xr.shape[0] == 0:
+            dw = slot
+            if need_w and slot is None:
+                dw = torch.empty(weight.shape, dtype=weight.dtype, device=x.device)
+            if a.rows == 0:
                 if dw is not None and slot is None:
                     dw.zero_()
             else:
                 g = dloss.to(torch.float32).contiguous()
-                a = _lce_args(xr, w, t, ldx, ldw, *ctx.meta, state)
-                a.grad_out = g.data_ptr()
-                a.dx, a.dw, a.dw_accumulate = (None if dx is None else dx.data_ptr()), (None if dw is None else dw.data_ptr()), int(slot is not None)
-                ws = _lce_workspace(a, True, x.device)
-                L.check(lib.s2ag_lce_bwd(C.byref(a), _stream(x)), 'lce_bwd')
-                del ws
+                b = L.LceArgs.from_buffer_copy(a)                # (a graph that is kept runs backward again)
+                b.grad_out, b.dx, b.dw, b.dw_accumulate = g.data_ptr(), _p(dx), _p(dw), slot is not None
+                ws = _lce_workspace(lib, b, True, x.device)
+                L.check(lib.s2ag_lce_bwd(b, _stream(ws)), 'lce_bwd')
         return dx, (dw if slot is None else None), None, None, None
 
 

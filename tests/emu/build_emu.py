@@ -3,13 +3,14 @@
 
     python tests/emu/build_emu.py [--force]
 
-The sources are used as they are except for six textual rewrites that a header cannot express (done on a copy under
+The sources are used as they are except for seven textual rewrites that a header cannot express (done on a copy under
 _build/src, line numbers kept):
   * `extern __shared__ [attrs] T name[];`  ->  `T* name = (T*)emu::dyn_smem();`   (dynamic LDS of the running workgroup)
   * `asm volatile("s_waitcnt ...")`        ->  nothing   (waits for the wave's own memory operations: no-ops in this model)
   * `asm volatile("s_waitcnt lgkmcnt(0)\\n\\ts_barrier")` -> `__syncthreads()`
   * `asm("v_mfma_f32_16x16x32_bf16 ..." : "+a"(c) ...)` -> the builtin of that instruction
   * `asm volatile("v_accvgpr_read_b32 ...")` -> an assignment
+  * `asm volatile("s_mov_b32 m0 ...; buffer_load_dwordx4 ... lds")` -> emu_buffer_to_lds (hip_runtime.h)
   * `asm volatile("s_nop ...")`            ->  nothing
 The library exports the same C ABI as libs2ag_hip.so (include/s2ag_hip.h) plus s2ag_emu_set_sched / s2ag_emu_counters."""
 import concurrent.futures as cf
@@ -40,6 +41,7 @@ _ASM_WAIT = re.compile(r'asm volatile\("s_waitcnt [a-z]+cnt\(\d+\)"\s*:::\s*"mem
 
 
 _ASM_MFMA = re.compile(r'asm\("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "\+a"\((\w+)\) : "v"\((\w+)\), "v"\((\w+)\)\);')
+_ASM_LDS = re.compile(r'const unsigned at = [^\n]*\n\s*asm volatile\("s_mov_b32 m0, %0\\n\\ts_nop 0\\n\\tbuffer_load_dwordx4 %1, %2, %3 offen lds" [^\n]*\n')
 _ASM_ACC = re.compile(r'asm volatile\("v_accvgpr_read_b32 %0, %1" : "=v"\((\w+)\) : "a"\((\w+)\)\);')
 _ASM_NOP = re.compile(r'asm volatile\("s_nop \d+(?:\\n\\ts_nop \d+)*"\s*:::\s*"memory"\)')
 
@@ -49,6 +51,7 @@ def rewrite(text: str) -> str:
     text = _ASM_BAR.sub('__syncthreads()', text)
     text = _ASM_WAIT.sub('((void)0)', text)
     text = _ASM_NOP.sub('((void)0)', text)
+    text = _ASM_LDS.sub('emu_buffer_to_lds(from, dst, lane_offset, offset);\n', text)
     text = _ASM_ACC.sub(lambda m: '%s = %s;' % (m.group(1), m.group(2)), text)
     text = _ASM_MFMA.sub(lambda m: '%s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(%s, %s, %s, 0, 0, 0);' % (m.group(1), m.group(2), m.group(3), m.group(1)), text)
     if 'asm volatile' in text or 'extern __shared__' in text:

@@ -430,14 +430,19 @@ static inline emu::u32x4_t emu_raw_buffer_load_b128(emu_buffer_rsrc r, unsigned 
 }
 #define __builtin_amdgcn_make_buffer_rsrc(p, stride, n, flags) emu_make_buffer_rsrc(p, stride, n, flags)
 #define __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, aux) emu_raw_buffer_load_b128(r, voff, soff, aux)
-// buffer_load_dwordx4 ... lds: lane l's 16 bytes land at the wavefront's LDS base + 16 l; a lane out of range stores zeros
+// buffer_load_dwordx4 ... lds: lane l's 16 bytes land at the wavefront's LDS base + 16 l; a lane out of range stores zeros.
+// `from`: the four words of a raw descriptor (address, its upper half, bytes, flags).
 template <typename P>
-static inline void emu_raw_ptr_buffer_load_lds(emu_buffer_rsrc r, P lds, unsigned size, unsigned voffset, unsigned soffset, unsigned inst, unsigned aux) {
-    if (size != 16) { fprintf(stderr, "[s2ag emu] buffer load to LDS of %u bytes\n", size); abort(); }
-    const emu::u32x4_t v = emu_raw_buffer_load_b128(r, voffset, soffset + inst, aux);
+static inline void emu_buffer_to_lds(emu::u32x4_t from, P lds, unsigned voffset, unsigned soffset) {
+    const emu_buffer_rsrc r{(const char*)(uintptr_t)(from[0] | (unsigned long long)from[1] << 32), from[2]};
+    // (the range check is on the lane's offset: the scalar one moves along rows that are inside)
+    emu::u32x4_t v = {0u, 0u, 0u, 0u};
+    if (voffset < r.num_records) {
+        if (voffset + 16ULL > r.num_records) { fprintf(stderr, "[s2ag emu] buffer load to LDS straddles num_records: %u of %u\n", voffset, r.num_records); abort(); }
+        memcpy(&v, r.base + voffset + soffset, 16);
+    }
     memcpy((char*)(uintptr_t)lds + 16 * emu::g_cur->lane, &v, 16);
 }
-#define __builtin_amdgcn_raw_ptr_buffer_load_lds(r, lds, size, voff, soff, inst, aux) emu_raw_ptr_buffer_load_lds(r, lds, size, voff, soff, inst, aux)
 #define __builtin_amdgcn_readlane(v, l) __shfl(v, l)
 #define __builtin_amdgcn_sched_barrier(x) ((void)0)
 #define __builtin_amdgcn_sched_group_barrier(a, b, c) ((void)0)
