@@ -178,8 +178,9 @@ __device__ __forceinline__ u32x4 buffer(const void* p, unsigned bytes) {
 
 // 16 bytes a lane from the buffer to LDS: lane l's land at dst + 16 l.  Written out, because behind the builtin the compiler lets
 // every transposing read wait for all requests that are out; no register is loaded, and the waits for LDS are the kernel's own.
-__device__ __forceinline__ void to_lds(u32x4 from, bf16_t* dst, unsigned lane_offset, int offset) {
-    const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)S2AG_LDS_PTR(void, dst));
+typedef __attribute__((address_space(3))) bf16_t* LdsPtr;       // (from a general pointer the compiler tests for null every time)
+__device__ __forceinline__ void to_lds(u32x4 from, LdsPtr dst, unsigned lane_offset, int offset) {
+    const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)dst);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "s"(at), "v"(lane_offset), "s"(from), "s"(offset) : "memory");
 }
 
@@ -307,18 +308,24 @@ __device__ __forceinline__ unsigned request_at(int i, int tid, long long ld) {
     }
 }
 
-// the operand's 16 rows (or columns) from x on, k = 32 ks + 8 fk + 0..7
+// Where a lane finds its part of the operand's fragments (16 rows or columns each) from x on.  k along the rows: place n is that of
+// half n of a stage, the fragments 16 rows apart; down the columns: place n is that of fragment n, the halves 32 rows apart.
 template <int B, bool DOWN>
-__device__ __forceinline__ bf16x8 fragment(const bf16_t* tile, int x, int ks, int fl, int fk) {
+__device__ __forceinline__ LdsPtr fragment_place(LdsPtr tile, int x, int n, int fl, int fk) {
+    if constexpr (!DOWN) return tile + slot_at(x + fl, n * 4 + fk);
+    else return tile + pair_at<B>(fk * 8 + (fl >> 2), (x >> 4) + n) + (fl & 3) * 4;
+}
+// k = 32 ks + 8 fk + 0..7 of the fragment
+template <int B, bool DOWN>
+__device__ __forceinline__ bf16x8 fragment(LdsPtr at) {
     if constexpr (!DOWN) {
-        return *reinterpret_cast<const bf16x8*>(tile + slot_at(x + fl, ks * 4 + fk));
+        return *(__attribute__((address_space(3))) const bf16x8*)at;
     } else {
         bf16x8 v;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int k = ks * 32 + fk * 8 + h * 4 + (fl >> 2);
             const bf16x4 y = __builtin_bit_cast(
-                bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(S2AG_LDS_PTR(s16x4_t, tile + pair_at<B>(k, x >> 4) + (fl & 3) * 4)));
+                bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(at + h * 4 * B)));
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[h * 4 + e] = y[e];
         }
@@ -334,6 +341,7 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
     constexpr int STAGE = (BR + BQ) * BK;
     constexpr bool RK = END == STORE, QK = END == STORE || END == ACCUM;       // k runs down the operand's columns
     extern __shared__ __attribute__((aligned(16))) bf16_t lds[];
+    const LdsPtr r_tiles = (LdsPtr)lds, q_tiles = r_tiles + 2 * BR * BK;       // two of each
     bf16_t* const scratch = lds + 2 * STAGE;                                   // 64 x BQ, for the ends
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -408,9 +416,17 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
         }
         return buffer(at, left > 0 ? (unsigned)bytes : 0u);
     };
+    int whole = 0;                                               // stages from here on that no end of a column cuts
+    const unsigned long long r_step = 2ULL * BK * p.r.ld, q_step = 2ULL * BK * p.q.ld;
     auto descriptors = [&]() {
         rr = descriptor(p.r, piece_r(PRECISE ? pair : 5), RK, r0_next, p.r_rows, BR, p.r_deep, p.r_cols);
         qr = descriptor(p.q, piece_q(PRECISE ? pair : 5), QK, c0_next, p.q_rows, BQ, p.q_deep, p.q_cols);
+        if (QK) whole = (int)((RK && p.r_deep < p.q_deep ? p.r_deep : p.q_deep) / BK) - kk;
+    };
+    auto move = [](u32x4& d, unsigned long long bytes) {
+        const unsigned long long at = (d[0] | (unsigned long long)d[1] << 32) + bytes;
+        d[0] = (unsigned)at;
+        d[1] = (unsigned)(at >> 32);
     };
     auto next_tile = [&]() {
         left = 0;
@@ -430,56 +446,81 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
         if (--left <= 0) {
             next_tile();
         } else {
-            const bool wrap = ++kk == ts.kt;
-            if (wrap) {
+            if (++kk == ts.kt) {
                 kk = 0;
                 ++pair;
+                descriptors();
+            } else if (QK) {                                     // down the columns: few scalar instructions, the matrix unit waits for them
+                if (--whole > 0) {
+                    if (RK) move(rr, r_step);
+                    move(qr, q_step);
+                } else {
+                    descriptors();
+                }
             }
-            if (RK || QK || wrap) descriptors();
         }
     };
     // requests [from, from + n) of the LR + LQ of a stage
     auto issue = [&](int buf, int from, int n) {
-        bf16_t* s = lds + buf * STAGE + wave * 512;
+        const LdsPtr r_to = r_tiles + buf * (BR * BK) + wave * 512, q_to = q_tiles + buf * (BQ * BK) + wave * 512;
         const int off = kk * (BK * 2);                           // (down the columns the descriptor moves)
 #pragma unroll
         for (int i = from; i < from + n; ++i) {
-            if (i < LR) to_lds(rr, s + i * NT * 8, r_off[i < LR ? i : 0], RK ? 0 : off);
-            else to_lds(qr, s + BR * BK + (i - LR) * NT * 8, q_off[i < LR ? 0 : i - LR], QK ? 0 : off);
+            if (i < LR) to_lds(rr, r_to + i * NT * 8, r_off[i < LR ? i : 0], RK ? 0 : off);
+            else to_lds(qr, q_to + (i - LR) * NT * 8, q_off[i < LR ? 0 : i - LR], QK ? 0 : off);
         }
     };
 
     f32x4 acc[QI][RI];
     const int fl = lane & 15, fk = lane >> 4;
-    // fragments [from, to) of half ks of a stage
-    auto read_q = [&](bf16x8 (&a)[QI], int buf, int ks, int from, int to) {
+    // The places in the stage that is read; on to the other one of the two and back.  (As few vector instructions as can be: the
+    // matrix unit waits for them too.)
+    constexpr int RN = RK ? RI : 2, QN = QK ? QI : 2;
+    LdsPtr r_place[RN], q_place[QN];
 #pragma unroll
-        for (int i = from; i < to; ++i) a[i] = fragment<BQ, QK>(lds + buf * STAGE + BR * BK, wq * TQ + i * 16, ks, fl, fk);
-    };
-    auto read_r = [&](bf16x8 (&b)[RI], int buf, int ks, int from, int to) {
+    for (int n = 0; n < RN; ++n) r_place[n] = fragment_place<BR, RK>(r_tiles, wr * TR, n, fl, fk);
 #pragma unroll
-        for (int j = from; j < to; ++j) b[j] = fragment<BR, RK>(lds + buf * STAGE, wr * TR + j * 16, ks, fl, fk);
+    for (int n = 0; n < QN; ++n) q_place[n] = fragment_place<BQ, QK>(q_tiles, wq * TQ, n, fl, fk);
+    int r_other = BR * BK, q_other = BQ * BK;
+    auto read_q = [&](bf16x8 (&a)[QI], int ks, int i) {
+        if constexpr (QK) a[i] = fragment<BQ, QK>(q_place[i] + ks * 32 * BQ);
+        else a[i] = fragment<BQ, QK>(q_place[ks] + i * 16 * BK);
     };
-    auto multiply = [&](const bf16x8 (&a)[QI], const bf16x8 (&b)[RI], int i) {
-#pragma unroll
-        for (int j = 0; j < RI; ++j) {
-            if constexpr (RI * QI * 4 == 256) mfma_acc(acc[i][j], a[i], b[j]);
-            else acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], acc[i][j], 0, 0, 0);
-        }
+    auto read_r = [&](bf16x8 (&b)[RI], int ks, int j) {
+        if constexpr (RK) b[j] = fragment<BR, RK>(r_place[j] + ks * 32 * BR);
+        else b[j] = fragment<BR, RK>(r_place[ks] + j * 16 * BK);
     };
-
+    auto multiply = [&](const bf16x8& a, const bf16x8& b, int i, int j) {
+        if constexpr (RI * QI * 4 == 256) mfma_acc(acc[i][j], a, b);
+        else acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc[i][j], 0, 0, 0);
+    };
     auto value = [&](int i, int j, int e) {
         if constexpr (RI * QI * 4 == 256) return acc_read(acc[i][j][e]);
         else return acc[i][j][e];
     };
 
-    // Two stages in LDS, two halves of a stage in registers, matrix instructions in QI groups a half.  While the first half of a
-    // stage is multiplied its second half is read, R before Q: when every wavefront has its part of R, R's place is free and the
-    // R of the stage after the next is requested; in the middle of the stage all of it is read, the next stage (requested a
-    // stage ago) has landed, and while the second half is multiplied the first half of the next stage is read and the Q of the
-    // stage after it is requested.  A request keeps a wavefront's issue busy for as long as eight of its matrix instructions may
-    // take: one or two a group; twice as many at half the places cost a tenth of the rate.
-    constexpr int G = QI, EARLY = G / 2 - 1, RN = G - EARLY, RB = RI / (G / 4), QB = QI / (G / 4);
+    // Two stages in LDS, two halves of a stage in registers.  While the first half of a stage is multiplied its second half is
+    // read, R before Q: when every wavefront has its part of R, R's place is free and the R of the stage after the next is
+    // requested; in the middle of the stage all of it is read, the next stage (requested a stage ago) has landed, and while the
+    // second half is multiplied the first half of the next stage is read and the Q of the stage after it is requested.
+    // A wavefront is alone on its matrix unit, which waits for whatever stands between two of its instructions for longer than
+    // one of them takes.  So reads and requests are dealt out singly: a fragment behind every PER-th matrix instruction of the
+    // first half of the groups (the others cover the reads' way), a request behind every RPER-th or QPER-th.
+    constexpr int G = QI, M = QI * RI, EARLY = (G / 2 - 1) * RI, PER = M / 2 / (QI + RI), RPER = (M - EARLY - 1) / LR, QPER = M / LQ;
+    static_assert(M / 2 % (QI + RI) == 0 && M % LQ == 0 && RI * PER <= EARLY, "dealing out");
+    auto deal = [&](bf16x8 (&a)[QI], bf16x8 (&b)[RI], int ks, int m) {       // what follows matrix instruction m
+        if (m < M / 2 && m % PER == 0) {
+            const int u = m / PER;
+            if (ks == 0) {                                       // (the first reads of the other stage)
+                if (RK ? u < RI : u == 0)
+                    for (int n = RK ? u : 0; n < (RK ? u + 1 : RN); ++n) r_place[n] += r_other;
+                if (QK ? u >= RI : u == RI)
+                    for (int n = QK ? u - RI : 0; n < (QK ? u - RI + 1 : QN); ++n) q_place[n] += q_other;
+            }
+            if (u < RI) read_r(b, ks, u);
+            else read_q(a, ks, u - RI);
+        }
+    };
     bf16x8 a0[QI], b0[RI], a1[QI], b1[RI];
     next_tile();
     issue(0, 0, LR + LQ);
@@ -488,8 +529,10 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
     __syncthreads();
     issue(1, 0, LR + LQ);
     advance();
-    read_r(b0, 0, 0, 0, RI);
-    read_q(a0, 0, 0, 0, QI);
+#pragma unroll
+    for (int j = 0; j < RI; ++j) read_r(b0, 0, j);
+#pragma unroll
+    for (int i = 0; i < QI; ++i) read_q(a0, 0, i);
     int buf = 0;
     for (int tile = first; tile < last; tile += step) {
         const Place t = place(tile);
@@ -500,19 +543,21 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
         settle();
         for (int n = t.it0; n < t.it1; ++n) {
 #pragma unroll
-            for (int i = 0; i < G; ++i) {
-                multiply(a0, b0, i);
-                __builtin_amdgcn_sched_barrier(0);
-                if (i < G / 4) read_r(b1, buf, 1, i * RB, (i + 1) * RB);
-                if (i == EARLY) {
-                    if constexpr (G / 4 < EARLY && !QK) asm volatile("s_waitcnt lgkmcnt(4)" ::: "memory");      // (Q's reads so far)
-                    else if constexpr (G / 4 < EARLY) asm volatile("s_waitcnt lgkmcnt(8)" ::: "memory");
+            for (int m = 0; m < M; ++m) {
+                if (m == EARLY) {
+                    // (the reads of Q that were dealt out behind R's are still out)
+                    constexpr int OUT = (EARLY / PER - RI) * (QK ? 2 : 1);
+                    static_assert(OUT == 0 || OUT == 4 || OUT == 8, "");
+                    if constexpr (OUT == 8) asm volatile("s_waitcnt lgkmcnt(8)" ::: "memory");
+                    else if constexpr (OUT == 4) asm volatile("s_waitcnt lgkmcnt(4)" ::: "memory");
                     else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                     __builtin_amdgcn_s_barrier();
                     asm volatile("s_waitcnt lgkmcnt(15)" ::: "memory");      // (keeps the requests behind the barrier)
                 }
-                if (i >= G / 4 && i < G / 2) read_q(a1, buf, 1, (i - G / 4) * QB, (i - G / 4 + 1) * QB);
-                if (i >= EARLY) issue(buf, (i - EARLY) * LR / RN, (i - EARLY + 1) * LR / RN - (i - EARLY) * LR / RN);
+                multiply(a0[m / RI], b0[m % RI], m / RI, m % RI);
+                __builtin_amdgcn_sched_barrier(0);
+                deal(a1, b1, 1, m);
+                if (m > EARLY && (m - EARLY) % RPER == 0 && (m - EARLY) / RPER <= LR) issue(buf, (m - EARLY) / RPER - 1, 1);
                 __builtin_amdgcn_sched_barrier(0);
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -522,16 +567,17 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
             __builtin_amdgcn_s_barrier();
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (keeps the reads behind the barrier)
 #pragma unroll
-            for (int i = 0; i < G; ++i) {
-                multiply(a1, b1, i);
+            for (int m = 0; m < M; ++m) {
+                multiply(a1[m / RI], b1[m % RI], m / RI, m % RI);
                 __builtin_amdgcn_sched_barrier(0);
-                if (i < G / 4) read_r(b0, buf ^ 1, 0, i * RB, (i + 1) * RB);
-                if (i >= G / 4 && i < G / 2) read_q(a0, buf ^ 1, 0, (i - G / 4) * QB, (i - G / 4 + 1) * QB);
-                issue(buf, LR + i * LQ / G, (i + 1) * LQ / G - i * LQ / G);
+                deal(a0, b0, 0, m);
+                if (m % QPER == QPER - 1) issue(buf, LR + m / QPER, 1);
                 __builtin_amdgcn_sched_barrier(0);
             }
             advance();
             buf ^= 1;
+            r_other = -r_other;
+            q_other = -q_other;
         }
         settle();
 
