@@ -176,10 +176,16 @@ __device__ __forceinline__ u32x4 buffer(const void* p, unsigned bytes) {
     return u32x4{(unsigned)a, (unsigned)(a >> 32), bytes, 0x00020000u};
 }
 
-// 16 bytes a lane from the buffer to LDS: lane l's land at dst + 16 l.  Written out, because behind the builtin the compiler lets
-// every transposing read wait for all requests that are out; no register is loaded, and the waits for LDS are the kernel's own.
 typedef __attribute__((address_space(3))) bf16_t* LdsPtr;       // (from a general pointer the compiler tests for null every time)
+
+// 16 bytes a lane from the buffer to LDS: lane l's land at dst + 16 l.
 __device__ __forceinline__ void to_lds(u32x4 from, LdsPtr dst, unsigned lane_offset, int offset) {
+    __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(from[0] | (unsigned long long)from[1] << 32), 0, (int)from[2], (int)from[3]);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)dst, 16, lane_offset, offset, 0, 0);
+}
+// The same, written out: behind the builtin the compiler lets every transposing read wait for all requests that are out.  No
+// register is loaded, and the waits for LDS are the kernel's own.  (Only where there are such reads: it costs 2 to 8 %.)
+__device__ __forceinline__ void to_lds_beside_transposing_reads(u32x4 from, LdsPtr dst, unsigned lane_offset, int offset) {
     const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)dst);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "s"(at), "v"(lane_offset), "s"(from), "s"(offset) : "memory");
 }
@@ -217,7 +223,8 @@ __device__ __forceinline__ float exp_of(float d) {
 
 // The tiles of a launch, in the order in which they are handed out; everything here is one for the workgroup.
 struct Tiles {
-    int n, splits, per, group, tiles_r, kt, total;
+    int n, splits, per, group, tiles_r, kt;
+    int stages, more;                   // of a part of k; so many parts have one more
 };
 __host__ __device__ inline int splits_of(int tiles, int most, int slots) {       // few tiles: k is split to fill the card
     const int s = tiles > 0 ? slots / tiles : 1;
@@ -361,7 +368,8 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
     ts.tiles_r = __builtin_amdgcn_readfirstlane((live + BR - 1) / BR);
     ts.splits = __builtin_amdgcn_readfirstlane(splits_of(ts.tiles_r * p.tiles_q, p.splits, p.slots));
     ts.kt = p.k_count ? __builtin_amdgcn_readfirstlane((*p.k_count + BK - 1) / BK) : p.k / BK;
-    ts.total = ts.kt * pairs;
+    ts.stages = __builtin_amdgcn_readfirstlane(ts.kt * pairs / ts.splits);
+    ts.more = ts.kt * pairs - ts.stages * ts.splits;
     ts.group = p.group;
     ts.per = p.group * p.tiles_q;
     ts.n = ts.tiles_r * p.tiles_q * ts.splits;
@@ -385,8 +393,8 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
         const int grp = __builtin_amdgcn_readfirstlane(v / ts.per), g0 = grp * ts.group, gsz = min(ts.tiles_r - g0, ts.group);
         t.r0 = (long long)__builtin_amdgcn_readfirstlane(g0 + (v - grp * ts.per) % gsz) * BR;
         t.c0 = (long long)__builtin_amdgcn_readfirstlane((v - grp * ts.per) / gsz) * BQ;
-        t.it0 = __builtin_amdgcn_readfirstlane((int)((long long)ts.total * t.split / ts.splits));
-        t.it1 = __builtin_amdgcn_readfirstlane((int)((long long)ts.total * (t.split + 1) / ts.splits));
+        t.it0 = ts.stages * t.split + min(t.split, ts.more);
+        t.it1 = t.it0 + ts.stages + (t.split < ts.more ? 1 : 0);
         return t;
     };
 
@@ -466,8 +474,12 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
         const int off = kk * (BK * 2);                           // (down the columns the descriptor moves)
 #pragma unroll
         for (int i = from; i < from + n; ++i) {
-            if (i < LR) to_lds(rr, r_to + i * NT * 8, r_off[i < LR ? i : 0], RK ? 0 : off);
-            else to_lds(qr, q_to + (i - LR) * NT * 8, q_off[i < LR ? 0 : i - LR], QK ? 0 : off);
+            const u32x4 from = i < LR ? rr : qr;
+            const LdsPtr to = i < LR ? r_to + i * NT * 8 : q_to + (i - LR) * NT * 8;
+            const unsigned lane_offset = i < LR ? r_off[i < LR ? i : 0] : q_off[i < LR ? 0 : i - LR];
+            const int move = (i < LR ? RK : QK) ? 0 : off;
+            if constexpr (QK) to_lds_beside_transposing_reads(from, to, lane_offset, move);
+            else to_lds(from, to, lane_offset, move);
         }
     };
 
@@ -522,13 +534,14 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
         }
     };
     bf16x8 a0[QI], b0[RI], a1[QI], b1[RI];
-    next_tile();
-    issue(0, 0, LR + LQ);
-    advance();
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    issue(1, 0, LR + LQ);
-    advance();
+#pragma unroll 1
+    for (int b = 0; b < 2; ++b) {
+        advance();
+        issue(b, 0, LR + LQ);
+        if (b) break;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    }
 #pragma unroll
     for (int j = 0; j < RI; ++j) read_r(b0, 0, j);
 #pragma unroll
@@ -542,9 +555,10 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
             for (int j = 0; j < RI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         settle();
         for (int n = t.it0; n < t.it1; ++n) {
-#pragma unroll
-            for (int m = 0; m < M; ++m) {
-                if (m == EARLY) {
+            each<0, M, 1>([&](auto at_m) {
+                constexpr int m = decltype(at_m)::value;
+                if constexpr (m == (M > 16 ? EARLY : 0)) advance();          // (scalar work, where little or nothing waits for it)
+                if constexpr (m == EARLY) {
                     // (the reads of Q that were dealt out behind R's are still out)
                     constexpr int OUT = (EARLY / PER - RI) * (QK ? 2 : 1);
                     static_assert(OUT == 0 || OUT == 4 || OUT == 8, "");
@@ -559,22 +573,21 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
                 deal(a1, b1, 1, m);
                 if (m > EARLY && (m - EARLY) % RPER == 0 && (m - EARLY) / RPER <= LR) issue(buf, (m - EARLY) / RPER - 1, 1);
                 __builtin_amdgcn_sched_barrier(0);
-            }
+            });
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             if constexpr (LR == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
             else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
             static_assert(LR == 8 || LR == 4, "the requests for R of the stage after the next stay out");
             __builtin_amdgcn_s_barrier();
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (keeps the reads behind the barrier)
-#pragma unroll
-            for (int m = 0; m < M; ++m) {
+            each<0, M, 1>([&](auto at_m) {
+                constexpr int m = decltype(at_m)::value;
                 multiply(a1[m / RI], b1[m % RI], m / RI, m % RI);
                 __builtin_amdgcn_sched_barrier(0);
                 deal(a0, b0, 0, m);
                 if (m % QPER == QPER - 1) issue(buf, LR + m / QPER, 1);
                 __builtin_amdgcn_sched_barrier(0);
-            }
-            advance();
+            });
             buf ^= 1;
             r_other = -r_other;
             q_other = -q_other;
@@ -604,10 +617,11 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
                         for (int i = 0; i < QI * 4; ++i)
                             if (i / 4 * 16 + i % 4 >= words) z[i] = -INFINITY;
                     }
-                    if (at < (unsigned)TQ) {
+                    if (at < (unsigned)TQ && (at & 12) == 0) {       // (four columns of sixteen are the lane's)
+                        float logit = z[0];
 #pragma unroll
-                        for (int i = 0; i < QI * 4; ++i)
-                            if (at == (unsigned)(i / 4 * 16 + i % 4)) p.target_logit[row] = z[i];
+                        for (int i = 1; i < QI * 4; ++i) logit = at == (unsigned)(i / 4 * 16 + i % 4) ? z[i] : logit;
+                        p.target_logit[row] = logit;
                     }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) m4[e] = z[e];
@@ -659,10 +673,9 @@ __global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
                         const unsigned place = (unsigned)(tgt[jj + j] - word0);      // the target's, if it is the lane's
 #pragma unroll
                         for (int i = 0; i < QI * 4; ++i) g[j][i] = exp_of<PRECISE>(value(i / 4, jj + j, i % 4) - lse[jj + j]);
-                        if (place < (unsigned)TQ) {
+                        if (place < (unsigned)TQ && (place & 12) == 0) {
 #pragma unroll
-                            for (int i = 0; i < QI * 4; ++i)
-                                if (place == (unsigned)(i / 4 * 16 + i % 4)) g[j][i] -= 1.f;
+                            for (int i = 0; i < QI * 4; ++i) g[j][i] -= place == (unsigned)(i / 4 * 16 + i % 4) ? 1.f : 0.f;
                         }
                         if (edge) {
 #pragma unroll

@@ -443,6 +443,13 @@ static inline void emu_buffer_to_lds(emu::u32x4_t from, P lds, unsigned voffset,
     }
     memcpy((char*)(uintptr_t)lds + 16 * emu::g_cur->lane, &v, 16);
 }
+template <typename P>
+static inline void emu_raw_ptr_buffer_load_lds(emu_buffer_rsrc r, P lds, unsigned size, unsigned voffset, unsigned soffset, unsigned inst, unsigned) {
+    if (size != 16) { fprintf(stderr, "[s2ag emu] buffer load to LDS of %u bytes\n", size); abort(); }
+    const unsigned long long a = (unsigned long long)(uintptr_t)r.base;
+    emu_buffer_to_lds(emu::u32x4_t{(unsigned)a, (unsigned)(a >> 32), r.num_records, 0u}, lds, voffset, soffset + inst);
+}
+#define __builtin_amdgcn_raw_ptr_buffer_load_lds(r, lds, size, voff, soff, inst, aux) emu_raw_ptr_buffer_load_lds(r, lds, size, voff, soff, inst, aux)
 #define __builtin_amdgcn_readlane(v, l) __shfl(v, l)
 #define __builtin_amdgcn_sched_barrier(x) ((void)0)
 #define __builtin_amdgcn_sched_group_barrier(a, b, c) ((void)0)
