@@ -341,7 +341,7 @@ __device__ __forceinline__ bf16x8 fragment(LdsPtr at) {
 }
 
 template <int BR, int BQ, int WR, int WQ, End END, bool PRECISE>
-__global__ __launch_bounds__(64 * WR * WQ, 1) void product_k(Product p) {
+__global__ __launch_bounds__(64 * WR * WQ, BR == 256 ? 1 : 2) void product_k(Product p) {
     constexpr int NT = 64 * WR * WQ;
     constexpr int TR = BR / WR, TQ = BQ / WQ, RI = TR / 16, QI = TQ / 16;      // a wavefront's part
     constexpr int LR = BR * 8 / NT, LQ = BQ * 8 / NT;                          // 16-byte loads per thread and stage
