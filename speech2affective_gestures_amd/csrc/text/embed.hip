@@ -481,7 +481,7 @@ int launch_sums(const unsigned* keys, const int* pos, int n, const void* dy, lon
     const long long blocks = ((long long)tiles * chunks + 3) / 4;
     const int zero_rows = n_entries < 65536 ? 16 : 64;            // a small table: more wavefronts
     const long long zero = touched ? (n_entries + 4 * zero_rows - 1) / (4 * zero_rows) : 0;
-    if (blocks + zero > 0x7fffffffLL) return S2AG_E_UNSUPPORTED;
+    if (blocks + zero > 0x7fffffffLL || (long long)tiles * chunks > 0x7fffffffLL) return S2AG_E_UNSUPPORTED;
     if (blocks + zero)
         hipLaunchKernelGGL(sum_k<T>, dim3((unsigned)(blocks + zero)), dim3(256), 0, st, keys, pos, n, static_cast<const T*>(dy), ldy, dim,
                            n_entries, scale, static_cast<T*>(dtable), accumulate, tl, tiles, chunks, pieces, touched, (int)blocks, zero_rows);

@@ -181,6 +181,7 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float 
         norm = torch.empty((), dtype=torch.float32, device=dev)
         L.check(lib.s2ag_clip_grads(table, k, max_norm, int(inf), C.c_void_p(partials.data_ptr()), C.c_void_p(norm.data_ptr()),
                                     C.c_void_p(torch.cuda.current_stream().cuda_stream)), 'clip_grads')
+    torch.autograd.graph.increment_version(results)                # written behind torch's back
     return norm
 
 

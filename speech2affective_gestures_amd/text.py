@@ -224,6 +224,9 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, ignore_index
         raise TypeError(f'{what}: x is {x.dtype} and weight {weight.dtype}')
     if x.dim() < 1 or x.shape[-1] != weight.shape[1] or x.shape[:-1] != target.shape:
         raise ValueError(f'{what}: x {tuple(x.shape)}, weight {tuple(weight.shape)} and target {tuple(target.shape)} do not go together')
+    ignore_index = int(ignore_index)
+    if not -(1 << 63) <= ignore_index < 1 << 63:
+        raise ValueError(f'{what}: ignore_index {ignore_index} is no int64')
     if target.numel() > MAX_ROWS or weight.shape[0] > MAX_WORDS or weight.shape[1] > (1 << 20):
         raise ValueError(f'{what}: at most {MAX_ROWS} rows, {MAX_WORDS} words and {1 << 20} columns')
-    return _LinearCrossEntropy.apply(x, weight, target, int(ignore_index), _REDUCTIONS[reduction])
+    return _LinearCrossEntropy.apply(x, weight, target, ignore_index, _REDUCTIONS[reduction])

@@ -537,3 +537,193 @@ def test_clip_grads_refusals(S):
                        (([t[:5], t[5:]], 1.0), dict(out=[t[5:], t[:5]]), ValueError)]:
         with pytest.raises(err):
             f(*a, **kw)
+
+
+# ---- streams, graphs, large tensors, a run of them together ---------------------------------------------------------------------
+def text_step(S, x, w, ids, table, target, grads, max_norm=0.5):
+    """One pass of each operator with all gradients; tensors of a few hundred rows."""
+    y = S['ops'].embedding_sorted(ids, table, scale=3.0)
+    (dt,) = torch.autograd.grad(y, (table,), x.detach())
+    loss = S['ops'].linear_cross_entropy(x, w, target)
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    out = [torch.empty_like(g) for g in grads]
+    norm = S['optim'].clip_grads(grads, max_norm, out=out)
+    return [y.detach(), dt, loss.detach(), dx, dw, norm] + out
+
+
+def text_inputs(seed, dtype=torch.bfloat16):
+    g = torch.Generator().manual_seed(seed)
+    n, d, v = 300, 72, 1500
+    x, w, table = (torch.randn(*s, generator=g).to(dtype).cuda() for s in ((n, d), (v, d), (v, d)))
+    ids, target = torch.randint(0, v, (n,), generator=g), torch.randint(0, v, (n,), generator=g)
+    target[::7] = IGNORE
+    ids[::2] = 0
+    return x, w, ids.cuda(), table, target.cuda(), [torch.randn(700, generator=g).cuda(), torch.randn(3, 5, generator=g).to(dtype).cuda()]
+
+
+@pytest.mark.skipif(EMU, reason='graphs and streams are not modelled')
+@pytest.mark.parametrize('dtype', list(DTYPES))
+def test_text_operators_in_captured_graphs(S, dtype):
+    """Forward and backward of all three captured twice on the same inputs' buffers; replays in turn, with new inputs and eager work
+    between them, give the eager results' bits."""
+    static = text_inputs(1, DTYPES[dtype])
+    live = [t for t in static[:5]] + static[5]
+
+    def leaves():
+        x, w, ids, table, target, grads = static
+        return x.detach().requires_grad_(True), w.detach().requires_grad_(True), ids, table.detach().requires_grad_(True), target, grads
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        text_step(S, *leaves())
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = text_step(S, *leaves())
+        graphs.append((g, out))
+    for seed in range(2, 6):
+        fresh = text_inputs(seed, DTYPES[dtype])
+        want = text_step(S, *[t.requires_grad_(True) if i in (0, 1, 3) else t for i, t in enumerate(fresh)])
+        for a, b in zip(live, [t for t in fresh[:5]] + fresh[5]):
+            a.copy_(b.detach())
+        for g, out in (graphs[seed % 2], graphs[1 - seed % 2]):
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.skipif(EMU, reason='graphs and streams are not modelled')
+def test_text_operators_on_two_streams_at_once(S):
+    ins = [text_inputs(s) for s in (11, 12)]
+    for i in ins:
+        for k in (0, 1, 3):
+            i[k].requires_grad_(True)
+    want = [text_step(S, *i) for i in ins]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in ins]
+    got = [None, None]
+    for rep in range(3):
+        for k, st in enumerate(streams):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                got[k] = text_step(S, *ins[k])
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.skipif(EMU, reason='gigabytes')
+def test_embedding_sorted_offsets_beyond_32_bits(S):
+    entries, dim = (1 << 20) + 40001, 2080                 # 2.26e9 elements
+    t = torch.zeros(entries, dim, dtype=torch.bfloat16, device='cuda')
+    rows = torch.tensor([0, 5, 1 << 20, entries - 2, entries - 1, entries - 1])
+    g = torch.Generator().manual_seed(1)
+    vals = torch.randn(5, dim, generator=g).to(torch.bfloat16)
+    t[rows[:5].cuda()] = vals.cuda()
+    t.requires_grad_(True)
+    ids = rows.repeat(40).cuda()
+    y = S['ops'].embedding_sorted(ids, t)
+    assert torch.equal(y[:5].detach().cpu(), vals) and torch.equal(y[5].detach().cpu(), vals[4])
+    (dt,) = torch.autograd.grad(y, (t,), torch.ones_like(y))
+    assert torch.equal(dt[rows.cuda()].float().cpu(), torch.tensor([40., 40., 40., 40., 80., 80.])[:, None].expand(6, dim))
+    assert float(dt.sum(dtype=torch.float64)) == 240.0 * dim
+
+
+@pytest.mark.skipif(EMU, reason='gigabytes')
+def test_clip_grads_offsets_beyond_32_bits(S):
+    n = (1 << 32) + 70003
+    t = torch.full((n,), 2.0 ** -10, dtype=torch.bfloat16, device='cuda')
+    t[-1] = 8.0
+    norm = math.sqrt((n - 1) * 2.0 ** -20 + 64.0)
+    got = S['optim'].clip_grads([t], norm / 2)
+    assert abs(float(got) - norm) <= 2 * U * norm
+    assert float(t[0]) == 2.0 ** -11 and float(t[(1 << 32) + 5]) == 2.0 ** -11 and float(t[-1]) == 4.0
+    assert float(t[:-1].max()) == 2.0 ** -11 == float(t[:-1].min())
+
+
+@pytest.mark.skipif(EMU, reason='gigabytes')
+def test_linear_cross_entropy_offsets_beyond_32_bits(S):
+    """The most rows there may be, 2.3e9 elements of x: the last rows as they are by themselves, to the bounds."""
+    n, d, v = 1 << 21, 1088, 40
+    g = torch.Generator().manual_seed(21)
+    w = torch.randn(v, d, generator=g) * 0.05
+    w = w.to(torch.bfloat16)
+    x = torch.randn(512, d, generator=g).to(torch.bfloat16)
+    t = torch.randint(0, v, (512,), generator=g)
+    xg = x.cuda().repeat(n // 512, 1).requires_grad_(True)
+    loss = S['ops'].linear_cross_entropy(xg, w.cuda(), t.cuda().repeat(n // 512), reduction='none')
+    (l, lb), (dx, dxb), _ = lce_reference(x, w, t, torch.ones(512), 'none')
+    within(loss[-512:], l, lb)
+    (gx,) = torch.autograd.grad(loss, (xg,), torch.ones_like(loss))
+    within(gx[-512:], dx, dxb)
+    within(gx[:512], dx, dxb)
+    del xg, gx, loss
+
+
+def test_linear_cross_entropy_kept_graph_and_one_row(S):
+    x, w, t, g = lce_case(40, 24, 100, 'fp32', 0.2)
+    xg, wg = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    loss = S['ops'].linear_cross_entropy(xg, wg, t.cuda())
+    a = torch.autograd.grad(loss, (xg, wg), retain_graph=True)
+    b = torch.autograd.grad(loss, (xg, wg))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    one = S['ops'].linear_cross_entropy(xg[3], wg, t.cuda()[3], reduction='none')       # a vector and a number
+    assert one.shape == () and torch.equal(one.detach(), S['ops'].linear_cross_entropy(xg, wg, t.cuda(), reduction='none')[3].detach())
+
+
+def test_linear_cross_entropy_changed_weight_is_noticed(S):
+    """A weight that is changed between the passes: torch's own error, not gradients of two different weights."""
+    x, w, t, g = lce_case(10, 24, 30, 'fp32', 0.0)
+    xg, wg = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    loss = S['ops'].linear_cross_entropy(xg, wg, t.cuda())
+    with torch.no_grad():
+        wg += 1.0
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        loss.backward()
+
+
+def test_clip_grads_counts_as_a_change(S):
+    t = torch.ones(10).cuda()
+    before = t._version
+    S['optim'].clip_grads([t], 0.1)
+    assert t._version > before
+
+
+def test_a_step_of_a_text_model(S):
+    """The operators as they are used: scaled embedding, a layer of the framework's own, cross entropy over the tied table, the norm
+    of all gradients in the arena, clipping, Adam -- against the same step in 64 bits."""
+    ops, optim = S['ops'], S['optim']
+    g = torch.Generator().manual_seed(31)
+    v, d, B, T = 700, 64, 5, 34
+    table, mix, bias = torch.randn(v, d, generator=g) * 0.3, torch.randn(d, d, generator=g) / 8, torch.randn(d, generator=g) * 0.1
+    ids = torch.randint(0, v, (B, T), generator=g)
+    ids[torch.rand(B, T, generator=g) < 0.5] = 0
+    target = torch.roll(ids, -1, 1).clone()
+    target[:, -1] = IGNORE
+    target[target == 0] = IGNORE
+    E, M, b = (torch.nn.Parameter(t.cuda()) for t in (table, mix, bias))
+    arena = optim.ParamArena([E, M, b])
+    adam = optim.FusedAdam(arena, lr=1e-2, betas=(0.9, 0.999), eps=1e-2)
+    adam.zero_grad()
+    h = ops.linear(ops.embedding_sorted(ids.cuda(), E, scale=8.0).view(B * T, d), M, b)
+    loss = ops.linear_cross_entropy(h.view(B, T, d), E, target.cuda())
+    loss.backward()
+    norm = adam.clip_grad_norm(0.5)
+    grads = [p.grad.clone() for p in (E, M, b)]
+    adam.step()
+    Er, Mr, br = (t.double().requires_grad_(True) for t in (table, mix, bias))
+    hr = torch.nn.functional.linear(Er[ids.view(-1)] * 8.0, Mr, br)
+    lr_ = torch.nn.functional.cross_entropy(hr @ Er.t(), target.view(-1), ignore_index=IGNORE)
+    ref = torch.autograd.grad(lr_, (Er, Mr, br))
+    nr = math.sqrt(sum(float(t.square().sum()) for t in ref))
+    tol = 1e-4                                             # the layer's own, relative to the largest element (tests/test_gpu_ops.py)
+    assert abs(float(loss) - float(lr_)) < tol * float(lr_) and abs(float(norm) - nr) < tol * nr and nr > 0.5
+    for p, gr, r, start in zip((E, M, b), grads, ref, (table, mix, bias)):
+        r = r * min(1.0, 0.5 / (nr + 1e-6))
+        err = tol * float(r.abs().max())
+        assert float((gr.cpu().double() - r).abs().max()) < err
+        # Adam's first step: lr g / (|g| + eps), which moves by lr / eps of what g is off; the moments' bias corrections cancel
+        want = start.double() - 1e-2 * r / (r.abs() + 1e-2)
+        assert float((p.detach().cpu().double() - want).abs().max()) < 1e-2 / 1e-2 * err + 1e-6
