@@ -14,15 +14,23 @@
 // The rows that are ignored are left out of every product: the others are packed in front (rowmap), their number stays on the
 // device, and the tiles behind it end at once.
 //
-// fp32 operands are taken as three bf16 pieces (v = p0 + p1 + p2 to 2^-25) and the six products of pieces that matter at fp32's
-// own rounding: still more than twice the rate of the f32 matrix instructions.  bf16 operands need one product; there G is
-// rounded to bf16 (2^-9 of each value; sums stay in fp32), without its factor g where that is one number for all rows.
+// fp32 operands are taken in pieces on the same instructions, at more than the rate of the f32 ones.  For the logits as two
+// halves of 11 bits each (a power of two to every row, so that its largest value is near the top of the type's range): three
+// products; the fourth is 2^-22 of the whole, as is what the halves leave (2^-39 of the row's largest value where that is more,
+// for values below 2^-17 of it).  Six products of bf16 pieces took 32 us for the logits of 136 rows and 20 000 words of 300
+// values, these take 22.  For the gradient's products as three bf16 pieces (v = p0 + p1 + p2 to 2^-25) and the six products that
+// matter at fp32's own rounding: G has values of many magnitudes in a row, which bf16's range holds and a half's does not.
+// bf16 operands need one product; there G is rounded to bf16 (2^-9 of each value; sums stay in fp32), without its factor g where
+// that is one number for all rows.
 #include "text_common.h"
 #include <type_traits>
 
 namespace {
 using namespace s2ag;
 using namespace s2ag::text;
+
+typedef _Float16 f16_t;
+typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int BK = 64;                  // k of a stage: 128-byte rows in LDS, eight 16-byte slots
 constexpr int ROWS = 256;               // packed rows are padded to this
@@ -89,38 +97,78 @@ __device__ __forceinline__ void split3(float v, bf16_t* q) {
     q[2] = (bf16_t)(r1 - (float)q[1]);
 }
 
-// dst[r][0..kp) from row rowmap[r] (or r) of src, zeros behind column dim and for r >= count (up to `rows`).  An infinity
-// leaves NaN in the second piece, as its products would anyway.
+// Rows of the packed operand that are written: all of W, or the live rows of X and zeros up to a multiple of 256.
+__device__ __forceinline__ long long packed_rows(const int* count, long long rows, long long* live) {
+    *live = count ? (long long)*count : rows;
+    return count ? (*live + ROWS - 1) / ROWS * ROWS : rows;
+}
 template <typename T>
-__global__ __launch_bounds__(256) void pack_k(const T* __restrict__ src, long long ld, int dim, const int* __restrict__ rowmap,
-                                              const int* __restrict__ count, long long rows, bf16_t* __restrict__ dst, int kp,
-                                              long long plane) {
-    const long long live = count ? (long long)*count : rows;
-    const long long end = count ? (live + ROWS - 1) / ROWS * ROWS : rows;
+__device__ __forceinline__ void load8(const T* s, int c, int dim, bool in, float* v) {
+    if (in && c + 8 <= dim) {
+        for (int j = 0; j < 8; j += Vec<T>::N) Vec<T>::load_any(s + c + j, v + j);
+    } else {
+        for (int j = 0; j < 8; ++j) v[j] = in && c + j < dim ? (float)s[c + j] : 0.f;
+    }
+}
+
+// dst[r][0..kp) from row rowmap[r] (or r) of src, zeros behind column dim
+__global__ __launch_bounds__(256) void pack_k(const bf16_t* __restrict__ src, long long ld, int dim, const int* __restrict__ rowmap,
+                                              const int* __restrict__ count, long long rows, bf16_t* __restrict__ dst, int kp) {
+    long long live;
+    const long long end = packed_rows(count, rows, &live);
     const int groups = kp / 8;
     const long long total = end * groups;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
         const long long r = i / groups;
         const int c = (int)(i - r * groups) * 8;
         const bool in = r < live;
-        const T* s = src + (in ? (rowmap ? (long long)rowmap[r] : r) : 0) * ld;
-        bf16x8 q[3];
         float v[8];
-        if (in && c + 8 <= dim) {
-            for (int j = 0; j < 8; j += Vec<T>::N) Vec<T>::load_any(s + c + j, v + j);
-        } else {
-            for (int j = 0; j < 8; ++j) v[j] = in && c + j < dim ? (float)s[c + j] : 0.f;
+        load8(src + (in ? (rowmap ? (long long)rowmap[r] : r) : 0) * ld, c, dim, in, v);
+        Vec<bf16_t>::store(dst + r * kp + c, v);
+    }
+}
+
+// The same of fp32, a wavefront to a row: two halves, the row times 2^-power[r] of them, and three bf16 pieces if they are wanted.
+// An infinity leaves NaN in the pieces behind it, as its products would anyway.
+__global__ __launch_bounds__(256) void pack32_k(const float* __restrict__ src, long long ld, int dim, const int* __restrict__ rowmap,
+                                                const int* __restrict__ count, long long rows, int kp, f16_t* __restrict__ halves,
+                                                int* __restrict__ power, bf16_t* __restrict__ pieces, long long plane) {
+    long long live;
+    const long long end = packed_rows(count, rows, &live);
+    const int lane = threadIdx.x & 63;
+    for (long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); r < end; r += (long long)gridDim.x * 4) {
+        const bool in = r < live;
+        const float* s = src + (in ? (rowmap ? (long long)rowmap[r] : r) : 0) * ld;
+        float top = 0.f;
+        for (int c = lane * 8; c < kp; c += 512) {
+            float v[8];
+            load8(s, c, dim, in, v);
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
         }
-        for (int j = 0; j < 8; ++j) {
-            if constexpr (sizeof(T) == 2) {
-                q[0][j] = (bf16_t)v[j];
-            } else {
+        for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+        int up = 0;
+        if (top > 0.f && top < INFINITY) {
+            frexpf(top, &up);
+            up = 15 - up;                                        // the largest value to 2^14 .. 2^15
+        }
+        if (lane == 0) power[r] = -up;
+        for (int c = lane * 8; c < kp; c += 512) {
+            float v[8];
+            load8(s, c, dim, in, v);
+            f16x8 h[2];
+            bf16x8 q[3];
+            for (int j = 0; j < 8; ++j) {
+                const float t = ldexpf(v[j], up);
+                h[0][j] = (f16_t)t;
+                h[1][j] = (f16_t)(t - (float)h[0][j]);           // (the difference is exact)
                 bf16_t p[3];
                 split3(v[j], p);
                 for (int k = 0; k < 3; ++k) q[k][j] = p[k];
             }
+            for (int k = 0; k < 2; ++k) *reinterpret_cast<f16x8*>(halves + k * plane + r * kp + c) = h[k];
+            if (pieces)
+                for (int k = 0; k < 3; ++k) *reinterpret_cast<bf16x8*>(pieces + k * plane + r * kp + c) = q[k];
         }
-        for (int k = 0; k < (sizeof(T) == 2 ? 1 : 3); ++k) *reinterpret_cast<bf16x8*>(dst + k * plane + r * kp + c) = q[k];
     }
 }
 
@@ -136,7 +184,9 @@ struct Product {
     int k;                              // of one pair of pieces, a multiple of 64
     const int* k_count;                 // not null: k is this, rounded up to 64
     const int* r_count;                 // not null: rows of R that matter
-    int pairs;                          // 1, or 6 of three pieces
+    bool fp32;                          // operands in pieces
+    // STATS, GRADS of fp32: rows of R and Q are 2^power of what is multiplied
+    const int *r_power, *q_power;
     int tiles_q, group;
     int splits, slots;                  // the most parts of k; workgroups that run at a time
     // STATS: max and sum of exponentials [tile_q][padded rows], logit of the target
@@ -159,9 +209,10 @@ struct Product {
     int mean;
 };
 
-// pairs of pieces, the smallest products first: (0, 2) (1, 1) (2, 0) (0, 1) (1, 0) (0, 0), two bits each
-__device__ __forceinline__ int piece_r(int pair) { return (0x124 >> (2 * pair)) & 3; }
-__device__ __forceinline__ int piece_q(int pair) { return (0x046 >> (2 * pair)) & 3; }
+// Pairs of pieces, the smallest products first, two bits each: (0, 2) (1, 1) (2, 0) (0, 1) (1, 0) (0, 0) of three, (0, 1) (1, 0)
+// (0, 0) of two, (0, 0) of one.
+template <int PAIRS> __device__ __forceinline__ int piece_r(int pair) { return PAIRS == 1 ? 0 : ((PAIRS == 6 ? 0x124 : 0x04) >> (2 * pair)) & 3; }
+template <int PAIRS> __device__ __forceinline__ int piece_q(int pair) { return PAIRS == 1 ? 0 : ((PAIRS == 6 ? 0x046 : 0x01) >> (2 * pair)) & 3; }
 
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 #define S2AG_LDS_PTR(type, p) ((__attribute__((address_space(3))) type*)(p))
@@ -195,6 +246,9 @@ __device__ __forceinline__ void to_lds_beside_transposing_reads(u32x4 from, LdsP
 // and the first use of a result, and between the zeros and the first of them.
 __device__ __forceinline__ void mfma_acc(f32x4& c, bf16x8 a, bf16x8 b) {
     asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void mfma_acc_halves(f32x4& c, bf16x8 a, bf16x8 b) {
+    asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
 // One of its values, read where it is used (the compiler would read all 256 at once and not find registers for them).
 __device__ __forceinline__ float acc_read(float a) {
@@ -353,7 +407,8 @@ __global__ __launch_bounds__(64 * WR * WQ, BR == 256 ? 1 : 2) void product_k(Pro
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave / WQ, wq = wave % WQ;
-    constexpr int pairs = PRECISE ? 6 : 1;
+    constexpr bool HALVES = PRECISE && (END == STATS || END == GRADS);
+    constexpr int pairs = HALVES ? 3 : PRECISE ? 6 : 1;
     // (read here: a load that is still out behind the end of a tile would be waited for in every stage of the next one)
     float f = 1.f;
     if constexpr (END == STORE) {
@@ -427,8 +482,8 @@ __global__ __launch_bounds__(64 * WR * WQ, BR == 256 ? 1 : 2) void product_k(Pro
     int whole = 0;                                               // stages from here on that no end of a column cuts
     const unsigned long long r_step = 2ULL * BK * p.r.ld, q_step = 2ULL * BK * p.q.ld;
     auto descriptors = [&]() {
-        rr = descriptor(p.r, piece_r(PRECISE ? pair : 5), RK, r0_next, p.r_rows, BR, p.r_deep, p.r_cols);
-        qr = descriptor(p.q, piece_q(PRECISE ? pair : 5), QK, c0_next, p.q_rows, BQ, p.q_deep, p.q_cols);
+        rr = descriptor(p.r, piece_r<pairs>(pair), RK, r0_next, p.r_rows, BR, p.r_deep, p.r_cols);
+        qr = descriptor(p.q, piece_q<pairs>(pair), QK, c0_next, p.q_rows, BQ, p.q_deep, p.q_cols);
         if (QK) whole = (int)((RK && p.r_deep < p.q_deep ? p.r_deep : p.q_deep) / BK) - kk;
     };
     auto move = [](u32x4& d, unsigned long long bytes) {
@@ -503,7 +558,9 @@ __global__ __launch_bounds__(64 * WR * WQ, BR == 256 ? 1 : 2) void product_k(Pro
         else b[j] = fragment<BR, RK>(r_place[ks] + j * 16 * BK);
     };
     auto multiply = [&](const bf16x8& a, const bf16x8& b, int i, int j) {
-        if constexpr (RI * QI * 4 == 256) mfma_acc(acc[i][j], a, b);
+        if constexpr (RI * QI * 4 == 256 && HALVES) mfma_acc_halves(acc[i][j], a, b);
+        else if constexpr (RI * QI * 4 == 256) mfma_acc(acc[i][j], a, b);
+        else if constexpr (HALVES) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), acc[i][j], 0, 0, 0);
         else acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc[i][j], 0, 0, 0);
     };
     auto value = [&](int i, int j, int e) {
@@ -600,6 +657,27 @@ __global__ __launch_bounds__(64 * WR * WQ, BR == 256 ? 1 : 2) void product_k(Pro
             const int word0 = (int)(p.q0 + wc0) + fk * 4;        // the lane's first word
             const int words = (int)p.vocab - word0;              // that it may use, counted from there
             const bool edge = p.q0 + t.c0 + BQ > p.vocab;
+            // logits of fp32: the rows' and words' powers of two come back, the words' by way of LDS (behind what the ends use)
+            int* const word_power = reinterpret_cast<int*>(scratch + 32 * BQ);
+            int row_power[RI];
+            if constexpr (HALVES) {
+                for (int i = tid; i < BQ; i += NT) word_power[i] = p.q_power[t.c0 + i];
+#pragma unroll
+                for (int j = 0; j < RI; ++j) row_power[j] = p.r_power[wr0 + j * 16 + fl];
+                lds_barrier();
+            }
+            auto logits = [&](int j, float (&z)[QI * 4]) {
+#pragma unroll
+                for (int i = 0; i < QI; ++i) {
+                    int4 w;
+                    if constexpr (HALVES) w = *reinterpret_cast<const int4*>(word_power + wq * TQ + i * 16 + fk * 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        z[i * 4 + e] = value(i, j, e);
+                        if constexpr (HALVES) z[i * 4 + e] = ldexpf(z[i * 4 + e], row_power[j] + (e == 0 ? w.x : e == 1 ? w.y : e == 2 ? w.z : w.w));
+                    }
+                }
+            };
             if constexpr (END == STATS) {
                 float2* sm = reinterpret_cast<float2*>(scratch);     // [WQ][BR]
                 int tgt[RI];
@@ -610,8 +688,7 @@ __global__ __launch_bounds__(64 * WR * WQ, BR == 256 ? 1 : 2) void product_k(Pro
                     const int row = (int)wr0 + j * 16 + fl;
                     const unsigned at = (unsigned)(tgt[j] - word0);  // the target's place, if it is the lane's
                     float z[QI * 4], m4[4], s4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int i = 0; i < QI * 4; ++i) z[i] = value(i / 4, j, i % 4);
+                    logits(j, z);
                     if (edge) {
 #pragma unroll
                         for (int i = 0; i < QI * 4; ++i)
@@ -671,8 +748,9 @@ __global__ __launch_bounds__(64 * WR * WQ, BR == 256 ? 1 : 2) void product_k(Pro
 #pragma unroll
                     for (int j = 0; j < JS; ++j) {
                         const unsigned place = (unsigned)(tgt[jj + j] - word0);      // the target's, if it is the lane's
+                        logits(jj + j, g[j]);
 #pragma unroll
-                        for (int i = 0; i < QI * 4; ++i) g[j][i] = exp_of<PRECISE>(value(i / 4, jj + j, i % 4) - lse[jj + j]);
+                        for (int i = 0; i < QI * 4; ++i) g[j][i] = exp_of<PRECISE>(g[j][i] - lse[jj + j]);
                         if (place < (unsigned)TQ && (place & 12) == 0) {
 #pragma unroll
                             for (int i = 0; i < QI * 4; ++i) g[j][i] -= place == (unsigned)(i / 4 * 16 + i % 4) ? 1.f : 0.f;
@@ -805,12 +883,12 @@ __global__ __launch_bounds__(256) void finish_dx_k(const float* __restrict__ acc
 
 // ---- host --------------------------------------------------------------------------------------------------------------------
 struct Plan {
-    int planes, pairs;
+    int planes;
     long long np, vp;                   // rows and words, padded
     int kp;
     bool pack_w;
     // bytes from the state's start (kept) or the workspace's
-    long long xp, wp;
+    long long xp, wp, xh, wh, x_power, w_power;
     bool kept;
     // bytes from the workspace's start
     long long part, tl, row_loss, acc, g, bytes, state_bytes;
@@ -834,7 +912,6 @@ bool big_tiles(long long r, long long q) { return cdiv(r, 256) * (long long)cdiv
 Plan plan(const s2ag_lce_args* a, bool backward) {
     Plan p{};
     p.planes = a->bf16 ? 1 : 3;
-    p.pairs = a->bf16 ? 1 : 6;
     p.np = padded(a->rows);
     p.vp = round_up(a->vocab, 256);
     p.kp = (int)round_up(a->dim, BK);
@@ -846,16 +923,24 @@ Plan plan(const s2ag_lce_args* a, bool backward) {
         return here;
     };
     p.kept = backward || a->keep;
-    const long long x_bytes = round_up(2 * p.planes * p.np * p.kp, 256), w_bytes = p.pack_w ? round_up(2 * p.planes * a->vocab * p.kp, 256) : 0;
-    if (p.kept) {
-        p.xp = round_up(4 * state_words(a->rows), 256);
-        p.wp = p.xp + x_bytes;
-        p.state_bytes = p.wp + w_bytes;
-    } else {
-        p.xp = take(x_bytes);
-        p.wp = take(w_bytes);
-        p.state_bytes = 4 * state_words(a->rows);
+    long long kept_bytes = round_up(4 * state_words(a->rows), 256);
+    auto put = [&](long long b) {                                 // into the state, if that is kept
+        if (!p.kept) return take(b);
+        const long long here = kept_bytes;
+        kept_bytes += round_up(b, 256);
+        return here;
+    };
+    if (!a->bf16) {
+        p.xh = put(2 * 2 * p.np * p.kp);
+        p.wh = put(2 * 2 * a->vocab * p.kp);
+        p.x_power = put(4 * p.np);
+        p.w_power = put(4 * p.vp);
     }
+    if (a->bf16 || p.kept) {                                      // (the pieces are the gradient's)
+        p.xp = put(2 * p.planes * p.np * p.kp);
+        p.wp = p.pack_w ? put(2 * p.planes * a->vocab * p.kp) : 0;
+    }
+    p.state_bytes = kept_bytes;
     if (!backward) {
         p.part = take(8 * p.np * cdiv(a->vocab, 128));
         p.tl = take(4 * p.np);
@@ -868,7 +953,7 @@ Plan plan(const s2ag_lce_args* a, bool backward) {
         p.acc_ld = (int)round_up(a->dim, 4);
         // dX has few tiles: the words of a piece are split, down to eight stages each
         p.acc_tile = 256;
-        const long long stages = p.piece / BK * p.pairs;
+        const long long stages = p.piece / BK * (a->bf16 ? 1 : 6);
         p.splits = (int)(stages / 8 < 1 ? 1 : stages / 8 > SLOTS ? SLOTS : stages / 8);
         // (what fills the card with splits is no more than its tiles hold)
         p.acc = take(dx ? 4 * (p.np * p.acc_ld + (long long)SLOTS * 256 * 256) : 0);
@@ -902,7 +987,7 @@ int launch_tiles(Product& p, long long r_rows, long long q_rows, hipStream_t st)
 
 template <End END>
 int launch(Product& p, bool big, long long r_rows, long long q_rows, hipStream_t st) {
-    if (p.pairs > 1)
+    if (p.fp32)
         return big ? launch_tiles<256, 256, 2, 2, END, true>(p, r_rows, q_rows, st) : launch_tiles<128, 128, 2, 2, END, true>(p, r_rows, q_rows, st);
     return big ? launch_tiles<256, 256, 2, 2, END, false>(p, r_rows, q_rows, st) : launch_tiles<128, 128, 2, 2, END, false>(p, r_rows, q_rows, st);
 }
@@ -913,23 +998,49 @@ unsigned grid_of(long long work) {
 }
 
 // where the packed operands are, or the caller's W as it is
+char* packed(const s2ag_lce_args* a, const Plan& p) { return static_cast<char*>(p.kept ? a->state : a->workspace); }
 void operands(const s2ag_lce_args* a, const Plan& p, Operand* x, Operand* w) {
-    char* at = static_cast<char*>(p.kept ? a->state : a->workspace);
-    *x = Operand{reinterpret_cast<bf16_t*>(at + p.xp), p.np * p.kp, p.kp};
-    if (p.pack_w) *w = Operand{reinterpret_cast<bf16_t*>(at + p.wp), a->vocab * p.kp, p.kp};
+    *x = Operand{reinterpret_cast<bf16_t*>(packed(a, p) + p.xp), p.np * p.kp, p.kp};
+    if (p.pack_w) *w = Operand{reinterpret_cast<bf16_t*>(packed(a, p) + p.wp), a->vocab * p.kp, p.kp};
     else *w = Operand{static_cast<const bf16_t*>(a->w), 0, a->ldw};
 }
-
-template <typename T>
-int pack(const s2ag_lce_args* a, const Plan& p, const State& s, const Operand& x, const Operand& w, hipStream_t st) {
-    hipLaunchKernelGGL(pack_k<T>, dim3(grid_of(p.np * (p.kp / 8))), dim3(256), 0, st, static_cast<const T*>(a->x), a->ldx, a->dim, s.rowmap,
-                       s.count, p.np, const_cast<bf16_t*>(x.p), p.kp, x.plane);
-    S2AG_LAUNCH_CHECK();
-    if (p.pack_w) {
-        hipLaunchKernelGGL(pack_k<T>, dim3(grid_of(a->vocab * (p.kp / 8))), dim3(256), 0, st, static_cast<const T*>(a->w), a->ldw, a->dim,
-                           (const int*)nullptr, (const int*)nullptr, a->vocab, const_cast<bf16_t*>(w.p), p.kp, w.plane);
-        S2AG_LAUNCH_CHECK();
+// those of the logits from word v0 on
+void logit_operands(const s2ag_lce_args* a, const Plan& p, long long v0, Product* q) {
+    if (a->bf16) {
+        operands(a, p, &q->r, &q->q);
+    } else {
+        q->r = Operand{reinterpret_cast<bf16_t*>(packed(a, p) + p.xh), p.np * p.kp, p.kp};
+        q->q = Operand{reinterpret_cast<bf16_t*>(packed(a, p) + p.wh), a->vocab * p.kp, p.kp};
+        q->r_power = reinterpret_cast<int*>(packed(a, p) + p.x_power);
+        q->q_power = reinterpret_cast<int*>(packed(a, p) + p.w_power) + v0;
     }
+    q->q.p += v0 * q->q.ld;
+    q->r_rows = p.np;
+    q->k = p.kp;
+    q->fp32 = !a->bf16;
+}
+
+int pack(const s2ag_lce_args* a, const Plan& p, const State& s, hipStream_t st) {
+    char* at = packed(a, p);
+    if (a->bf16) {
+        hipLaunchKernelGGL(pack_k, dim3(grid_of(p.np * (p.kp / 8))), dim3(256), 0, st, static_cast<const bf16_t*>(a->x), a->ldx, a->dim, s.rowmap,
+                           s.count, p.np, reinterpret_cast<bf16_t*>(at + p.xp), p.kp);
+        S2AG_LAUNCH_CHECK();
+        if (p.pack_w) {
+            hipLaunchKernelGGL(pack_k, dim3(grid_of(a->vocab * (p.kp / 8))), dim3(256), 0, st, static_cast<const bf16_t*>(a->w), a->ldw, a->dim,
+                               (const int*)nullptr, (const int*)nullptr, a->vocab, reinterpret_cast<bf16_t*>(at + p.wp), p.kp);
+            S2AG_LAUNCH_CHECK();
+        }
+        return 0;
+    }
+    hipLaunchKernelGGL(pack32_k, dim3(grid_of(p.np * 64)), dim3(256), 0, st, static_cast<const float*>(a->x), a->ldx, a->dim, s.rowmap, s.count, p.np,
+                       p.kp, reinterpret_cast<f16_t*>(at + p.xh), reinterpret_cast<int*>(at + p.x_power),
+                       p.kept ? reinterpret_cast<bf16_t*>(at + p.xp) : nullptr, p.np * p.kp);
+    S2AG_LAUNCH_CHECK();
+    hipLaunchKernelGGL(pack32_k, dim3(grid_of(a->vocab * 64)), dim3(256), 0, st, static_cast<const float*>(a->w), a->ldw, a->dim, (const int*)nullptr,
+                       (const int*)nullptr, a->vocab, p.kp, reinterpret_cast<f16_t*>(at + p.wh), reinterpret_cast<int*>(at + p.w_power),
+                       p.kept ? reinterpret_cast<bf16_t*>(at + p.wp) : nullptr, a->vocab * p.kp);
+    S2AG_LAUNCH_CHECK();
     return 0;
 }
 
@@ -961,12 +1072,9 @@ extern "C" int s2ag_lce_fwd(const s2ag_lce_args* a, void* stream) {
     S2AG_LAUNCH_CHECK();
     if (a->rows) {
         Product q{};
-        operands(a, p, &q.r, &q.q);
-        if (int rc = a->bf16 ? pack<bf16_t>(a, p, s, q.r, q.q, st) : pack<float>(a, p, s, q.r, q.q, st)) return rc;
-        q.r_rows = p.np;
+        if (int rc = pack(a, p, s, st)) return rc;
+        logit_operands(a, p, 0, &q);
         q.q_rows = q.vocab = a->vocab;
-        q.k = p.kp;
-        q.pairs = p.pairs;
         q.r_count = s.count;
         q.tgt = s.tgt;
         q.part = reinterpret_cast<float2*>(ws + p.part);
@@ -1002,12 +1110,8 @@ extern "C" int s2ag_lce_bwd(const s2ag_lce_args* a, void* stream) {
         if (words <= 0) break;
         const long long wide = round_up(words, 256);
         Product q{};
-        q.r = x;
-        q.q = Operand{w.p + v0 * w.ld, w.plane, w.ld};
-        q.r_rows = p.np;
+        logit_operands(a, p, v0, &q);
         q.q_rows = words;
-        q.k = p.kp;
-        q.pairs = p.pairs;
         q.r_count = s.count;
         q.tgt = s.tgt;
         q.q0 = v0;
@@ -1028,7 +1132,7 @@ extern "C" int s2ag_lce_bwd(const s2ag_lce_args* a, void* stream) {
             d.q_deep = words;
             d.q_cols = p.pack_w ? p.kp : a->dim;
             d.k = (int)wide;
-            d.pairs = p.pairs;
+            d.fp32 = !a->bf16;
             d.r_count = s.count;
             d.splits = p.splits;
             d.out = acc;
@@ -1046,7 +1150,7 @@ extern "C" int s2ag_lce_bwd(const s2ag_lce_args* a, void* stream) {
             d.r_cols = (int)p.piece;
             d.q_cols = p.kp;
             d.k_count = s.count;
-            d.pairs = p.pairs;
+            d.fp32 = !a->bf16;
             d.out = a->bf16 ? (void*)(static_cast<bf16_t*>(a->dw) + v0 * a->dim) : (void*)(static_cast<float*>(a->dw) + v0 * a->dim);
             d.out_ld = a->dim;
             d.out_bf16 = a->bf16;

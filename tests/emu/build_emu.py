@@ -8,7 +8,7 @@ _build/src, line numbers kept):
   * `extern __shared__ [attrs] T name[];`  ->  `T* name = (T*)emu::dyn_smem();`   (dynamic LDS of the running workgroup)
   * `asm volatile("s_waitcnt ...")`        ->  nothing   (waits for the wave's own memory operations: no-ops in this model)
   * `asm volatile("s_waitcnt lgkmcnt(0)\\n\\ts_barrier")` -> `__syncthreads()`
-  * `asm("v_mfma_f32_16x16x32_bf16 ..." : "+a"(c) ...)` -> the builtin of that instruction
+  * `asm("v_mfma_f32_16x16x32_{bf16,f16} ..." : "+a"(c) ...)` -> the builtin of that instruction
   * `asm volatile("v_accvgpr_read_b32 ...")` -> an assignment
   * `asm volatile("s_mov_b32 m0 ...; buffer_load_dwordx4 ... lds")` -> emu_buffer_to_lds (hip_runtime.h)
   * `asm volatile("s_nop ...")`            ->  nothing
@@ -28,7 +28,7 @@ DEBUG = os.environ.get('S2AG_EMU_DEBUG', '0') == '1'      # -DS2AG_DEBUG=1: the 
 OUT = os.path.join(HERE, '_build', 'debug') if DEBUG else os.path.join(HERE, '_build')
 LIB = os.path.join(OUT, 'libs2ag_emu_debug.so' if DEBUG else 'libs2ag_emu.so')
 CXX = os.environ.get('S2AG_EMU_CXX', '/opt/rocm/lib/llvm/bin/clang++')
-FLAGS = ['-x', 'c++', '-std=c++17', '-O1', '-g1', '-fPIC', '-fno-strict-aliasing', '-ffp-contract=off', '-pthread',
+FLAGS = ['-x', 'c++', '-std=c++17', '-O1', '-g1', '-fPIC', '-fno-strict-aliasing', '-ffp-contract=off', '-pthread', '-mf16c',
          '-Wno-unknown-attributes', '-Wno-ignored-attributes', '-Wno-unused-value', '-Wno-pass-failed',
          '-Wno-unknown-pragmas', '-Wno-deprecated-declarations',
          '-DS2AG_DET=1',      # the model's library always carries the deterministic mode (the GPU build: flavour `det` only)
@@ -40,7 +40,7 @@ _ASM_BAR = re.compile(r'asm volatile\("s_waitcnt lgkmcnt\(0\)\\n\\ts_barrier"\s*
 _ASM_WAIT = re.compile(r'asm volatile\("s_waitcnt [a-z]+cnt\(\d+\)"\s*:::\s*"memory"\)')
 
 
-_ASM_MFMA = re.compile(r'asm\("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "\+a"\((\w+)\) : "v"\((\w+)\), "v"\((\w+)\)\);')
+_ASM_MFMA = re.compile(r'asm\("v_mfma_f32_16x16x32_(bf16|f16) %0, %1, %2, %0" : "\+a"\((\w+)\) : "v"\((\w+)\), "v"\((\w+)\)\);')
 _ASM_LDS = re.compile(r'const unsigned at = [^\n]*\n\s*asm volatile\("s_mov_b32 m0, %0\\n\\ts_nop 0\\n\\tbuffer_load_dwordx4 %1, %2, %3 offen lds" [^\n]*\n')
 _ASM_ACC = re.compile(r'asm volatile\("v_accvgpr_read_b32 %0, %1" : "=v"\((\w+)\) : "a"\((\w+)\)\);')
 _ASM_NOP = re.compile(r'asm volatile\("s_nop \d+(?:\\n\\ts_nop \d+)*"\s*:::\s*"memory"\)')
@@ -53,7 +53,7 @@ def rewrite(text: str) -> str:
     text = _ASM_NOP.sub('((void)0)', text)
     text = _ASM_LDS.sub('emu_buffer_to_lds(from, dst, lane_offset, offset);\n', text)
     text = _ASM_ACC.sub(lambda m: '%s = %s;' % (m.group(1), m.group(2)), text)
-    text = _ASM_MFMA.sub(lambda m: '%s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(%s, %s, %s, 0, 0, 0);' % (m.group(1), m.group(2), m.group(3), m.group(1)), text)
+    text = _ASM_MFMA.sub(lambda m: '%s = emu_mfma_of_%s(%s, %s, %s);' % (m.group(2), m.group(1), m.group(3), m.group(4), m.group(2)), text)
     if 'asm volatile' in text or 'extern __shared__' in text:
         bad = [l for l in text.splitlines() if 'asm volatile' in l or 'extern __shared__' in l]
         raise RuntimeError('construct the emulator build does not know how to rewrite: ' + bad[0].strip())

@@ -376,6 +376,22 @@ static inline emu::f32x4_t emu_mfma_16x16x4_f32(float a, float b, emu::f32x4_t c
     emu::collective(emu::OP_MFMA_F32_4, &emu::mfma_k4_fn, &r);
     return r.c;
 }
+typedef _Float16 emu_f16x8_t __attribute__((ext_vector_type(8)));
+static inline emu::f32x4_t emu_mfma_16x16x32_f16(emu_f16x8_t a, emu_f16x8_t b, emu::f32x4_t c, int, int, int) {
+    emu::MfmaRec r;                          // (products of halves are exact in fp32 too)
+    for (int i = 0; i < 8; ++i) { r.a[i] = (float)a[i]; r.b[i] = (float)b[i]; }
+    r.c = c;
+    emu::collective(emu::OP_MFMA_BF16_32, &emu::mfma_k32_fn, &r);
+    return r.c;
+}
+// the written-out forms: operands are 16 bytes of either type
+template <typename V> static inline emu::f32x4_t emu_mfma_of_bf16(V a, V b, emu::f32x4_t c) {
+    return emu_mfma_16x16x32_bf16(__builtin_bit_cast(emu::bf16x8_t, a), __builtin_bit_cast(emu::bf16x8_t, b), c, 0, 0, 0);
+}
+template <typename V> static inline emu::f32x4_t emu_mfma_of_f16(V a, V b, emu::f32x4_t c) {
+    return emu_mfma_16x16x32_f16(__builtin_bit_cast(emu_f16x8_t, a), __builtin_bit_cast(emu_f16x8_t, b), c, 0, 0, 0);
+}
+#define __builtin_amdgcn_mfma_f32_16x16x32_f16 emu_mfma_16x16x32_f16
 #define __builtin_amdgcn_mfma_f32_16x16x32_bf16 emu_mfma_16x16x32_bf16
 #define __builtin_amdgcn_mfma_f32_16x16x16bf16_1k emu_mfma_16x16x16_bf16_1k
 #define __builtin_amdgcn_mfma_f32_16x16x4f32 emu_mfma_16x16x4_f32

@@ -183,14 +183,17 @@ IGNORE = -100
 def lce_reference(x, w, target, gout, reduction, ignore=IGNORE):
     """(loss, bound), (dx, bound), (dw, bound) in 64 bits.  The bounds follow the kernels: a logit is a sum of `terms` fp32 terms;
     an exponential of an argument of size s is off by s u + 4 u of itself (its argument's product with log2 e, its own rounding);
-    G is rounded to bf16 for bf16 operands, its and the other operand's pieces carry 2^-23 for fp32."""
+    G is rounded to bf16 for bf16 operands, its and the other operand's pieces carry 2^-23 for fp32.  fp32 logits are three products of
+    two halves each: a value's second half leaves 2^-11 of the 2^-11 that the first left, 2^-22 = 4 u of it, and the product of the
+    second halves, another 2^-22, is left out: 12 u of |x| |w| in all.  A value below 2^-17 of its row's
+    largest keeps less, 2^-39 of that largest one: no test has such columns together with words that make them count."""
     dt = x.dtype
     pieces = 6 if dt == torch.float32 else 1
     x64, w64 = x.double(), w.double()
     n, d = x.shape
     z = x64 @ w64.t()
     za = (x64.abs() @ w64.abs().t()).max() if n else torch.tensor(0.0)
-    dz = float(za) * ((d * pieces + 4) * U + (4 * U if pieces > 1 else 0))          # sums; pieces that are left out
+    dz = float(za) * ((d * min(pieces, 3) + 4) * U + (12 * U if pieces > 1 else 0))  # sums; what the halves leave
     keep = target != ignore
     at = torch.where(keep, target, torch.zeros_like(target)).long()
     lse = torch.logsumexp(z, 1)
@@ -348,6 +351,31 @@ def test_linear_cross_entropy_large_logits(S):
     want = torch.zeros(3, 64)
     want[1, 2], want[1, 5] = 1.0, -1.0
     assert torch.equal(xg.grad.cpu(), want)
+
+
+@pytest.mark.parametrize('dtype', list(DTYPES))
+def test_linear_cross_entropy_powers_of_two_of_rows_and_words_cancel(S, dtype):
+    """Rows and words of very different sizes whose products are ordinary: a power of two changes no bit of the loss, and moves the
+    gradients by itself."""
+    x, w, t, _ = lce_case(70, 40, 300, dtype, 0.2)
+
+    def run(x, w):
+        x, w = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+        loss = S['ops'].linear_cross_entropy(x, w, t.cuda(), ignore_index=IGNORE, reduction='sum')
+        loss.backward()
+        return loss.detach(), x.grad, w.grad
+    loss, dx, dw = run(x, w)
+    for up in (30, -50):
+        l2, dx2, dw2 = run(x * 2.0 ** up, w * 2.0 ** -up)
+        assert torch.equal(loss, l2)
+        assert torch.equal(dx * 2.0 ** -up, dx2) and torch.equal(dw * 2.0 ** up, dw2)
+
+
+def test_linear_cross_entropy_columns_of_many_sizes(S):
+    """Within a row values down to 2^-16 of the largest, the words the other way round, so that every column counts alike."""
+    x, w, t, g = lce_case(50, 48, 300, 'fp32', 0.0)
+    size = 2.0 ** -(torch.arange(48) % 17).float()
+    lce_check(S, x * size, w / size, t, g, 'mean')
 
 
 @pytest.mark.parametrize('dtype', list(DTYPES))
