@@ -443,8 +443,8 @@ __global__ __launch_bounds__(64 * WR * WQ, BR == 256 ? 1 : 2) void product_k(Pro
     };
     auto place = [&](int v) {
         Place t;
-        t.split = __builtin_amdgcn_readfirstlane(v % ts.splits);
-        v = __builtin_amdgcn_readfirstlane(v / ts.splits);
+        t.split = __builtin_amdgcn_readfirstlane(v / (ts.tiles_r * p.tiles_q));
+        v -= t.split * ts.tiles_r * p.tiles_q;
         const int grp = __builtin_amdgcn_readfirstlane(v / ts.per), g0 = grp * ts.group, gsz = min(ts.tiles_r - g0, ts.group);
         t.r0 = (long long)__builtin_amdgcn_readfirstlane(g0 + (v - grp * ts.per) % gsz) * BR;
         t.c0 = (long long)__builtin_amdgcn_readfirstlane((v - grp * ts.per) / gsz) * BQ;
@@ -896,7 +896,9 @@ struct Plan {
     int acc_tile, splits, acc_ld;       // of the product that dX is
 };
 
-constexpr long long PIECE_VALUES = 1LL << 27;   // of G in a piece: 256 MB in bf16, beside which the fp32 sums of dX are small
+// Values of G in a piece of the vocabulary, 512 MB in bf16.  (Half as many: 8192 rows, 131072 words of 2048 values 13.0 against
+// 12.6 ms; 4352 rows, 85 % of them ignored, 20000 words of 300 values, fp32: 294 against 239 us, since pieces are made for all rows.)
+constexpr long long PIECE_VALUES = 1LL << 28;
 
 bool valid(const s2ag_lce_args* a) {
     // 2^21: a tile's rows stay within a 31-bit byte offset whichever way they run
@@ -905,9 +907,24 @@ bool valid(const s2ag_lce_args* a) {
 }
 
 constexpr int SLOTS = 256;              // large tiles: one workgroup on a compute unit; small ones: two
+constexpr int small_slots = 2 * SLOTS;
 
-// 256 x 256 tiles where they fill the 256 compute units, else 128 x 128
-bool big_tiles(long long r, long long q) { return cdiv(r, 256) * (long long)cdiv(q, 256) >= 256; }
+// Tiles of 256 x 256 or, at `percent` of their rate, of 128 x 128.  Large ones come in rounds of one on each of the 256 compute
+// units; the small ones pad less and leave less of a round idle, since half a unit's work is a finer measure.
+bool big_tiles(long long r, long long q, int percent) {
+    const long long big = (long long)cdiv(r, 256) * cdiv(q, 256), small = (long long)cdiv(r, 128) * cdiv(q, 128);
+    return (big + SLOTS - 1) / SLOTS * (2 * small_slots) * percent <= small * 100;
+}
+// (4096 rows and 32768 words of 1024 values: max and sum 283 us large, 326 small, G 301 and 332; dW 250 and 322, but of 640 values,
+// which large tiles pad to 768, 227 and 198)
+constexpr int LOGIT_RATE = 88, DW_RATE = 77;
+// Logits of short rows: a tile's end is long beside its products, and of two workgroups on a compute unit one multiplies while the
+// other ends (4096 rows, 320 wide: max and sum 131 us large, 133 small; 128 wide 94 and 85; fp32 320 wide 220 and 212, 1024 wide
+// 503 and 526).  G of fp32, three pieces of each value, takes small ones for every length (1024 wide: 688 and 607 us).
+bool short_rows(int k) { return k <= 320; }
+// dX, whose words are split until the card is full (4096 x 1024, 64 large tiles: 234 us large, 311 small; 1999 x 520, 24 of them:
+// 105 and 92)
+bool big_dx_tiles(long long rows, long long dim) { return (long long)cdiv(rows, 256) * cdiv(dim, 256) >= 48; }
 
 Plan plan(const s2ag_lce_args* a, bool backward) {
     Plan p{};
@@ -952,9 +969,9 @@ Plan plan(const s2ag_lce_args* a, bool backward) {
         const bool dx = a->dx != nullptr;
         p.acc_ld = (int)round_up(a->dim, 4);
         // dX has few tiles: the words of a piece are split, down to eight stages each
-        p.acc_tile = 256;
+        p.acc_tile = big_dx_tiles(p.np, a->dim) ? 256 : 128;
         const long long stages = p.piece / BK * (a->bf16 ? 1 : 6);
-        p.splits = (int)(stages / 8 < 1 ? 1 : stages / 8 > SLOTS ? SLOTS : stages / 8);
+        p.splits = (int)(stages / 8 < 1 ? 1 : stages / 8 > small_slots ? small_slots : stages / 8);
         // (what fills the card with splits is no more than its tiles hold)
         p.acc = take(dx ? 4 * (p.np * p.acc_ld + (long long)SLOTS * 256 * 256) : 0);
         p.g = take(2 * p.planes * p.np * p.piece);
@@ -987,8 +1004,11 @@ int launch_tiles(Product& p, long long r_rows, long long q_rows, hipStream_t st)
 
 template <End END>
 int launch(Product& p, bool big, long long r_rows, long long q_rows, hipStream_t st) {
-    if (p.fp32)
-        return big ? launch_tiles<256, 256, 2, 2, END, true>(p, r_rows, q_rows, st) : launch_tiles<128, 128, 2, 2, END, true>(p, r_rows, q_rows, st);
+    if constexpr (END == GRADS) {
+        if (p.fp32) return launch_tiles<128, 128, 2, 2, END, true>(p, r_rows, q_rows, st);
+    } else {
+        if (p.fp32) return big ? launch_tiles<256, 256, 2, 2, END, true>(p, r_rows, q_rows, st) : launch_tiles<128, 128, 2, 2, END, true>(p, r_rows, q_rows, st);
+    }
     return big ? launch_tiles<256, 256, 2, 2, END, false>(p, r_rows, q_rows, st) : launch_tiles<128, 128, 2, 2, END, false>(p, r_rows, q_rows, st);
 }
 
@@ -1080,7 +1100,7 @@ extern "C" int s2ag_lce_fwd(const s2ag_lce_args* a, void* stream) {
         q.part = reinterpret_cast<float2*>(ws + p.part);
         q.part_ld = p.np;
         q.target_logit = reinterpret_cast<float*>(ws + p.tl);
-        if (int rc = launch<STATS>(q, big_tiles(p.np, a->vocab), p.np, a->vocab, st)) return rc;
+        if (int rc = launch<STATS>(q, !short_rows(p.kp) && big_tiles(p.np, a->vocab, LOGIT_RATE), p.np, a->vocab, st)) return rc;
         hipLaunchKernelGGL(join_stats_k, dim3((unsigned)(p.np / 64)), dim3(1024), 0, st, q.part, q.part_ld, q.tiles_q, s, q.target_logit,
                            a->reduction, a->loss, row_loss);
         S2AG_LAUNCH_CHECK();
@@ -1122,7 +1142,7 @@ extern "C" int s2ag_lce_bwd(const s2ag_lce_args* a, void* stream) {
         q.g = g;
         q.g_ld = p.piece;
         q.g_plane = p.np * p.piece;
-        if (int rc = launch<GRADS>(q, big_tiles(p.np, wide), p.np, wide, st)) return rc;
+        if (int rc = launch<GRADS>(q, !short_rows(p.kp) && big_tiles(p.np, wide, LOGIT_RATE), p.np, wide, st)) return rc;
         if (a->dx) {
             Product d{};
             d.r = Operand{g, q.g_plane, p.piece};
@@ -1138,7 +1158,7 @@ extern "C" int s2ag_lce_bwd(const s2ag_lce_args* a, void* stream) {
             d.out = acc;
             d.out_ld = p.acc_ld;
             d.add = v0 > 0;
-            if (int rc = launch<ACCUM>(d, true, p.np, a->dim, st)) return rc;
+            if (int rc = launch<ACCUM>(d, p.acc_tile == 256, p.np, a->dim, st)) return rc;
         }
         if (a->dw) {
             Product d{};
@@ -1157,16 +1177,16 @@ extern "C" int s2ag_lce_bwd(const s2ag_lce_args* a, void* stream) {
             d.add = a->dw_accumulate;
             d.scale = each ? nullptr : a->grad_out;
             d.mean = mean;
-            if (int rc = launch<STORE>(d, big_tiles(words, a->dim), words, a->dim, st)) return rc;
+            if (int rc = launch<STORE>(d, big_tiles(words, a->dim, DW_RATE), words, a->dim, st)) return rc;
         }
     }
     if (a->dx && a->rows) {
         const unsigned gx = grid_of(a->rows * ((a->dim + 3) / 4));
         if (a->bf16)
-            hipLaunchKernelGGL(finish_dx_k<bf16_t>, dim3(gx), dim3(256), 0, st, acc, (long long)p.acc_ld, p.acc_tile, cdiv(a->dim, p.acc_tile), p.splits, SLOTS, s,
+            hipLaunchKernelGGL(finish_dx_k<bf16_t>, dim3(gx), dim3(256), 0, st, acc, (long long)p.acc_ld, p.acc_tile, cdiv(a->dim, p.acc_tile), p.splits, p.acc_tile == 256 ? SLOTS : small_slots, s,
                                each ? nullptr : a->grad_out, (int)mean, a->rows, a->dim, static_cast<bf16_t*>(a->dx));
         else
-            hipLaunchKernelGGL(finish_dx_k<float>, dim3(gx), dim3(256), 0, st, acc, (long long)p.acc_ld, p.acc_tile, cdiv(a->dim, p.acc_tile), p.splits, SLOTS, s,
+            hipLaunchKernelGGL(finish_dx_k<float>, dim3(gx), dim3(256), 0, st, acc, (long long)p.acc_ld, p.acc_tile, cdiv(a->dim, p.acc_tile), p.splits, p.acc_tile == 256 ? SLOTS : small_slots, s,
                                each ? nullptr : a->grad_out, (int)mean, a->rows, a->dim, static_cast<float*>(a->dx));
         S2AG_LAUNCH_CHECK();
     }

@@ -271,7 +271,8 @@ def test_linear_cross_entropy_reductions(S, reduction, dtype):
 
 @pytest.mark.skipif(EMU, reason='hundreds of large tiles: minutes on the device model')
 @pytest.mark.parametrize('dtype', list(DTYPES))
-@pytest.mark.parametrize('case', [(250, 64, 65536), (65530, 40, 300), (1100, 520, 50021)])
+@pytest.mark.parametrize('case', [(250, 64, 65536), (65530, 40, 300), (1100, 520, 50021), (1000, 520, 65536), (4100, 800, 700),
+                                  (40, 800, 30000)])
 def test_linear_cross_entropy_large_tiles(S, case, dtype):
     x, w, t, g = lce_case(*case, dtype, 0.2)
     lce_check(S, x, w, t, g, 'mean')
@@ -281,7 +282,7 @@ def test_linear_cross_entropy_large_tiles(S, case, dtype):
 @pytest.mark.parametrize('dtype', list(DTYPES))
 def test_linear_cross_entropy_in_pieces_of_the_vocabulary(S, dtype):
     """More rows times words than one piece holds."""
-    n, d, v = 20000, 8, 9001
+    n, d, v = 20000, 8, 13501
     x, w, t, g = lce_case(n, d, v, dtype, 0.1)
     lce_check(S, x, w, t, g, 'mean')
 
