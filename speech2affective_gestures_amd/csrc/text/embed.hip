@@ -76,7 +76,8 @@ __device__ __forceinline__ unsigned key_of(const void* ids, int ids_i32, long lo
     return (unsigned)((id < 0 || id >= n_entries || id == padding_idx) ? n_entries : id);
 }
 
-// Up to SMALL positions: one workgroup sorts them in LDS, 8 bits a pass.  Items go by wavefront, round and lane, which is their
+// Up to SMALL positions: one workgroup sorts them in LDS in one launch, 8 bits a pass (4352 positions: 13 us; the four launches that
+// more positions take 23; 8192: 19 and 25).  Items go by wavefront, round and lane, which is their
 // order; a wavefront counts its items per digit while it ranks them, so that a pass reads its items once.
 constexpr int SMALL = 8192;
 constexpr int SB = 8, SBINS = 1 << SB, SWAVES = 16;
@@ -163,7 +164,8 @@ __global__ __launch_bounds__(1024) void sort_small_k(const void* __restrict__ id
 
 // More: per pass of LB bits one launch counts the digits of every tile of LTILE items and one moves the items.  Up to DIRECT
 // tiles the second adds the counts of the tiles itself; more are added up by a launch between the two (a workgroup per digit).
-constexpr int LB = 9, LBINS = 1 << LB, LTILE = 2048, LWAVES = 4, LROUNDS = LTILE / 256, DIRECT = 64;
+// (32 tiles: 32 us in four launches, 32 in six; 64 tiles: 34 and 32; 128 tiles: 46 and 40)
+constexpr int LB = 9, LBINS = 1 << LB, LTILE = 2048, LWAVES = 4, LROUNDS = LTILE / 256, DIRECT = 32;
 struct SortIn {
     const void* ids;                    // first pass: the keys come from the ids, the positions count up
     int ids_i32;
@@ -294,6 +296,7 @@ __global__ __launch_bounds__(256) void sort_move_k(SortIn in, int shift, int til
 }
 
 // ---- sums ------------------------------------------------------------------------------------------------------------------
+constexpr int ZERO_ROWS = 64;           // a lane to each: 16 of them take as long
 constexpr int UNROLL = 8;               // rows in flight per wavefront: 8 KB, 128 KB on a compute unit with 16 wavefronts
 
 // A lane's V columns of a row: one 16-byte access at any alignment, element by element at the row's end.
@@ -342,13 +345,12 @@ template <typename T>
 __global__ __launch_bounds__(256) void sum_k(const unsigned* __restrict__ keys, const int* __restrict__ pos, int n,
                                              const T* __restrict__ dy, long long ldy, int dim, long long n_entries, float scale,
                                              T* __restrict__ dtable, int accumulate, int tile_len, int tiles, int chunks,
-                                             float* __restrict__ pieces, const unsigned char* __restrict__ touched, int sum_blocks,
-                                             int zero_rows) {
+                                             float* __restrict__ pieces, const unsigned char* __restrict__ touched, int sum_blocks) {
     constexpr int V = Vec<T>::N;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if ((int)blockIdx.x >= sum_blocks) {                          // rows without an id, zero_rows to a wavefront
-        const long long v0 = ((long long)(blockIdx.x - sum_blocks) * 4 + wave) * zero_rows;
-        const bool mine = lane < zero_rows && v0 + lane < n_entries && !touched[v0 + lane];
+    if ((int)blockIdx.x >= sum_blocks) {                          // rows without an id, ZERO_ROWS to a wavefront
+        const long long v0 = ((long long)(blockIdx.x - sum_blocks) * 4 + wave) * ZERO_ROWS;
+        const bool mine = v0 + lane < n_entries && !touched[v0 + lane];
         unsigned long long left = __ballot(mine);
         while (left) {
             const int at = __ffsll(left) - 1;
@@ -405,45 +407,83 @@ __global__ __launch_bounds__(256) void sum_k(const unsigned* __restrict__ keys, 
     else write_cols<T>(dtable + (long long)cur * dim, c, dim, acc, scale, accumulate);
 }
 
-// A workgroup per (tile, chunk) that a crossing run begins in: eight wavefronts add every eighth piece, then each other's sums.
+// Runs that cross a border, a wavefront to the (tile, chunk) that one begins in.  Most end in the next tile: the wavefront adds
+// their pieces by itself.  Of a long one its workgroup's eight wavefronts add every eighth piece, then each other's sums.  (5 us for
+// 65536 positions of 2048 columns; 89 us where half of a million positions of 64 columns hold one id, whose 7800 pieces are one
+// workgroup's.)
+constexpr int JOINERS = 8;
 template <typename T>
-__global__ __launch_bounds__(512) void join_k(const unsigned* __restrict__ keys, int n, int dim, long long n_entries, float scale,
-                                              T* __restrict__ dtable, int accumulate, int tile_len, int chunks,
-                                              float* __restrict__ pieces) {
+__global__ __launch_bounds__(64 * JOINERS) void join_k(const unsigned* __restrict__ keys, int n, int dim, long long n_entries,
+                                                       float scale, T* __restrict__ dtable, int accumulate, int tile_len, int tiles,
+                                                       int chunks, float* __restrict__ pieces) {
     constexpr int V = Vec<T>::N;
-    __shared__ float sm[8][64 * V];
-    const int tile = blockIdx.x / chunks, chunk = blockIdx.x - tile * chunks;
-    const int t0 = tile * tile_len, t1 = t0 + tile_len;
-    if (t1 >= n) return;
-    const unsigned cur = keys[t1 - 1];
-    if (cur >= (unsigned)n_entries || keys[t1] != cur) return;
-    if (t0 > 0 && keys[t0 - 1] == cur) return;                    // began in an earlier tile
-    int lo = t1, hi = n;                                          // first position behind the run
-    while (lo < hi) {
-        const int mid = lo + ((hi - lo) >> 1);
-        if (keys[mid] == cur) lo = mid + 1;
-        else hi = mid;
-    }
-    const int last = (lo - 1) / tile_len;
+    __shared__ float sm[JOINERS][64 * V];
+    __shared__ int last_s[JOINERS];
+    __shared__ unsigned cur_s[JOINERS];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    float acc[V];
-    for (int j = 0; j < V; ++j) acc[j] = 0.f;
-#pragma unroll 4
-    for (int t = tile + wave; t <= last; t += 8) {
-        const float* q = piece<V>(pieces, t, t == tile ? 1 : 0, chunk, chunks);
-        for (int j = 0; j < V; ++j) acc[j] += q[j * 64 + lane];
+    const int tile0 = (int)(blockIdx.x / chunks) * JOINERS, tile = tile0 + wave, chunk = blockIdx.x % chunks;
+    auto add = [&](float* acc, int tile, int from, int last, int step) {
+#pragma unroll 8
+        for (int t = from; t <= last; t += step) {
+            const float* q = piece<V>(pieces, t, t == tile ? 1 : 0, chunk, chunks);
+            for (int j = 0; j < V; ++j) acc[j] += q[j * 64 + lane];
+        }
+    };
+    int last = -1;
+    unsigned cur = ~0u;
+    if (tile < tiles - 1) {                                       // (the last tile has no border behind it)
+        const int t0 = tile * tile_len, t1 = t0 + tile_len;
+        cur = keys[t1 - 1];
+        if (cur < (unsigned)n_entries && keys[t1] == cur && !(t0 > 0 && keys[t0 - 1] == cur)) {
+            // the first tile whose last key is another one, or the last tile: 64 tiles looked at, then by halves
+            const int t = min(tile + 1 + lane, tiles - 1);
+            const unsigned long long other = __ballot(t == tiles - 1 || keys[(t + 1) * tile_len - 1] != cur);
+            if (other) {
+                last = min(tile + __ffsll(other), tiles - 1);
+            } else {
+                int lo = tile + 65, hi = tiles - 1;
+                while (lo < hi) {
+                    const int mid = lo + ((hi - lo) >> 1);
+                    if (keys[(mid + 1) * tile_len - 1] == cur) lo = mid + 1;
+                    else hi = mid;
+                }
+                last = lo;
+            }
+            if (keys[last * tile_len] != cur) --last;            // (the run ends with the tile before)
+        }
     }
-    for (int j = 0; j < V; ++j) sm[wave][j * 64 + lane] = acc[j];
-    __syncthreads();
-    if (wave == 0) {
-        for (int w = 1; w < 8; ++w)
-            for (int j = 0; j < V; ++j) acc[j] += sm[w][j * 64 + lane];
+    const bool alone = last >= 0 && last - tile < 2 * JOINERS;
+    if (alone) {
+        float acc[V];
+        for (int j = 0; j < V; ++j) acc[j] = 0.f;
+        add(acc, tile, tile, last, 1);
         write_cols<T>(dtable + (long long)cur * dim, (chunk * 64 + lane) * V, dim, acc, scale, accumulate);
+    }
+    if (lane == 0) {
+        last_s[wave] = alone ? -1 : last;
+        cur_s[wave] = cur;
+    }
+    __syncthreads();
+    for (int w = 0; w < JOINERS; ++w) {
+        if (last_s[w] < 0) continue;                              // (the same for the whole workgroup)
+        float acc[V];
+        for (int j = 0; j < V; ++j) acc[j] = 0.f;
+        add(acc, tile0 + w, tile0 + w + wave, last_s[w], JOINERS);
+        for (int j = 0; j < V; ++j) sm[wave][j * 64 + lane] = acc[j];
+        __syncthreads();
+        if (wave == 0) {
+            for (int o = 1; o < JOINERS; ++o)
+                for (int j = 0; j < V; ++j) acc[j] += sm[o][j * 64 + lane];
+            write_cols<T>(dtable + (long long)cur_s[w] * dim, (chunk * 64 + lane) * V, dim, acc, scale, accumulate);
+        }
+        __syncthreads();
     }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
-int tile_len_of(long long n) { return n <= SMALL ? 16 : 64; }     // few positions: more wavefronts
+// Short tiles where long ones are fewer than sixteen wavefronts for each of 256 compute units (sums and joins, bf16, 512 columns:
+// 65536 positions 72 us with 64, 42 with 16; 131072 66 and 58; 262144 97 and 117)
+int tile_len_of(long long n, int chunks) { return cdiv(n, 64) * (long long)chunks < 4096 ? 16 : 64; }
 
 struct Layout {
     long long keys[2], pos[2], counts, totals, pieces, touched, bytes;
@@ -464,7 +504,7 @@ Layout layout(long long n, int dim, long long n_entries) {
     }
     l.counts = take(small ? 0 : 4 * LBINS * tiles);
     l.totals = take(4 * LBINS);
-    l.pieces = take(4 * 2 * cols * cdiv(n, tile_len_of(n)));
+    l.pieces = take(4 * 2 * cols * cdiv(n, tile_len_of(n, cdiv(dim, 512))));      // (bf16 has the fewer chunks)
     l.touched = take(n_entries);        // (a multiple of 256: cleared in 16-byte steps)
     l.bytes = at;
     return l;
@@ -477,18 +517,17 @@ bool valid_sizes(long long n, int dim, long long n_entries) {
 template <typename T>
 int launch_sums(const unsigned* keys, const int* pos, int n, const void* dy, long long ldy, int dim, long long n_entries, float scale,
                 void* dtable, int accumulate, float* pieces, const unsigned char* touched, hipStream_t st) {
-    const int tl = tile_len_of(n), tiles = cdiv(n, tl), chunks = cdiv(dim, 64 * Vec<T>::N);
+    const int chunks = cdiv(dim, 64 * Vec<T>::N), tl = tile_len_of(n, chunks), tiles = cdiv(n, tl);
     const long long blocks = ((long long)tiles * chunks + 3) / 4;
-    const int zero_rows = n_entries < 65536 ? 16 : 64;            // a small table: more wavefronts
-    const long long zero = touched ? (n_entries + 4 * zero_rows - 1) / (4 * zero_rows) : 0;
+    const long long zero = touched ? (n_entries + 4 * ZERO_ROWS - 1) / (4 * ZERO_ROWS) : 0;
     if (blocks + zero > 0x7fffffffLL || (long long)tiles * chunks > 0x7fffffffLL) return S2AG_E_UNSUPPORTED;
     if (blocks + zero)
         hipLaunchKernelGGL(sum_k<T>, dim3((unsigned)(blocks + zero)), dim3(256), 0, st, keys, pos, n, static_cast<const T*>(dy), ldy, dim,
-                           n_entries, scale, static_cast<T*>(dtable), accumulate, tl, tiles, chunks, pieces, touched, (int)blocks, zero_rows);
+                           n_entries, scale, static_cast<T*>(dtable), accumulate, tl, tiles, chunks, pieces, touched, (int)blocks);
     S2AG_LAUNCH_CHECK();
     if (tiles > 1) {
-        hipLaunchKernelGGL(join_k<T>, dim3((unsigned)((long long)(tiles - 1) * chunks)), dim3(512), 0, st, keys, n, dim, n_entries, scale,
-                           static_cast<T*>(dtable), accumulate, tl, chunks, pieces);
+        hipLaunchKernelGGL(join_k<T>, dim3((unsigned)(cdiv(tiles - 1, JOINERS) * (long long)chunks)), dim3(64 * JOINERS), 0, st, keys,
+                           n, dim, n_entries, scale, static_cast<T*>(dtable), accumulate, tl, tiles, chunks, pieces);
         S2AG_LAUNCH_CHECK();
     }
     return 0;
@@ -538,7 +577,7 @@ extern "C" int s2ag_emb_grad(const void* ids, int ids_i32, const void* dy, long 
     int bits = 1;
     while ((n_entries >> bits) != 0) ++bits;                       // the keys 0 .. n_entries
     const bool small = n <= SMALL;
-    const bool clear_inside = n > 0 && (!small || n_entries <= 131072);        // by the sort's first launch
+    const bool clear_inside = n > 0 && (!small || n_entries <= 131072);        // by the sort's first launch (0.7 us of its one workgroup for 131072 rows; a launch of its own 2.4)
     if (touched && !clear_inside)
         if (hipError_t e = zero_async(touched, (size_t)round_up(n_entries, 4), st)) return (int)e;
     if (n > 0 && small) {

@@ -101,6 +101,24 @@ def test_embedding_sorted(S, case, kind, dtype):
     assert torch.equal(first, t.grad)
 
 
+@pytest.mark.parametrize('tile,dim,dtype', [(16, 20, 'fp32'), (16, 600, 'bf16'),
+                                            pytest.param(64, 4100, 'fp32', marks=pytest.mark.skipif(EMU, reason='a hundred million values'))])
+def test_embedding_sorted_runs_that_end_with_a_tile(S, tile, dim, dtype):
+    """Runs of equal ids that begin and end at borders of the tiles the sums go by, one short of them and one behind, across one tile
+    to more than 64 of them."""
+    tiles = [1, 1, 2, 3, 15, 16, 17, 63, 64, 65, 66, 130]
+    lengths = [tile * k for k in tiles] + [5] + [tile * k - 1 for k in tiles] + [tile * k + 1 for k in tiles] + [tile * k for k in tiles]
+    dt = DTYPES[dtype]
+    g = torch.Generator().manual_seed(tile + dim)
+    ids = torch.arange(len(lengths)).repeat_interleave(torch.tensor(lengths))
+    ids = ids[torch.randperm(ids.numel(), generator=g)]
+    table, dy = torch.randn(len(lengths), dim, generator=g).to(dt), torch.randn(ids.numel(), dim, generator=g).to(dt)
+    _, (gr, gb) = embedding_reference(ids, table, dy, 1.0, None, dt)
+    t = table.cuda().requires_grad_(True)
+    S['ops'].embedding_sorted(ids.cuda(), t).backward(dy.cuda())
+    within(t.grad, gr, gb)
+
+
 def test_embedding_sorted_padding_row_shapes_and_small_ids(S):
     g = torch.Generator().manual_seed(3)
     ids = ids_of('padded', 6 * 35, 50, g).view(6, 35)
