@@ -9,6 +9,10 @@
 // inside its tile, and leaves the sums of the runs that cross a tile's border (at most two a tile) to a second launch, which
 // adds the pieces of a run in order.
 //
+// Measured, 65536 ids of a table of 131072 x 2048, bf16: lookup 81 us (268 MB read, 268 written: 6.6 TB/s); gradient 211 us, of them
+// sorting 31, sums and zeros 172 (268 MB read, 537 written: 4.7 TB/s), joins 8.  4352 ids of a table of 20000 x 300, fp32: 5 us
+// and 34.  A copy of 2 GB runs at 4.7 TB/s.
+//
 // ids that are not in the table, and the padding row's, sort behind the last row under the key n_entries and are not summed.
 #include "text_common.h"
 

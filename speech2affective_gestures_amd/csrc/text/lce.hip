@@ -187,7 +187,7 @@ struct Product {
     bool fp32;                          // operands in pieces
     // STATS, GRADS of fp32: rows of R and Q are 2^power of what is multiplied
     const int *r_power, *q_power;
-    int tiles_q, group;
+    int tiles_q;
     int splits, slots;                  // the most parts of k; workgroups that run at a time
     // STATS: max and sum of exponentials [tile_q][padded rows], logit of the target
     const int* tgt;
@@ -275,9 +275,11 @@ __device__ __forceinline__ float exp_of(float d) {
     return fmaf(e * 0.693147180559945f, rest, e);
 }
 
+constexpr int GROUP = 8;                // row tiles that the columns pass by at a time
+
 // The tiles of a launch, in the order in which they are handed out; everything here is one for the workgroup.
 struct Tiles {
-    int n, splits, per, group, tiles_r, kt;
+    int n, splits, per, tiles_r, kt;
     int stages, more;                   // of a part of k; so many parts have one more
 };
 __host__ __device__ inline int splits_of(int tiles, int most, int slots) {       // few tiles: k is split to fill the card
@@ -425,13 +427,13 @@ __global__ __launch_bounds__(64 * WR * WQ, BR == 256 ? 1 : 2) void product_k(Pro
     ts.kt = p.k_count ? __builtin_amdgcn_readfirstlane((*p.k_count + BK - 1) / BK) : p.k / BK;
     ts.stages = __builtin_amdgcn_readfirstlane(ts.kt * pairs / ts.splits);
     ts.more = ts.kt * pairs - ts.stages * ts.splits;
-    ts.group = p.group;
-    ts.per = p.group * p.tiles_q;
+    ts.per = GROUP * p.tiles_q;
     ts.n = ts.tiles_r * p.tiles_q * ts.splits;
 
     // A workgroup takes many tiles, so that the operands of the next one are on their way while this one ends.  Workgroups are
     // dealt to the eight XCDs in turn; each XCD gets a contiguous range of tiles, and inside it the tiles go column by column
-    // over `group` row tiles, so that the tiles that run at the same time share operands in its L2.
+    // over GROUP row tiles, so that the tiles that run at the same time share operands in its L2.  (8192 rows,
+    // 131072 words of 2048 values: 12.3 ms with groups of 8 or 4, 12.7 of 2.)
     const int xcd = blockIdx.x & 7, step = gridDim.x >> 3;
     const int last = __builtin_amdgcn_readfirstlane((int)((long long)ts.n * (xcd + 1) / 8));
     const int first = __builtin_amdgcn_readfirstlane((int)((long long)ts.n * xcd / 8)) + (blockIdx.x >> 3);
@@ -445,7 +447,7 @@ __global__ __launch_bounds__(64 * WR * WQ, BR == 256 ? 1 : 2) void product_k(Pro
         Place t;
         t.split = __builtin_amdgcn_readfirstlane(v / (ts.tiles_r * p.tiles_q));
         v -= t.split * ts.tiles_r * p.tiles_q;
-        const int grp = __builtin_amdgcn_readfirstlane(v / ts.per), g0 = grp * ts.group, gsz = min(ts.tiles_r - g0, ts.group);
+        const int grp = __builtin_amdgcn_readfirstlane(v / ts.per), g0 = grp * GROUP, gsz = min(ts.tiles_r - g0, GROUP);
         t.r0 = (long long)__builtin_amdgcn_readfirstlane(g0 + (v - grp * ts.per) % gsz) * BR;
         t.c0 = (long long)__builtin_amdgcn_readfirstlane((v - grp * ts.per) / gsz) * BQ;
         t.it0 = ts.stages * t.split + min(t.split, ts.more);
@@ -987,11 +989,6 @@ int launch_tiles(Product& p, long long r_rows, long long q_rows, hipStream_t st)
     // (every time: the attribute belongs to the current device)
     if (hipFuncSetAttribute((const void*)product_k<BR, BQ, WR, WQ, END, PRECISE>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess)
         return S2AG_E_UNSUPPORTED;
-    // The rows of R of a group stay in an XCD's 4 MB L2 while the columns pass, if half of it holds them (k of 1024: 4 row tiles
-    // 816 TFLOP/s, 8 of them 560; of 2048: 2 row tiles 1023, 8 of them 841); where not two fit, the 8 x 4 tiles that run at a time
-    // share what they can.
-    const long long fit = (2LL << 20) / (2LL * BR * (p.k_count ? p.r_deep : p.k));
-    p.group = fit >= 8 || fit < 2 ? 8 : fit >= 4 ? 4 : 2;
     p.tiles_q = cdiv(q_rows, BQ);
     p.slots = SLOTS * PER_CU;
     if (p.splits < 1) p.splits = 1;
