@@ -36,7 +36,8 @@ int s2ag_clip_grads(const s2ag_clip_tensor* t /*host*/, int tensors, float max_n
  * out[i] = round(scale * table[ids[i]]), rows of `dim` elements, contiguous.  An id outside [0, n_entries) reads as zeros. */
 int s2ag_emb_lookup(const void* ids, int ids_i32, const void* table, int bf16, long long n, int dim, long long n_entries,
                     float scale, void* out, void* stream);
-/* dtable[v] = round(scale * sum of dy[i] over the i with ids[i] == v, in the order of i); rows without an id and the row
+/* dtable[v] = round(scale * sum of dy[i] over the i with ids[i] == v, in an order that the ids
+ * decide); rows without an id and the row
  * `padding_idx` (-1: none) are written as zeros.  accumulate: fp32 only, dtable[v] += ... and rows without an id are left as
  * they are.  `ldy`: row pitch of dy in elements.  ids outside [0, n_entries) send nothing.  n < 2^31 - 2^16, n_entries < 2^30. */
 long long s2ag_emb_grad_workspace_bytes(long long n, int dim, long long n_entries);

@@ -91,7 +91,8 @@ struct Operand {
 };
 
 __device__ __forceinline__ void split3(float v, bf16_t* q) {
-    q[0] = (bf16_t)v;
+    const float most = 3.3895313892515355e38f;                   // bf16's largest: fp32's own would round to an infinity
+    q[0] = fabsf(v) < INFINITY ? (bf16_t)fminf(fmaxf(v, -most), most) : (bf16_t)v;
     const float r1 = v - (float)q[0];   // exact
     q[1] = (bf16_t)r1;
     q[2] = (bf16_t)(r1 - (float)q[1]);

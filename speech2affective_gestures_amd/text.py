@@ -129,7 +129,7 @@ def embedding_sorted(ids: Tensor, table: Tensor, scale: float = 1.0, padding_idx
 
     ids: int64 or int32, any shape; an id outside the table reads as a row of zeros and sends no gradient.  table: (n, dim) fp32 or
     bf16.  padding_idx: a row that is looked up like any other and gets no gradient.
-    The table's gradient is summed per id in the order of the positions, in fp32, and rounded once.  Where the table is a parameter of
+    The table's gradient is summed per id in fp32, in an order that the ids alone decide, and rounded once.  Where the table is a parameter of
     an optim.ParamArena, the backward pass adds to its gradient there, in the rows that were looked up, and hands autograd None."""
     what = 'embedding_sorted'
     _check_tensors(what, ids=ids, table=table)
@@ -211,7 +211,7 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, ignore_index
     x: (..., dim), weight: (vocab, dim), both fp32 or both bf16; target: (...) int64 or int32.  Rows whose target is
     ``ignore_index`` have a loss and a gradient of zero and are left out of every product.  reduction: 'mean' over the other rows
     (0 if there are none), 'sum', or 'none' (target's shape).  A target outside the vocabulary that is not ``ignore_index`` makes that
-    row's loss NaN, and every gradient that it enters.
+    row's loss NaN, and every gradient that it enters.  So does, in fp32, an infinity in a row of x or weight.
     At most 2^21 rows and 2^21 words.  Where the weight is a parameter of an optim.ParamArena, the backward pass adds to its gradient
     there and hands autograd None."""
     what = 'linear_cross_entropy'

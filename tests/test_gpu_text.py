@@ -373,6 +373,25 @@ def test_linear_cross_entropy_large_logits(S):
 
 
 @pytest.mark.parametrize('dtype', list(DTYPES))
+def test_linear_cross_entropy_words_of_the_lowest_value(S, dtype):
+    """Words that their weights rule out, every one the type's lowest value: as if the vocabulary did not have them."""
+    x, w, t, g = lce_case(40, 24, 300, dtype, 0.2)
+    x = x.abs() + 0.125
+    t = torch.where(t == IGNORE, t, t % 250)
+    low = w.clone()
+    low[250:] = torch.finfo(w.dtype).min
+    gout = torch.randn((), generator=g)
+    (l, lb), (dx, dxb), (dw, dwb) = lce_reference(x, w[:250], t, gout, 'mean')
+    xg, wg = x.cuda().requires_grad_(True), low.cuda().requires_grad_(True)
+    loss = S['ops'].linear_cross_entropy(xg, wg, t.cuda())
+    within(loss, l, lb)
+    loss.backward(gout.cuda())
+    within(xg.grad, dx, dxb)
+    within(wg.grad[:250], dw, dwb)
+    assert float(wg.grad[250:].abs().max()) == 0.0
+
+
+@pytest.mark.parametrize('dtype', list(DTYPES))
 def test_linear_cross_entropy_powers_of_two_of_rows_and_words_cancel(S, dtype):
     """Rows and words of very different sizes whose products are ordinary: a power of two changes no bit of the loss, and moves the
     gradients by itself."""
