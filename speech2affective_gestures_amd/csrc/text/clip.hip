@@ -219,12 +219,9 @@ int run(const s2ag_clip_tensor* a, int tensors, float max_norm, double* partials
     at = tensors > 0 ? (tensors - 1) / GROUP * GROUP : 0;
     do {
         const unsigned chunks = fill(t, a, at, tensors);
-        bool any = out != nullptr;
         bool write = false;
-        for (int i = 0; i < t.tensors; ++i)
-            write |= t.dst[i] != nullptr && (t.dst[i] != t.src[i] || max_norm < INFINITY);
-        any |= write;
-        if (any) {
+        for (int i = 0; i < t.tensors; ++i) write |= t.dst[i] != nullptr;
+        if (write || out) {
             if (!write) t.first[t.tensors] = 0;
             hipLaunchKernelGGL(scale_k<INF>, dim3(write ? blocks_of(chunks) : 1), dim3(256), 0, st, t, partials, count, max_norm, out);
             S2AG_LAUNCH_CHECK();

@@ -89,7 +89,8 @@ class FusedAdam:
         a.epoch += 1            # tensors derived from these parameters (ops._DerivedGroup) are stale now
 
     def clip_grad_norm(self, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
-        """Clips the arena's gradients in place (``clip_grads``); call it between the backward pass and ``step``."""
+        """Clips the arena's gradients in place (``clip_grads``); call it between the backward pass and ``step``.  The norm is that of
+        the gradients as they stand: before ``step``'s grad_scale, which has to be allowed for in max_norm."""
         return clip_grads([self.arena.grad], max_norm, norm_type)
 
     def state_dict(self):

@@ -559,6 +559,11 @@ def test_clip_grads_values_out_of_the_ordinary(S):
             x = x.cuda()
             assert math.isnan(float(S['optim'].clip_grads([x], 1.0, norm_type)))
             assert torch.isnan(x).all()
+        x, y = torch.ones(1000).cuda(), torch.full((7,), float('nan')).cuda()
+        assert math.isnan(float(S['optim'].clip_grads([x, y], math.inf, norm_type))) and torch.isnan(x).all()
+        x = torch.randn(1000).cuda()
+        y = x.clone()
+        assert float(S['optim'].clip_grads([x], math.inf, norm_type)) > 0 and torch.equal(x, y)
     z = torch.zeros(30).cuda()
     assert float(S['optim'].clip_grads([z], 1.0)) == 0.0 and float(z.abs().max()) == 0.0
     assert float(S['optim'].clip_grads([torch.zeros(0).cuda()], 1.0)) == 0.0
