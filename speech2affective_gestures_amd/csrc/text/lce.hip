@@ -54,14 +54,22 @@ State state_of(void* p, long long rows) {
 }
 
 // ---- rows that have a target, packed in order --------------------------------------------------------------------------------
-__global__ __launch_bounds__(1024) void select_rows_k(const void* __restrict__ target, int i32, long long rows, long long vocab,
-                                                      long long ignore, State s, float* loss_rows) {
+struct Select {
+    const void* target;
+    int i32;
+    long long rows, vocab, ignore;
+    State s;
+    float* loss_rows;
+};
+__device__ __forceinline__ void select_rows(const Select& q) {   // one workgroup of 1024
+    const long long rows = q.rows, vocab = q.vocab, ignore = q.ignore;
+    const State& s = q.s;
     __shared__ int sm[16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int base = 0;
     for (long long r0 = 0; r0 < rows; r0 += 1024) {
         const long long r = r0 + threadIdx.x;
-        const long long t = r < rows ? load_id(target, i32, r) : ignore;
+        const long long t = r < rows ? load_id(q.target, q.i32, r) : ignore;
         const bool keep = t != ignore;
         const unsigned long long m = __ballot(keep);
         if (lane == 0) sm[wave] = __popcll(m);
@@ -77,12 +85,13 @@ __global__ __launch_bounds__(1024) void select_rows_k(const void* __restrict__ t
         }
         if (r < rows) {
             s.inv[r] = keep ? at : -1;
-            if (loss_rows && !keep) loss_rows[r] = 0.f;
+            if (q.loss_rows && !keep) q.loss_rows[r] = 0.f;
         }
         __syncthreads();
     }
     if (threadIdx.x == 0) *s.count = base;
 }
+__global__ __launch_bounds__(1024) void select_rows_k(Select q) { select_rows(q); }
 
 // ---- operands: rows of features, padded with zeros to a multiple of 64, fp32 as three bf16 pieces --------------------------------
 struct Operand {
@@ -112,14 +121,39 @@ __device__ __forceinline__ void load8(const T* s, int c, int dim, bool in, float
     }
 }
 
+// What a packing launch does: rows of `src` by way of rowmap, or all of them, to `dst` or to the halves, powers and pieces.
+template <typename T> struct Pack;
+template <> struct Pack<bf16_t> {
+    const bf16_t* src;
+    long long ld;
+    int dim, kp;
+    const int *rowmap, *count;
+    long long rows;
+    bf16_t* dst;
+};
+template <> struct Pack<float> {
+    const float* src;
+    long long ld;
+    int dim, kp;
+    const int *rowmap, *count;
+    long long rows;
+    f16_t* halves;
+    int* power;
+    bf16_t* pieces;                     // may be null
+    long long plane;
+};
+
 // dst[r][0..kp) from row rowmap[r] (or r) of src, zeros behind column dim
-__global__ __launch_bounds__(256) void pack_k(const bf16_t* __restrict__ src, long long ld, int dim, const int* __restrict__ rowmap,
-                                              const int* __restrict__ count, long long rows, bf16_t* __restrict__ dst, int kp) {
+__device__ __forceinline__ void pack_rows(const Pack<bf16_t>& q, unsigned block, unsigned blocks) {
+    const bf16_t* __restrict__ src = q.src;
+    bf16_t* __restrict__ dst = q.dst;
+    const int* rowmap = q.rowmap;
+    const long long ld = q.ld;
+    const int dim = q.dim, kp = q.kp, groups = kp / 8;
     long long live;
-    const long long end = packed_rows(count, rows, &live);
-    const int groups = kp / 8;
+    const long long end = packed_rows(q.count, q.rows, &live);
     const long long total = end * groups;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    for (long long i = (long long)block * blockDim.x + threadIdx.x; i < total; i += (long long)blocks * blockDim.x) {
         const long long r = i / groups;
         const int c = (int)(i - r * groups) * 8;
         const bool in = r < live;
@@ -131,13 +165,18 @@ __global__ __launch_bounds__(256) void pack_k(const bf16_t* __restrict__ src, lo
 
 // The same of fp32, a wavefront to a row: two halves, the row times 2^-power[r] of them, and three bf16 pieces if they are wanted.
 // An infinity leaves NaN in the pieces behind it, as its products would anyway.
-__global__ __launch_bounds__(256) void pack32_k(const float* __restrict__ src, long long ld, int dim, const int* __restrict__ rowmap,
-                                                const int* __restrict__ count, long long rows, int kp, f16_t* __restrict__ halves,
-                                                int* __restrict__ power, bf16_t* __restrict__ pieces, long long plane) {
+__device__ __forceinline__ void pack_rows(const Pack<float>& p, unsigned block, unsigned blocks) {
+    const float* __restrict__ src = p.src;
+    f16_t* __restrict__ halves = p.halves;
+    bf16_t* __restrict__ pieces = p.pieces;
+    int* __restrict__ power = p.power;
+    const int* rowmap = p.rowmap;
+    const long long ld = p.ld, plane = p.plane;
+    const int dim = p.dim, kp = p.kp, waves = blockDim.x >> 6;
     long long live;
-    const long long end = packed_rows(count, rows, &live);
+    const long long end = packed_rows(p.count, p.rows, &live);
     const int lane = threadIdx.x & 63;
-    for (long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); r < end; r += (long long)gridDim.x * 4) {
+    for (long long r = (long long)block * waves + (threadIdx.x >> 6); r < end; r += (long long)blocks * waves) {
         const bool in = r < live;
         const float* s = src + (in ? (rowmap ? (long long)rowmap[r] : r) : 0) * ld;
         float top = 0.f;
@@ -162,15 +201,22 @@ __global__ __launch_bounds__(256) void pack32_k(const float* __restrict__ src, l
                 const float t = ldexpf(v[j], up);
                 h[0][j] = (f16_t)t;
                 h[1][j] = (f16_t)(t - (float)h[0][j]);           // (the difference is exact)
-                bf16_t p[3];
-                split3(v[j], p);
-                for (int k = 0; k < 3; ++k) q[k][j] = p[k];
+                bf16_t piece[3];
+                split3(v[j], piece);
+                for (int k = 0; k < 3; ++k) q[k][j] = piece[k];
             }
             for (int k = 0; k < 2; ++k) *reinterpret_cast<f16x8*>(halves + k * plane + r * kp + c) = h[k];
             if (pieces)
                 for (int k = 0; k < 3; ++k) *reinterpret_cast<bf16x8*>(pieces + k * plane + r * kp + c) = q[k];
         }
     }
+}
+
+template <typename T> __global__ __launch_bounds__(256) void pack_k(Pack<T> q) { pack_rows(q, blockIdx.x, gridDim.x); }
+// W does not wait for the rows: its packing and their selection are one launch.
+template <typename T> __global__ __launch_bounds__(1024) void select_and_pack_k(Select s, Pack<T> q) {
+    if (blockIdx.x == 0) select_rows(s);
+    else pack_rows(q, blockIdx.x - 1, gridDim.x - 1);
 }
 
 // ---- the tiled product -------------------------------------------------------------------------------------------------------
@@ -1010,10 +1056,11 @@ int launch(Product& p, bool big, long long r_rows, long long q_rows, hipStream_t
     return big ? launch_tiles<256, 256, 2, 2, END, false>(p, r_rows, q_rows, st) : launch_tiles<128, 128, 2, 2, END, false>(p, r_rows, q_rows, st);
 }
 
-unsigned grid_of(long long work) {
-    const long long b = (work + 255) / 256;
-    return (unsigned)(b < 1 ? 1 : b > 4096 ? 4096 : b);
+unsigned grid_of(long long work, int block = 256) {
+    const long long b = (work + block - 1) / block, most = 4096 * 256 / block;
+    return (unsigned)(b < 1 ? 1 : b > most ? most : b);
 }
+template <typename T> long long packers(int kp) { return sizeof(T) == 4 ? 64 : kp / 8; }      // threads to a row
 
 // where the packed operands are, or the caller's W as it is
 char* packed(const s2ag_lce_args* a, const Plan& p) { return static_cast<char*>(p.kept ? a->state : a->workspace); }
@@ -1038,28 +1085,47 @@ void logit_operands(const s2ag_lce_args* a, const Plan& p, long long v0, Product
     q->fp32 = !a->bf16;
 }
 
-int pack(const s2ag_lce_args* a, const Plan& p, const State& s, hipStream_t st) {
-    char* at = packed(a, p);
-    if (a->bf16) {
-        hipLaunchKernelGGL(pack_k, dim3(grid_of(p.np * (p.kp / 8))), dim3(256), 0, st, static_cast<const bf16_t*>(a->x), a->ldx, a->dim, s.rowmap,
-                           s.count, p.np, reinterpret_cast<bf16_t*>(at + p.xp), p.kp);
-        S2AG_LAUNCH_CHECK();
-        if (p.pack_w) {
-            hipLaunchKernelGGL(pack_k, dim3(grid_of(a->vocab * (p.kp / 8))), dim3(256), 0, st, static_cast<const bf16_t*>(a->w), a->ldw, a->dim,
-                               (const int*)nullptr, (const int*)nullptr, a->vocab, reinterpret_cast<bf16_t*>(at + p.wp), p.kp);
-            S2AG_LAUNCH_CHECK();
-        }
-        return 0;
-    }
-    hipLaunchKernelGGL(pack32_k, dim3(grid_of(p.np * 64)), dim3(256), 0, st, static_cast<const float*>(a->x), a->ldx, a->dim, s.rowmap, s.count, p.np,
-                       p.kp, reinterpret_cast<f16_t*>(at + p.xh), reinterpret_cast<int*>(at + p.x_power),
-                       p.kept ? reinterpret_cast<bf16_t*>(at + p.xp) : nullptr, p.np * p.kp);
+template <typename T>
+int pack(const s2ag_lce_args* a, const Plan& p, const Select& s, Pack<T> x, Pack<T> w, hipStream_t st) {
+    x.src = static_cast<const T*>(a->x);
+    x.ld = a->ldx;
+    x.rows = p.np;
+    x.rowmap = s.s.rowmap;
+    x.count = s.s.count;
+    w.src = static_cast<const T*>(a->w);
+    w.ld = a->ldw;
+    w.rows = a->vocab;
+    x.dim = w.dim = a->dim;
+    x.kp = w.kp = p.kp;
+    if (p.pack_w)
+        hipLaunchKernelGGL(select_and_pack_k<T>, dim3(1 + grid_of(a->vocab * packers<T>(p.kp), 1024)), dim3(1024), 0, st, s, w);
+    else
+        hipLaunchKernelGGL(select_rows_k, dim3(1), dim3(1024), 0, st, s);
     S2AG_LAUNCH_CHECK();
-    hipLaunchKernelGGL(pack32_k, dim3(grid_of(a->vocab * 64)), dim3(256), 0, st, static_cast<const float*>(a->w), a->ldw, a->dim, (const int*)nullptr,
-                       (const int*)nullptr, a->vocab, p.kp, reinterpret_cast<f16_t*>(at + p.wh), reinterpret_cast<int*>(at + p.w_power),
-                       p.kept ? reinterpret_cast<bf16_t*>(at + p.wp) : nullptr, a->vocab * p.kp);
+    hipLaunchKernelGGL(pack_k<T>, dim3(grid_of(p.np * packers<T>(p.kp), 256)), dim3(256), 0, st, x);
     S2AG_LAUNCH_CHECK();
     return 0;
+}
+int select_and_pack(const s2ag_lce_args* a, const Plan& p, const Select& s, hipStream_t st) {
+    char* at = packed(a, p);
+    if (a->bf16) {
+        Pack<bf16_t> x{}, w{};
+        x.dst = reinterpret_cast<bf16_t*>(at + p.xp);
+        w.dst = reinterpret_cast<bf16_t*>(at + p.wp);
+        return pack(a, p, s, x, w, st);
+    }
+    Pack<float> x{}, w{};
+    x.halves = reinterpret_cast<f16_t*>(at + p.xh);
+    w.halves = reinterpret_cast<f16_t*>(at + p.wh);
+    x.power = reinterpret_cast<int*>(at + p.x_power);
+    w.power = reinterpret_cast<int*>(at + p.w_power);
+    if (p.kept) {
+        x.pieces = reinterpret_cast<bf16_t*>(at + p.xp);
+        w.pieces = reinterpret_cast<bf16_t*>(at + p.wp);
+    }
+    x.plane = p.np * p.kp;
+    w.plane = a->vocab * p.kp;
+    return pack(a, p, s, x, w, st);
 }
 
 bool ready(const s2ag_lce_args* a, const Plan& p) {
@@ -1085,12 +1151,13 @@ extern "C" int s2ag_lce_fwd(const s2ag_lce_args* a, void* stream) {
     const State s = state_of(a->state, a->rows);
     char* ws = static_cast<char*>(a->workspace);
     float* row_loss = reinterpret_cast<float*>(ws + p.row_loss);
-    hipLaunchKernelGGL(select_rows_k, dim3(1), dim3(1024), 0, st, a->target, a->target_i32, a->rows, a->vocab, a->ignore_index, s,
-                       a->reduction == S2AG_LCE_NONE ? a->loss : nullptr);
-    S2AG_LAUNCH_CHECK();
-    if (a->rows) {
+    const Select sel{a->target, a->target_i32, a->rows, a->vocab, a->ignore_index, s, a->reduction == S2AG_LCE_NONE ? a->loss : nullptr};
+    if (a->rows == 0) {
+        hipLaunchKernelGGL(select_rows_k, dim3(1), dim3(1024), 0, st, sel);
+        S2AG_LAUNCH_CHECK();
+    } else {
         Product q{};
-        if (int rc = pack(a, p, s, st)) return rc;
+        if (int rc = select_and_pack(a, p, sel, st)) return rc;
         logit_operands(a, p, 0, &q);
         q.q_rows = q.vocab = a->vocab;
         q.r_count = s.count;
