@@ -855,29 +855,33 @@ __global__ __launch_bounds__(64 * WR * WQ, BR == 256 ? 1 : 2) void product_k(Pro
 
 // ---- joins -------------------------------------------------------------------------------------------------------------------
 // A lane per row, sixteen wavefronts over the tiles.
+// 16 rows to a workgroup, 64 lanes to a row: a few loads in turn for any vocabulary (391 tiles: 7 us; 64 rows to a workgroup,
+// 16 lanes to a row, took 14)
+struct MaxSum {
+    float m, sum;
+    __device__ __forceinline__ void take(float2 q) {
+        const float n = q.x > m ? q.x : m, ns = n == -INFINITY ? 0.f : n;
+        sum = sum * expf(m - ns) + q.y * expf(q.x - ns);
+        m = n;
+    }
+};
 __global__ __launch_bounds__(1024) void join_stats_k(const float2* __restrict__ part, long long part_ld, int tiles, State s,
                                                      const float* __restrict__ target_logit, int reduction, float* __restrict__ loss,
                                                      float* __restrict__ row_loss) {
-    __shared__ float2 sm[16][64];
+    __shared__ float2 sm[16][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, count = *s.count;
-    const int row = blockIdx.x * 64 + lane;
-    if ((int)(blockIdx.x * 64) >= count) return;
-    float m = -INFINITY, sum = 0.f;
-    for (int t = wave; t < tiles; t += 16) {
-        const float2 q = part[t * part_ld + row];
-        const float n = q.x > m ? q.x : m, ns = n == -INFINITY ? 0.f : n;
-        sum = sum * expf(m - ns) + q.y * expf(q.x - ns);
-        m = n;
-    }
-    sm[wave][lane] = make_float2(m, sum);
+    if ((int)(blockIdx.x * 16) >= count) return;
+    const int row = blockIdx.x * 16 + (lane & 15);
+    MaxSum a{-INFINITY, 0.f};
+#pragma unroll 4
+    for (int t = wave * 4 + (lane >> 4); t < tiles; t += 64) a.take(part[t * part_ld + row]);
+    a.take(make_float2(__shfl_xor(a.m, 16), __shfl_xor(a.sum, 16)));
+    a.take(make_float2(__shfl_xor(a.m, 32), __shfl_xor(a.sum, 32)));
+    if (lane < 16) sm[wave][lane] = make_float2(a.m, a.sum);
     __syncthreads();
-    if (wave != 0 || row >= count) return;
-    for (int w = 1; w < 16; ++w) {
-        const float2 q = sm[w][lane];
-        const float n = q.x > m ? q.x : m, ns = n == -INFINITY ? 0.f : n;
-        sum = sum * expf(m - ns) + q.y * expf(q.x - ns);
-        m = n;
-    }
+    if (threadIdx.x >= 16 || row >= count) return;
+    for (int w = 1; w < 16; ++w) a.take(sm[w][lane]);
+    const float m = a.m, sum = a.sum;
     const bool known = s.tgt[row] >= 0;
     const float lse = known ? m + logf(sum) : NAN;
     s.lse[row] = lse;
@@ -900,30 +904,43 @@ __global__ __launch_bounds__(1024) void sum_loss_k(const float* __restrict__ row
     *loss = (float)(reduction == S2AG_LCE_MEAN ? s / (n > 0 ? n : 1) : s);
 }
 
-// dx[r] = factor * sum over the splits of the packed row, zeros for rows that were ignored
+// dx[r] = factor * sum over the splits of the packed row, zeros for rows that were ignored.  Many splits of few values go over
+// the four wavefronts of a workgroup (136 x 300 in 85 splits: 6.2 us; a thread to each four columns 8.3; but 1999 x 520 11 and 8.5).
 template <typename T>
 __global__ __launch_bounds__(256) void finish_dx_k(const float* __restrict__ acc, long long ld, int tile, int tiles_q, int most, int slots,
                                                    State s, const float* __restrict__ scale, int mean, long long rows, int dim,
                                                    T* __restrict__ dx) {
+    __shared__ f32x4 sm[4][64];
     const float f = scale ? (mean ? *scale / (float)max(1, *s.count) : *scale) : 1.f;
     const int groups = (dim + 3) / 4, tiles_r = (*s.count + tile - 1) / tile, splits = splits_of(tiles_r * tiles_q, most, slots);
     const long long split = (long long)tiles_r * tile * ld;
     const long long total = rows * groups;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const long long r = i / groups;
-        const int c = (int)(i - r * groups) * 4, at = s.inv[r];
+    const bool spread = splits > 8 && total <= 65536;            // (the same for every workgroup)
+    const int items = spread ? 64 : 256, first = spread ? threadIdx.x >> 6 : 0, step = spread ? 4 : 1;
+    const int mine = threadIdx.x & (items - 1);
+    for (long long i0 = (long long)blockIdx.x * items; i0 < total; i0 += (long long)gridDim.x * items) {
+        const long long i = i0 + mine, r = i / groups;
+        const int c = (int)(i - r * groups) * 4, at = i < total ? s.inv[r] : -1;
         f32x4 x = {0.f, 0.f, 0.f, 0.f};
         if (at >= 0) {
             const float* q = acc + at * ld + c;
-            int k = 0;
-            for (; k + 8 <= splits; k += 8) {                    // eight loads in flight
+            int k = first;
+            for (; k + 7 * step < splits; k += 8 * step) {       // eight loads in flight
                 f32x4 v[8];
-                for (int u = 0; u < 8; ++u) v[u] = *reinterpret_cast<const f32x4*>(q + (k + u) * split);
+                for (int u = 0; u < 8; ++u) v[u] = *reinterpret_cast<const f32x4*>(q + (k + u * step) * split);
                 for (int u = 0; u < 8; ++u) x += v[u];
             }
-            for (; k < splits; ++k) x += *reinterpret_cast<const f32x4*>(q + k * split);
-            x *= f;
+            for (; k < splits; k += step) x += *reinterpret_cast<const f32x4*>(q + k * split);
         }
+        if (spread) {
+            sm[first][mine] = x;
+            __syncthreads();
+            if (first == 0)
+                for (int w = 1; w < 4; ++w) x += sm[w][mine];
+            __syncthreads();
+        }
+        if (first || i >= total) continue;
+        x *= f;
         T* o = dx + r * dim + c;
         for (int e = 0; e < 4; ++e)
             if (c + e < dim) o[e] = (T)x[e];
@@ -1166,7 +1183,7 @@ extern "C" int s2ag_lce_fwd(const s2ag_lce_args* a, void* stream) {
         q.part_ld = p.np;
         q.target_logit = reinterpret_cast<float*>(ws + p.tl);
         if (int rc = launch<STATS>(q, !short_rows(p.kp) && big_tiles(p.np, a->vocab, LOGIT_RATE), p.np, a->vocab, st)) return rc;
-        hipLaunchKernelGGL(join_stats_k, dim3((unsigned)(p.np / 64)), dim3(1024), 0, st, q.part, q.part_ld, q.tiles_q, s, q.target_logit,
+        hipLaunchKernelGGL(join_stats_k, dim3((unsigned)(p.np / 16)), dim3(1024), 0, st, q.part, q.part_ld, q.tiles_q, s, q.target_logit,
                            a->reduction, a->loss, row_loss);
         S2AG_LAUNCH_CHECK();
     }
@@ -1246,7 +1263,7 @@ extern "C" int s2ag_lce_bwd(const s2ag_lce_args* a, void* stream) {
         }
     }
     if (a->dx && a->rows) {
-        const unsigned gx = grid_of(a->rows * ((a->dim + 3) / 4));
+        const unsigned gx = grid_of(a->rows * ((a->dim + 3) / 4) * 4);
         if (a->bf16)
             hipLaunchKernelGGL(finish_dx_k<bf16_t>, dim3(gx), dim3(256), 0, st, acc, (long long)p.acc_ld, p.acc_tile, cdiv(a->dim, p.acc_tile), p.splits, p.acc_tile == 256 ? SLOTS : small_slots, s,
                                each ? nullptr : a->grad_out, (int)mean, a->rows, a->dim, static_cast<bf16_t*>(a->dx));
