@@ -93,7 +93,7 @@ def _arena_slot(p: Tensor) -> Optional[Tensor]:
 # ----------------------------------------------------------------------------------------------------
 class _EmbeddingSorted(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, ids, table, scale, padding_idx):
+    def forward(ctx, ids, table, scale, padding_idx, grads):
         lib = L.load()
         with _on(table):
             ids = ids.contiguous()
@@ -103,7 +103,7 @@ class _EmbeddingSorted(torch.autograd.Function):
             out = torch.empty(*ids.shape, dim, dtype=data.dtype, device=data.device)
             L.check(lib.s2ag_emb_lookup(ids.data_ptr(), i32, data.data_ptr(), bf16, n, dim, entries, scale, out.data_ptr(), _stream(out)),
                     'emb_lookup')
-        if ctx.needs_input_grad[1]:
+        if grads and ctx.needs_input_grad[1]:
             ctx.save_for_backward(ids)
             # (all that the backward pass needs to know: its thread runs Python code slowly)
             ctx.plan = (lib, table, i32, bf16, n, dim, entries, padding_idx, scale, lib.s2ag_emb_grad_workspace_bytes(n, dim, entries))
@@ -121,7 +121,7 @@ class _EmbeddingSorted(torch.autograd.Function):
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dy.device)
             L.check(lib.s2ag_emb_grad(ids.data_ptr(), i32, dy.data_ptr(), ld, bf16, n, dim, entries, padding_idx, scale, dt.data_ptr(),
                                       slot is not None, ws.data_ptr(), ws_bytes, _stream(dy)), 'emb_grad')
-        return None, (dt if slot is None else None), None, None
+        return None, (dt if slot is None else None), None, None, None
 
 
 def embedding_sorted(ids: Tensor, table: Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> Tensor:
@@ -143,7 +143,7 @@ def embedding_sorted(ids: Tensor, table: Tensor, scale: float = 1.0, padding_idx
         pad = int(padding_idx) + (n if padding_idx < 0 else 0)
         if not 0 <= pad < n:
             raise ValueError(f'{what}: padding_idx {padding_idx} is not a row of a table of {n}')
-    return _EmbeddingSorted.apply(ids, table, float(scale), pad)
+    return _EmbeddingSorted.apply(ids, table, float(scale), pad, torch.is_grad_enabled())
 
 
 # ----------------------------------------------------------------------------------------------------
@@ -160,7 +160,7 @@ def _lce_workspace(lib, a, backward: bool, device) -> Tensor:
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, target, ignore_index, reduction):
+    def forward(ctx, x, weight, target, ignore_index, reduction, grads):
         lib, a = L.load(), L.LceArgs()
         with _on(x):
             xr, a.ldx = _rows(x)
@@ -169,7 +169,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
             a.x, a.w, a.target = xr.data_ptr(), w.data_ptr(), t.data_ptr()
             a.target_i32, a.bf16 = t.dtype == torch.int32, x.dtype == torch.bfloat16
             (a.rows, a.dim), a.vocab = xr.shape, w.shape[0]
-            a.ignore_index, a.reduction, a.keep = ignore_index, reduction, any(ctx.needs_input_grad)
+            # (grads: grad mode at the call; in here it is off, and needs_input_grad does not know of it)
+            a.ignore_index, a.reduction, a.keep = ignore_index, reduction, grads and any(ctx.needs_input_grad)
             state = torch.empty(lib.s2ag_lce_state_bytes(a), dtype=torch.uint8, device=x.device)
             loss = torch.empty(target.shape if reduction == 2 else (), dtype=torch.float32, device=x.device)
             a.state = state.data_ptr()
@@ -202,7 +203,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
                 b.grad_out, b.dx, b.dw, b.dw_accumulate = g.data_ptr(), _p(dx), _p(dw), slot is not None
                 ws = _lce_workspace(lib, b, True, x.device)
                 L.check(lib.s2ag_lce_bwd(b, _stream(ws)), 'lce_bwd')
-        return dx, (dw if slot is None else None), None, None, None
+        return dx, (dw if slot is None else None), None, None, None, None
 
 
 def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, ignore_index: int = -100, reduction: str = 'mean') -> Tensor:
@@ -229,4 +230,4 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, ignore_index
         raise ValueError(f'{what}: ignore_index {ignore_index} is no int64')
     if target.numel() > MAX_ROWS or weight.shape[0] > MAX_WORDS or weight.shape[1] > (1 << 20):
         raise ValueError(f'{what}: at most {MAX_ROWS} rows, {MAX_WORDS} words and {1 << 20} columns')
-    return _LinearCrossEntropy.apply(x, weight, target, ignore_index, _REDUCTIONS[reduction])
+    return _LinearCrossEntropy.apply(x, weight, target, ignore_index, _REDUCTIONS[reduction], torch.is_grad_enabled())

@@ -744,6 +744,23 @@ def test_linear_cross_entropy_kept_graph_and_one_row(S):
     assert one.shape == () and torch.equal(one.detach(), S['ops'].linear_cross_entropy(xg, wg, t.cuda(), reduction='none')[3].detach())
 
 
+def test_text_operators_prepare_no_backward_pass_without_grad_mode(S, monkeypatch):
+    """Parameters under no_grad: scoring a model keeps nothing for a backward pass that cannot come."""
+    from speech2affective_gestures_amd import text
+    kept = []
+    real = text._lce_workspace
+    monkeypatch.setattr(text, '_lce_workspace', lambda lib, a, backward, device: (kept.append(a.keep), real(lib, a, backward, device))[1])
+    x, w, t, _ = lce_case(30, 20, 50, 'fp32', 0.1)
+    x, w, t = x.cuda(), torch.nn.Parameter(w.cuda()), t.cuda()
+    with torch.no_grad():
+        a = S['ops'].linear_cross_entropy(x, w, t)
+        e = S['ops'].embedding_sorted(t.clamp(min=0), w)
+    assert not a.requires_grad and not e.requires_grad
+    b = S['ops'].linear_cross_entropy(x, w, t)
+    assert b.requires_grad and torch.equal(a, b.detach())
+    assert kept == [0, 1]
+
+
 def test_linear_cross_entropy_changed_weight_is_noticed(S):
     """A weight that is changed between the passes: torch's own error, not gradients of two different weights."""
     x, w, t, g = lce_case(10, 24, 30, 'fp32', 0.0)
