@@ -28,6 +28,7 @@
 // fp32: 21, 28, 30 and 28 us, packing 24, the joins and sums 16: there nothing fills the card, and launches and the ends of tiles
 // are most of it.
 #include "text_common.h"
+#include <algorithm>
 #include <type_traits>
 
 namespace {
@@ -909,26 +910,39 @@ __global__ __launch_bounds__(1024) void sum_loss_k(const float* __restrict__ row
     *loss = (float)(reduction == S2AG_LCE_MEAN ? s / (n > 0 ? n : 1) : s);
 }
 
-// dx[r] = factor * sum over the splits of the packed row, zeros for rows that were ignored.  Many splits of few values go over
-// the four wavefronts of a workgroup (136 x 300 in 85 splits: 6.2 us; a thread to each four columns 8.3; but 1999 x 520 11 and 8.5).
+// out[r] = factor * sum over the splits: rows of dX, found by their packed place and zeros where they were ignored, or rows of dW.
+// Many splits of few values go over the four wavefronts of a workgroup (136 x 300 in 85 splits: 6.2 us; a thread to each four
+// columns 8.3; but 1999 x 520 11 and 8.5).
+struct Finish {
+    const float* acc;
+    long long ld;
+    int tile, tiles_q, most, slots;     // of the product
+    const int *count, *inv;             // packed rows and their places; null: every row is its own
+    const int* mean;                    // the number that `scale` is divided by, or null
+    const float* scale;                 // or null
+    long long rows;
+    int dim, add;
+    void* out;
+};
 template <typename T>
-__global__ __launch_bounds__(256) void finish_dx_k(const float* __restrict__ acc, long long ld, int tile, int tiles_q, int most, int slots,
-                                                   State s, const float* __restrict__ scale, int mean, long long rows, int dim,
-                                                   T* __restrict__ dx) {
+__global__ __launch_bounds__(256) void finish_k(Finish p) {
     __shared__ f32x4 sm[4][64];
-    const float f = scale ? (mean ? *scale / (float)max(1, *s.count) : *scale) : 1.f;
-    const int groups = (dim + 3) / 4, tiles_r = (*s.count + tile - 1) / tile, splits = splits_of(tiles_r * tiles_q, most, slots);
-    const long long split = (long long)tiles_r * tile * ld;
-    const long long total = rows * groups;
+    float f = p.scale ? *p.scale : 1.f;
+    if (p.mean) f /= (float)max(1, *p.mean);
+    const int groups = (p.dim + 3) / 4, tiles_r = ((p.count ? *p.count : (int)p.rows) + p.tile - 1) / p.tile;
+    const int splits = splits_of(tiles_r * p.tiles_q, p.most, p.slots);
+    const long long split = (long long)tiles_r * p.tile * p.ld;
+    const long long total = p.rows * groups;
     const bool spread = splits > 8 && total <= 65536;            // (the same for every workgroup)
     const int items = spread ? 64 : 256, first = spread ? threadIdx.x >> 6 : 0, step = spread ? 4 : 1;
     const int mine = threadIdx.x & (items - 1);
     for (long long i0 = (long long)blockIdx.x * items; i0 < total; i0 += (long long)gridDim.x * items) {
         const long long i = i0 + mine, r = i / groups;
-        const int c = (int)(i - r * groups) * 4, at = i < total ? s.inv[r] : -1;
+        const int c = (int)(i - r * groups) * 4;
+        const long long at = i >= total ? -1 : p.inv ? (long long)p.inv[r] : r;
         f32x4 x = {0.f, 0.f, 0.f, 0.f};
         if (at >= 0) {
-            const float* q = acc + at * ld + c;
+            const float* q = p.acc + at * p.ld + c;
             int k = first;
             for (; k + 7 * step < splits; k += 8 * step) {       // eight loads in flight
                 f32x4 v[8];
@@ -946,9 +960,9 @@ __global__ __launch_bounds__(256) void finish_dx_k(const float* __restrict__ acc
         }
         if (first || i >= total) continue;
         x *= f;
-        T* o = dx + r * dim + c;
+        T* o = static_cast<T*>(p.out) + r * p.dim + c;
         for (int e = 0; e < 4; ++e)
-            if (c + e < dim) o[e] = (T)x[e];
+            if (c + e < p.dim) o[e] = (T)(p.add ? (float)o[e] + x[e] : x[e]);
     }
 }
 
@@ -962,7 +976,7 @@ struct Plan {
     long long xp, wp, xh, wh, x_power, w_power;
     bool kept;
     // bytes from the workspace's start
-    long long part, tl, row_loss, acc, g, bytes, state_bytes;
+    long long part, tl, row_loss, acc, g, dw, bytes, state_bytes;
     long long piece;                    // words of a piece of the vocabulary
     int acc_tile, splits, acc_ld;       // of the product that dX is
 };
@@ -996,6 +1010,16 @@ bool short_rows(int k) { return k <= 320; }
 // dX, whose words are split until the card is full (4096 x 1024, 64 large tiles: 234 us large, 311 small; 1999 x 520, 24 of them:
 // 105 and 92)
 bool big_dx_tiles(long long rows, long long dim) { return (long long)cdiv(rows, 256) * cdiv(dim, 256) >= 48; }
+
+// dW of few words and columns: the rows are split until the card is full, down to eight stages each (8192 rows, 2000 words of 256
+// values, fp32: 64 us with the launch that joins them, in one part 400; 4096 rows, 20000 words of 128: 204 and 291).  Two parts are
+// not worth that launch (bf16, 4096 rows, 10000 words of 320: 47 and 45).
+int dw_splits(long long words, int dim, long long rows, int products) {
+    if (big_tiles(words, dim, DW_RATE)) return 1;
+    const long long tiles = (long long)cdiv(words, 128) * cdiv(dim, 128), stages = rows / BK * products;
+    const long long splits = std::min(small_slots / tiles, stages / 8);
+    return splits < 3 ? 1 : (int)splits;
+}
 
 Plan plan(const s2ag_lce_args* a, bool backward) {
     Plan p{};
@@ -1046,6 +1070,10 @@ Plan plan(const s2ag_lce_args* a, bool backward) {
         // (what fills the card with splits is no more than its tiles hold)
         p.acc = take(dx ? 4 * (p.np * p.acc_ld + (long long)SLOTS * 256 * 256) : 0);
         p.g = take(2 * p.planes * p.np * p.piece);
+        // (splits that fill the card are no more than its tiles hold; the last piece may be split where the others are not)
+        const long long last = a->vocab - (p.vp - 1) / p.piece * p.piece;
+        const bool split = dw_splits(last < p.piece ? last : p.piece, a->dim, p.np, a->bf16 ? 1 : 6) > 1;
+        p.dw = take(a->dw && split ? 4LL * small_slots * 128 * 128 : 0);
     }
     p.bytes = at;
     return p;
@@ -1150,6 +1178,14 @@ int select_and_pack(const s2ag_lce_args* a, const Plan& p, const Select& s, hipS
     return pack(a, p, s, x, w, st);
 }
 
+int finish(const s2ag_lce_args* a, Finish& e, hipStream_t st) {
+    e.dim = a->dim;
+    const dim3 grid(grid_of(e.rows * ((a->dim + 3) / 4) * 4));
+    if (a->bf16) hipLaunchKernelGGL(finish_k<bf16_t>, grid, dim3(256), 0, st, e);
+    else hipLaunchKernelGGL(finish_k<float>, grid, dim3(256), 0, st, e);
+    S2AG_LAUNCH_CHECK();
+    return 0;
+}
 bool ready(const s2ag_lce_args* a, const Plan& p) {
     return a->x && a->w && a->target && a->state && a->workspace && a->workspace_bytes >= p.bytes && aligned16(a->workspace) && aligned16(a->state);
 }
@@ -1258,7 +1294,28 @@ extern "C" int s2ag_lce_bwd(const s2ag_lce_args* a, void* stream) {
             d.q_cols = p.kp;
             d.k_count = s.count;
             d.fp32 = !a->bf16;
-            d.out = a->bf16 ? (void*)(static_cast<bf16_t*>(a->dw) + v0 * a->dim) : (void*)(static_cast<float*>(a->dw) + v0 * a->dim);
+            void* dw = a->bf16 ? (void*)(static_cast<bf16_t*>(a->dw) + v0 * a->dim) : (void*)(static_cast<float*>(a->dw) + v0 * a->dim);
+            d.splits = dw_splits(words, a->dim, p.np, a->bf16 ? 1 : 6);
+            if (d.splits > 1) {
+                Finish e{};
+                e.most = d.splits;
+                d.out = ws + p.dw;
+                d.out_ld = p.acc_ld;
+                if (int rc = launch<STORE>(d, false, words, a->dim, st)) return rc;
+                e.acc = reinterpret_cast<const float*>(ws + p.dw);
+                e.ld = p.acc_ld;
+                e.tile = 128;
+                e.tiles_q = cdiv(a->dim, 128);
+                e.slots = small_slots;
+                e.scale = each ? nullptr : a->grad_out;
+                e.mean = !each && mean ? s.count : nullptr;
+                e.rows = words;
+                e.add = a->dw_accumulate;
+                e.out = dw;
+                if (int rc = finish(a, e, st)) return rc;
+                continue;
+            }
+            d.out = dw;
             d.out_ld = a->dim;
             d.out_bf16 = a->bf16;
             d.add = a->dw_accumulate;
@@ -1268,14 +1325,20 @@ extern "C" int s2ag_lce_bwd(const s2ag_lce_args* a, void* stream) {
         }
     }
     if (a->dx && a->rows) {
-        const unsigned gx = grid_of(a->rows * ((a->dim + 3) / 4) * 4);
-        if (a->bf16)
-            hipLaunchKernelGGL(finish_dx_k<bf16_t>, dim3(gx), dim3(256), 0, st, acc, (long long)p.acc_ld, p.acc_tile, cdiv(a->dim, p.acc_tile), p.splits, p.acc_tile == 256 ? SLOTS : small_slots, s,
-                               each ? nullptr : a->grad_out, (int)mean, a->rows, a->dim, static_cast<bf16_t*>(a->dx));
-        else
-            hipLaunchKernelGGL(finish_dx_k<float>, dim3(gx), dim3(256), 0, st, acc, (long long)p.acc_ld, p.acc_tile, cdiv(a->dim, p.acc_tile), p.splits, p.acc_tile == 256 ? SLOTS : small_slots, s,
-                               each ? nullptr : a->grad_out, (int)mean, a->rows, a->dim, static_cast<float*>(a->dx));
-        S2AG_LAUNCH_CHECK();
+        Finish e{};
+        e.acc = acc;
+        e.ld = p.acc_ld;
+        e.tile = p.acc_tile;
+        e.tiles_q = cdiv(a->dim, p.acc_tile);
+        e.most = p.splits;
+        e.slots = p.acc_tile == 256 ? SLOTS : small_slots;
+        e.count = s.count;
+        e.inv = s.inv;
+        e.scale = each ? nullptr : a->grad_out;
+        e.mean = !each && mean ? s.count : nullptr;
+        e.rows = a->rows;
+        e.out = a->dx;
+        if (int rc = finish(a, e, st)) return rc;
     }
     return 0;
 }

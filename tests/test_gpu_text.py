@@ -461,6 +461,27 @@ def test_linear_cross_entropy_gradient_against_differences(S):
     assert abs(slope - got) < 1e-5 * (float((gx.cpu().double() * ux).abs().sum() + (gw.cpu().double() * uw).abs().sum())) + 1e-6
 
 
+@pytest.mark.parametrize('dtype', list(DTYPES))
+@pytest.mark.parametrize('ignored', [0.0, 0.95, 1.0])
+@pytest.mark.parametrize('reduction', ['mean', 'none'])
+def test_linear_cross_entropy_many_rows_few_words(S, reduction, ignored, dtype):
+    """The weight's gradient in parts of the rows, more parts than rows that count among them."""
+    x, w, t, g = lce_case(1100, 70, 130, dtype, ignored)
+    lce_check(S, x, w, t, g, reduction)
+
+
+def test_linear_cross_entropy_many_rows_few_words_in_the_arena(S):
+    x, w, t, g = lce_case(1500, 36, 150, 'fp32', 0.3)
+    p, xg = torch.nn.Parameter(w.cuda()), x.cuda()
+    arena = S['optim'].ParamArena([p])
+    start = torch.randn(arena.numel, generator=g)
+    arena.grad.copy_(start.cuda())
+    _, _, (dw, dwb) = lce_reference(x, w, t, torch.tensor(1.0), 'mean')
+    S['ops'].linear_cross_entropy(xg, p, t.cuda()).backward()
+    before = start[:w.numel()].view_as(w).double()
+    within(p.grad, before + dw, dwb + U * (before.abs() + dw.abs() + dwb) * 1.01)
+
+
 def test_linear_cross_entropy_adds_to_the_arena(S):
     x, w, t, g = lce_case(33, 20, 90, 'fp32', 0.3)
     p = torch.nn.Parameter(w.cuda())
