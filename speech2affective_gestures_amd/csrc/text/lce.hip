@@ -262,10 +262,12 @@ struct Product {
     int mean;
 };
 
-// Pairs of pieces, the smallest products first, two bits each: (0, 2) (1, 1) (2, 0) (0, 1) (1, 0) (0, 0) of three, (0, 1) (1, 0)
-// (0, 0) of two, (0, 0) of one.
-template <int PAIRS> __device__ __forceinline__ int piece_r(int pair) { return PAIRS == 1 ? 0 : ((PAIRS == 6 ? 0x124 : 0x04) >> (2 * pair)) & 3; }
-template <int PAIRS> __device__ __forceinline__ int piece_q(int pair) { return PAIRS == 1 ? 0 : ((PAIRS == 6 ? 0x046 : 0x01) >> (2 * pair)) & 3; }
+// Pairs of pieces, two bits each, every one with a piece of R or Q from the one before it, which is then not requested again (7
+// requests of 12, or 4 of 6): (0, 2) (0, 1) (1, 1) (1, 0) (0, 0) (2, 0) of three pieces, (0, 1) (0, 0) (1, 0) of two.  One bit to a
+// pair: R, or Q, is another piece than before.
+template <int PAIRS> struct Pairs {
+    static constexpr int r = PAIRS == 6 ? 0x850 : 0x10, q = PAIRS == 6 ? 0x016 : 0x01, r_new = PAIRS == 6 ? 0x35 : 0x5, q_new = PAIRS == 6 ? 0x0b : 0x3;
+};
 
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 #define S2AG_LDS_PTR(type, p) ((__attribute__((address_space(3))) type*)(p))
@@ -516,12 +518,14 @@ __global__ __launch_bounds__(64 * WR * WQ, BR == 256 ? 1 : 2) void product_k(Pro
 
     // the stage that is requested next: its tile, pair of pieces and place along k; behind the last one the descriptors are
     // empty, so that the loop has no branch
+    constexpr bool REUSE = pairs > 1;
     int next = first - step, pair = 0, kk = 0, left = 0;
+    int r_new = 1, q_new = 1, r_to_buf = 1, q_to_buf = 1, r_last = 1, q_last = 1;          // (REUSE)
     long long r0_next = 0, c0_next = 0;
-    u32x4 rr, qr;
+    u32x4 rr, qr, r_base, q_base;
     // an operand's part of that stage: from row x of R or Q, or from its column x on
-    auto descriptor = [&](const Operand& o, int piece, bool down, long long x, long long rows, int tile, long long deep, int cols) {
-        const bf16_t* at = o.p + piece * o.plane;
+    auto descriptor = [&](const Operand& o, bool down, long long x, long long rows, int tile, long long deep, int cols) {
+        const bf16_t* at = o.p;
         long long bytes;
         if (down) {
             const long long k0 = (long long)kk * BK, n = deep - k0 < BK ? deep - k0 : BK;
@@ -537,8 +541,8 @@ __global__ __launch_bounds__(64 * WR * WQ, BR == 256 ? 1 : 2) void product_k(Pro
     int whole = 0;                                               // stages from here on that no end of a column cuts
     const unsigned long long r_step = 2ULL * BK * p.r.ld, q_step = 2ULL * BK * p.q.ld;
     auto descriptors = [&]() {
-        rr = descriptor(p.r, piece_r<pairs>(pair), RK, r0_next, p.r_rows, BR, p.r_deep, p.r_cols);
-        qr = descriptor(p.q, piece_q<pairs>(pair), QK, c0_next, p.q_rows, BQ, p.q_deep, p.q_cols);
+        rr = descriptor(p.r, RK, r0_next, p.r_rows, BR, p.r_deep, p.r_cols);
+        qr = descriptor(p.q, QK, c0_next, p.q_rows, BQ, p.q_deep, p.q_cols);
         if (QK) whole = (int)((RK && p.r_deep < p.q_deep ? p.r_deep : p.q_deep) / BK) - kk;
     };
     auto move = [](u32x4& d, unsigned long long bytes) {
@@ -546,41 +550,77 @@ __global__ __launch_bounds__(64 * WR * WQ, BR == 256 ? 1 : 2) void product_k(Pro
         d[0] = (unsigned)at;
         d[1] = (unsigned)(at >> 32);
     };
+    // Of the pair's pieces what is in LDS stays there: its requests get an empty descriptor, so that there are always as many of
+    // them to wait for, and put zeros where nothing lies that is still read.
+    auto aim = [&](bool all) {
+        r_new = all ? 1 : (Pairs<pairs>::r_new >> pair) & 1;
+        q_new = all ? 1 : (Pairs<pairs>::q_new >> pair) & 1;
+        rr = r_base;
+        qr = q_base;
+        move(rr, 2ULL * p.r.plane * ((Pairs<pairs>::r >> (2 * pair)) & 3));
+        move(qr, 2ULL * p.q.plane * ((Pairs<pairs>::q >> (2 * pair)) & 3));
+        if (!r_new) rr[2] = 0;
+        if (!q_new) qr[2] = 0;
+        r_to_buf = r_last ^ 1;
+        q_to_buf = q_last ^ 1;
+        r_last ^= r_new;
+        q_last ^= q_new;
+    };
     auto next_tile = [&]() {
         left = 0;
         for (next += step; next < last; next += step) {
             const Place t = place(next);
             left = t.it1 - t.it0;
             if (left <= 0) continue;                             // (no stage: nothing to request)
-            pair = __builtin_amdgcn_readfirstlane(t.it0 / ts.kt);
-            kk = t.it0 - pair * ts.kt;
+            kk = REUSE ? __builtin_amdgcn_readfirstlane(t.it0 / pairs) : t.it0;
+            pair = t.it0 - kk * pairs;
             r0_next = t.r0;
             c0_next = t.c0;
             break;
         }
         descriptors();
+        if constexpr (REUSE) {
+            r_base = rr;
+            q_base = qr;
+            aim(true);
+        }
+    };
+    auto next_k = [&]() {
+        ++kk;
+        if (QK) {                                                // down the columns: few scalar instructions, the matrix unit waits for them
+            if constexpr (REUSE) {
+                rr = r_base;
+                qr = q_base;
+            }
+            if (--whole > 0) {
+                if (RK) move(rr, r_step);
+                move(qr, q_step);
+            } else {
+                descriptors();
+            }
+            if constexpr (REUSE) {
+                r_base = rr;
+                q_base = qr;
+            }
+        }
     };
     auto advance = [&]() {
         if (--left <= 0) {
             next_tile();
-        } else {
-            if (++kk == ts.kt) {
-                kk = 0;
-                ++pair;
-                descriptors();
-            } else if (QK) {                                     // down the columns: few scalar instructions, the matrix unit waits for them
-                if (--whole > 0) {
-                    if (RK) move(rr, r_step);
-                    move(qr, q_step);
-                } else {
-                    descriptors();
-                }
+        } else if constexpr (REUSE) {
+            if (++pair == pairs) {
+                pair = 0;
+                next_k();
             }
+            aim(false);
+        } else {
+            next_k();
         }
     };
     // requests [from, from + n) of the LR + LQ of a stage
     auto issue = [&](int buf, int from, int n) {
-        const LdsPtr r_to = r_tiles + buf * (BR * BK) + wave * 512, q_to = q_tiles + buf * (BQ * BK) + wave * 512;
+        const LdsPtr r_to = r_tiles + (REUSE ? r_to_buf : buf) * (BR * BK) + wave * 512;
+        const LdsPtr q_to = q_tiles + (REUSE ? q_to_buf : buf) * (BQ * BK) + wave * 512;
         const int off = kk * (BK * 2);                           // (down the columns the descriptor moves)
 #pragma unroll
         for (int i = from; i < from + n; ++i) {
@@ -603,7 +643,7 @@ __global__ __launch_bounds__(64 * WR * WQ, BR == 256 ? 1 : 2) void product_k(Pro
     for (int n = 0; n < RN; ++n) r_place[n] = fragment_place<BR, RK>(r_tiles, wr * TR, n, fl, fk);
 #pragma unroll
     for (int n = 0; n < QN; ++n) q_place[n] = fragment_place<BQ, QK>(q_tiles, wq * TQ, n, fl, fk);
-    int r_other = BR * BK, q_other = BQ * BK;
+    int r_other = BR * BK, q_other = BQ * BK, r_go = 0, q_go = 0;
     auto read_q = [&](bf16x8 (&a)[QI], int ks, int i) {
         if constexpr (QK) a[i] = fragment<BQ, QK>(q_place[i] + ks * 32 * BQ);
         else a[i] = fragment<BQ, QK>(q_place[ks] + i * 16 * BK);
@@ -637,9 +677,9 @@ __global__ __launch_bounds__(64 * WR * WQ, BR == 256 ? 1 : 2) void product_k(Pro
             const int u = m / PER;
             if (ks == 0) {                                       // (the first reads of the other stage)
                 if (RK ? u < RI : u == 0)
-                    for (int n = RK ? u : 0; n < (RK ? u + 1 : RN); ++n) r_place[n] += r_other;
+                    for (int n = RK ? u : 0; n < (RK ? u + 1 : RN); ++n) r_place[n] += REUSE ? r_go : r_other;
                 if (QK ? u >= RI : u == RI)
-                    for (int n = QK ? u - RI : 0; n < (QK ? u - RI + 1 : QN); ++n) q_place[n] += q_other;
+                    for (int n = QK ? u - RI : 0; n < (QK ? u - RI + 1 : QN); ++n) q_place[n] += REUSE ? q_go : q_other;
             }
             if (u < RI) read_r(b, ks, u);
             else read_q(a, ks, u - RI);
@@ -667,6 +707,10 @@ __global__ __launch_bounds__(64 * WR * WQ, BR == 256 ? 1 : 2) void product_k(Pro
             for (int j = 0; j < RI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         settle();
         for (int n = t.it0; n < t.it1; ++n) {
+            if constexpr (REUSE) {                               // to the next stage's pieces, if they are others
+                r_go = r_new ? r_other : 0;
+                q_go = q_new ? q_other : 0;
+            }
             each<0, M, 1>([&](auto at_m) {
                 constexpr int m = decltype(at_m)::value;
                 if constexpr (m == (M > 16 ? EARLY : 0)) advance();          // (scalar work, where little or nothing waits for it)
@@ -701,8 +745,13 @@ __global__ __launch_bounds__(64 * WR * WQ, BR == 256 ? 1 : 2) void product_k(Pro
                 __builtin_amdgcn_sched_barrier(0);
             });
             buf ^= 1;
-            r_other = -r_other;
-            q_other = -q_other;
+            if constexpr (REUSE) {
+                r_other = r_go ? -r_other : r_other;
+                q_other = q_go ? -q_other : q_other;
+            } else {
+                r_other = -r_other;
+                q_other = -q_other;
+            }
         }
         settle();
 
