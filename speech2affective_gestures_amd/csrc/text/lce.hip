@@ -25,7 +25,7 @@
 //
 // Measured, 7373 of 8192 rows counting, 131072 words of 2048 values, bf16: max and sum 3.0 ms (1320 TFLOP/s), G 3.3 (1190), dX 3.1
 // (1290), dW 2.9 (1360); a library product of 8192 cubed ran at 1280, of 16384 cubed at 1540.  136 rows, 20000 words of 300 values,
-// fp32: 21, 28, 30 and 28 us, packing 24, the joins and sums 16: there nothing fills the card, and launches and the ends of tiles
+// fp32: 22, 29, 30 and 28 us, packing 24, the joins and sums 16: there nothing fills the card, and launches and the ends of tiles
 // are most of it.
 #include "text_common.h"
 #include <algorithm>
@@ -1031,7 +1031,7 @@ struct Plan {
 };
 
 // Values of G in a piece of the vocabulary, 512 MB in bf16.  (Half as many: 8192 rows, 131072 words of 2048 values 13.0 against
-// 12.6 ms; 4352 rows, 85 % of them ignored, 20000 words of 300 values, fp32: 294 against 239 us, since pieces are made for all rows.)
+// 12.8 ms; fp32, 4352 rows, 85 % of them ignored, 20000 words of 300 values: 295 against 246 us, since pieces are made for all rows.)
 constexpr long long PIECE_VALUES = 1LL << 28;
 
 bool valid(const s2ag_lce_args* a) {
@@ -1049,19 +1049,20 @@ bool big_tiles(long long r, long long q, int percent) {
     const long long big = (long long)cdiv(r, 256) * cdiv(q, 256), small = (long long)cdiv(r, 128) * cdiv(q, 128);
     return (big + SLOTS - 1) / SLOTS * (2 * small_slots) * percent <= small * 100;
 }
-// (4096 rows and 32768 words of 1024 values: max and sum 283 us large, 326 small, G 301 and 332; dW 250 and 322, but of 640 values,
-// which large tiles pad to 768, 227 and 198)
+// (bf16, 4096 rows and 32768 words of 1024 values: max and sum 281 us large, 321 small, G 306 and 320; dW 250 and 312, but of 640
+// values, which large tiles pad to 768, 226 and 191)
 constexpr int LOGIT_RATE = 88, DW_RATE = 77;
 // Logits of short rows: a tile's end is long beside its products, and of two workgroups on a compute unit one multiplies while the
-// other ends (4096 rows, 320 wide: max and sum 131 us large, 133 small; 128 wide 94 and 85; fp32 320 wide 220 and 212, 1024 wide
-// 503 and 526).  G of fp32, three pieces of each value, takes small ones for every length (1024 wide: 688 and 607 us).
+// other ends (bf16, the same rows, 320 wide: max and sum 131 us large, 129 small; 128 wide 92 and 85; fp32, 20000 words, 320 wide 238
+// and 226, 1024 wide 551 and 568).  G of fp32, three pieces of each value, takes small ones for every length (320 wide: 330 and
+// 291 us, 1024 wide 639 and 622).
 bool short_rows(int k) { return k <= 320; }
-// dX, whose words are split until the card is full (4096 x 1024, 64 large tiles: 234 us large, 311 small; 1999 x 520, 24 of them:
-// 105 and 92)
+// dX, whose words are split until the card is full (bf16, 4096 x 1024, 64 large tiles: 244 us large, 310 small; 1999 x 520, 24 of
+// them: 148 and 139)
 bool big_dx_tiles(long long rows, long long dim) { return (long long)cdiv(rows, 256) * cdiv(dim, 256) >= 48; }
 
-// dW of few words and columns: the rows are split until the card is full, down to eight stages each (8192 rows, 2000 words of 256
-// values, fp32: 64 us with the launch that joins them, in one part 400; 4096 rows, 20000 words of 128: 204 and 291).  Two parts are
+// dW of few words and columns: the rows are split until the card is full, down to eight stages each (fp32, 8192 rows, 2000 words
+// of 256 values: 65 us with the launch that joins them, in one part 417; 4096 rows, 20000 words of 128: 165 and 280).  Two parts are
 // not worth that launch (bf16, 4096 rows, 10000 words of 320: 47 and 45).
 int dw_splits(long long words, int dim, long long rows, int products) {
     if (big_tiles(words, dim, DW_RATE)) return 1;
