@@ -30,8 +30,12 @@ _NOTHING = contextlib.nullcontext()
 
 def _on(t: Tensor):
     """Context in which ``t``'s device is the current one (nothing to do where it is: the usual case)."""
-    dev = t.device
-    return _NOTHING if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    dev = t.device                                                 # (torch.cuda.current_device asks first whether torch is set up)
+    return _NOTHING if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
+
+
+def _like(t: Tensor) -> Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)      # (half the time of torch.empty with a shape)
 
 
 def _stream(t: Tensor) -> int:
@@ -100,7 +104,7 @@ class _EmbeddingSorted(torch.autograd.Function):
             data = table.contiguous()
             n, (entries, dim) = ids.numel(), data.shape
             i32, bf16 = ids.dtype == torch.int32, data.dtype == torch.bfloat16
-            out = torch.empty(*ids.shape, dim, dtype=data.dtype, device=data.device)
+            out = data.new_empty(ids.shape + (dim,))
             L.check(lib.s2ag_emb_lookup(ids.data_ptr(), i32, data.data_ptr(), bf16, n, dim, entries, scale, out.data_ptr(), _stream(out)),
                     'emb_lookup')
         if grads and ctx.needs_input_grad[1]:
@@ -117,7 +121,7 @@ class _EmbeddingSorted(torch.autograd.Function):
         with _on(dy):
             dy, ld = _rows(dy)
             slot = _arena_slot(table)
-            dt = torch.empty(entries, dim, dtype=dy.dtype, device=dy.device) if slot is None else slot
+            dt = _like(table) if slot is None else slot
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dy.device)
             L.check(lib.s2ag_emb_grad(ids.data_ptr(), i32, dy.data_ptr(), ld, bf16, n, dim, entries, padding_idx, scale, dt.data_ptr(),
                                       slot is not None, ws.data_ptr(), ws_bytes, _stream(dy)), 'emb_grad')
@@ -190,15 +194,15 @@ class _LinearCrossEntropy(torch.autograd.Function):
         need_x, need_w = ctx.needs_input_grad[:2]
         with _on(x):
             slot = _arena_slot(leaf) if need_w else None
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+            dx = _like(x) if need_x else None
             dw = slot
             if need_w and slot is None:
-                dw = torch.empty(weight.shape, dtype=weight.dtype, device=x.device)
+                dw = _like(weight)
             if a.rows == 0:
                 if dw is not None and slot is None:
                     dw.zero_()
             else:
-                g = dloss.to(torch.float32).contiguous()
+                g = dloss.contiguous()                           # (fp32, as the loss is)
                 b = L.LceArgs.from_buffer_copy(a)                # (a graph that is kept runs backward again)
                 b.grad_out, b.dx, b.dw, b.dw_accumulate = g.data_ptr(), _p(dx), _p(dw), slot is not None
                 ws = _lce_workspace(lib, b, True, x.device)

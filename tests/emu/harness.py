@@ -148,6 +148,7 @@ def install():
     tc.current_device = lambda: 0
     tc.set_device = lambda d: None
     torch._C._cuda_getCurrentRawStream = lambda index: 0
+    torch._C._cuda_getDevice = lambda: 0
     tc.device = lambda d=None: contextlib.nullcontext()
     tc.synchronize = lambda *a, **k: None
     tc.current_stream = lambda *a, **k: cur
