@@ -14,6 +14,7 @@ from typing import Iterable, List, Optional, Sequence, Union
 import torch
 
 from . import _lib as L
+from .text import _on, _stream
 
 
 class ParamArena:
@@ -177,17 +178,17 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float 
     k = len(rows) // 4
     table = C.cast((C.c_longlong * max(len(rows), 1))(*rows), C.POINTER(L.ClipTensor))
     lib = L.load()
-    with torch.cuda.device(dev):
+    with _on(grads[0]):
         partials = torch.empty(lib.s2ag_clip_partials(table, k), dtype=torch.float64, device=dev)
         norm = torch.empty((), dtype=torch.float32, device=dev)
-        L.check(lib.s2ag_clip_grads(table, k, max_norm, int(inf), C.c_void_p(partials.data_ptr()), C.c_void_p(norm.data_ptr()),
-                                    C.c_void_p(torch.cuda.current_stream().cuda_stream)), 'clip_grads')
+        L.check(lib.s2ag_clip_grads(table, k, max_norm, inf, partials.data_ptr(), norm.data_ptr(), _stream(norm)), 'clip_grads')
     torch.autograd.graph.increment_version(results)                # written behind torch's back
     return norm
 
 
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
-    """``clip_grads`` in place over the ``.grad`` of the parameters that have one (torch.nn.utils.clip_grad_norm_'s call)."""
+    """``clip_grads`` in place over the ``.grad`` of the parameters that have one (torch.nn.utils.clip_grad_norm_'s call);
+    ValueError where none has one."""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
     return clip_grads([p.grad for p in parameters if p.grad is not None], max_norm, norm_type)
