@@ -5,6 +5,7 @@ arena, its gradient a view into a second one.  Consequences: ``zero_grad`` is on
 kernel launch per optimizer (s2ag_adam_step), and the data-parallel gradient exchange is a single RCCL
 all-reduce over the arena (parallel.py) instead of one collective per tensor.
 """
+import array
 import ctypes as C
 import itertools
 import math
@@ -150,7 +151,7 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float 
     dev = grads[0].device
     if not grads[0].is_cuda:
         raise RuntimeError('clip_grads: got a CPU tensor; the S2AG ops run on MI355X only and there is no CPU fallback')
-    if any(d != dev for d in map(_DEVICE, tensors)):
+    if len(set(map(torch.Tensor.get_device, tensors))) > 1:
         raise ValueError(f'clip_grads: tensors on {sorted(set(map(str, map(_DEVICE, tensors))))}')
     kinds = list(map(_CLIP_DTYPES.get, map(_DTYPE, tensors)))
     if None in kinds:
@@ -174,9 +175,9 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float 
     spans.sort()
     if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
         raise ValueError('clip_grads: two of the tensors share memory, or one that is listed twice has two outputs')
-    rows = list(itertools.chain.from_iterable(rows))
-    k = len(rows) // 4
-    table = C.cast((C.c_longlong * max(len(rows), 1))(*rows), C.POINTER(L.ClipTensor))
+    k = len(rows)
+    words = array.array('q', itertools.chain.from_iterable(rows))
+    table = (L.ClipTensor * k).from_buffer(words) if k else (L.ClipTensor * 1)()
     lib = L.load()
     with _on(grads[0]):
         partials = torch.empty(lib.s2ag_clip_partials(table, k), dtype=torch.float64, device=dev)
