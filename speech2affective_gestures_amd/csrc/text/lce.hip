@@ -238,7 +238,7 @@ struct Product {
     const int* k_count;                 // not null: k is this, rounded up to 64
     const int* r_count;                 // not null: rows of R that matter
     bool fp32;                          // operands in pieces
-    // STATS, GRADS of fp32: rows of R and Q are 2^power of what is multiplied
+    // STATS, GRADS of fp32: rows of R and Q times 2^power are what is multiplied
     const int *r_power, *q_power;
     int tiles_q;
     int splits, slots;                  // the most parts of k; workgroups that run at a time
