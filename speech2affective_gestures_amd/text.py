@@ -204,6 +204,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
             else:
                 g = dloss.contiguous()                           # (fp32, as the loss is)
                 b = L.LceArgs.from_buffer_copy(a)                # (a graph that is kept runs backward again)
+                # hooks on saved tensors and checkpoints hand back others than were saved, whose memory is gone
+                b.x, b.target, b.state = x.data_ptr(), t.data_ptr(), state.data_ptr()
                 b.grad_out, b.dx, b.dw, b.dw_accumulate = g.data_ptr(), _p(dx), _p(dw), slot is not None
                 ws = _lce_workspace(lib, b, True, x.device)
                 L.check(lib.s2ag_lce_bwd(b, _stream(ws)), 'lce_bwd')

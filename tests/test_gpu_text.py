@@ -836,3 +836,62 @@ def test_a_step_of_a_text_model(S):
         # Adam's first step: lr g / (|g| + eps), which moves by lr / eps of what g is off; the moments' bias corrections cancel
         want = start.double() - 1e-2 * r / (r.abs() + 1e-2)
         assert float((p.detach().cpu().double() - want).abs().max()) < 1e-2 / 1e-2 * err + 1e-6
+
+
+def _by_clones(run):
+    """Saved tensors as copies of themselves, the memory of what was saved given to others before the backward pass."""
+    held = []
+
+    def pack(t):
+        return t.detach().clone()
+
+    def unpack(t):
+        held.extend(torch.full((n,), 0x7f, dtype=torch.uint8, device=t.device) for n in sizes for _ in range(3))
+        return t.clone()
+    sizes = (64, 512, 1024, 4096, 16384, 65536, 262144)
+    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+        return run()
+
+
+def _on_the_host(run):
+    with torch.autograd.graph.save_on_cpu():
+        return run()
+
+
+def _by_checkpoint(run):
+    from torch.utils.checkpoint import checkpoint
+    return checkpoint(run, use_reentrant=False, preserve_rng_state=False)
+
+
+@pytest.mark.parametrize('dtype', list(DTYPES))
+@pytest.mark.parametrize('saving', [_by_clones, _on_the_host, _by_checkpoint])
+def test_text_operators_read_the_saved_tensors_that_they_are_given(S, saving, dtype):
+    """Hooks on saved tensors and checkpointing hand the backward pass other tensors than were saved: the same bits as without them."""
+    ops = S['ops']
+    for n, d, v in ((40, 24, 100), (130, 64, 300)):                # (64 columns: bf16 words are read where they lie)
+        x, w, t, g = lce_case(n, d, v, dtype, 0.2)
+        ids = ids_of('padded', n, v, g)
+        dy = torch.randn(n, d, generator=g).to(DTYPES[dtype]).cuda()
+        xg, wg, tg, ig = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True), t.cuda(), ids.cuda()
+        for run, leaves, grad in ((lambda: ops.linear_cross_entropy(xg, wg, tg), (xg, wg), None),
+                                  (lambda: ops.linear_cross_entropy(xg, wg, tg, reduction='none').sum(), (xg, wg), None),
+                                  (lambda: ops.embedding_sorted(ig, wg, scale=2.0), (wg,), dy)):
+            plain = run()
+            want = torch.autograd.grad(plain, leaves, grad)
+            other = saving(run)
+            got = torch.autograd.grad(other, leaves, grad)
+            assert torch.equal(other, plain)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_linear_cross_entropy_in_the_arena_under_a_checkpoint(S):
+    """The weight of a ParamArena, its gradient added there once though the forward pass runs twice."""
+    x, w, t, g = lce_case(40, 24, 100, 'fp32', 0.2)
+    grads = []
+    for saving in (lambda run: run(), _by_checkpoint):
+        xg, wg = x.cuda().requires_grad_(True), torch.nn.Parameter(w.cuda())
+        arena = S['optim'].ParamArena([wg])
+        arena.grad.fill_(0.5)
+        saving(lambda: S['ops'].linear_cross_entropy(xg, wg, t.cuda())).backward()
+        grads.append((xg.grad, wg.grad.clone()))
+    assert torch.equal(grads[0][0], grads[1][0]) and torch.equal(grads[0][1], grads[1][1])
