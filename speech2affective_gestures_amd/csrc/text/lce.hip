@@ -330,6 +330,12 @@ __device__ __forceinline__ float exp_of(float d) {
     return fmaf(e * 0.693147180559945f, rest, e);
 }
 
+// The factor of all rows.  Where none counts there is nothing that it enters: an infinite one leaves the zeros as they are.
+__device__ __forceinline__ float scale_of(const float* scale, int mean, int kept) {
+    if (kept == 0) return 1.f;
+    return mean ? *scale / (float)kept : *scale;
+}
+
 constexpr int GROUP = 8;                // row tiles that the columns pass by at a time
 
 // The tiles of a launch, in the order in which they are handed out; everything here is one for the workgroup.
@@ -469,7 +475,7 @@ __global__ __launch_bounds__(64 * WR * WQ, BR == 256 ? 1 : 2) void product_k(Pro
     // (read here: a load that is still out behind the end of a tile would be waited for in every stage of the next one)
     float f = 1.f;
     if constexpr (END == STORE) {
-        if (p.scale) f = p.mean ? *p.scale / (float)max(1, *p.k_count) : *p.scale;
+        if (p.scale) f = scale_of(p.scale, p.mean, *p.k_count);
         f = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(f)));
     }
 
@@ -967,8 +973,9 @@ struct Finish {
     long long ld;
     int tile, tiles_q, most, slots;     // of the product
     const int *count, *inv;             // packed rows and their places; null: every row is its own
-    const int* mean;                    // the number that `scale` is divided by, or null
-    const float* scale;                 // or null
+    const float* scale;                 // or null; over the number of rows that count with `mean`
+    int mean;
+    const int* kept;                    // that number
     long long rows;
     int dim, add;
     void* out;
@@ -976,8 +983,7 @@ struct Finish {
 template <typename T>
 __global__ __launch_bounds__(256) void finish_k(Finish p) {
     __shared__ f32x4 sm[4][64];
-    float f = p.scale ? *p.scale : 1.f;
-    if (p.mean) f /= (float)max(1, *p.mean);
+    const float f = p.scale ? scale_of(p.scale, p.mean, *p.kept) : 1.f;
     const int groups = (p.dim + 3) / 4, tiles_r = ((p.count ? *p.count : (int)p.rows) + p.tile - 1) / p.tile;
     const int splits = splits_of(tiles_r * p.tiles_q, p.most, p.slots);
     const long long split = (long long)tiles_r * p.tile * p.ld;
@@ -1008,7 +1014,7 @@ __global__ __launch_bounds__(256) void finish_k(Finish p) {
             __syncthreads();
         }
         if (first || i >= total) continue;
-        x *= f;
+        if (at >= 0) x *= f;                                     // (an infinite factor does not reach a row that was ignored)
         T* o = static_cast<T*>(p.out) + r * p.dim + c;
         for (int e = 0; e < 4; ++e)
             if (c + e < p.dim) o[e] = (T)(p.add ? (float)o[e] + x[e] : x[e]);
@@ -1358,7 +1364,8 @@ extern "C" int s2ag_lce_bwd(const s2ag_lce_args* a, void* stream) {
                 e.tiles_q = cdiv(a->dim, 128);
                 e.slots = small_slots;
                 e.scale = each ? nullptr : a->grad_out;
-                e.mean = !each && mean ? s.count : nullptr;
+                e.mean = mean;
+                e.kept = s.count;
                 e.rows = words;
                 e.add = a->dw_accumulate;
                 e.out = dw;
@@ -1385,7 +1392,8 @@ extern "C" int s2ag_lce_bwd(const s2ag_lce_args* a, void* stream) {
         e.count = s.count;
         e.inv = s.inv;
         e.scale = each ? nullptr : a->grad_out;
-        e.mean = !each && mean ? s.count : nullptr;
+        e.mean = mean;
+        e.kept = s.count;
         e.rows = a->rows;
         e.out = a->dx;
         if (int rc = finish(a, e, st)) return rc;

@@ -895,3 +895,24 @@ def test_linear_cross_entropy_in_the_arena_under_a_checkpoint(S):
         saving(lambda: S['ops'].linear_cross_entropy(xg, wg, t.cuda())).backward()
         grads.append((xg.grad, wg.grad.clone()))
     assert torch.equal(grads[0][0], grads[1][0]) and torch.equal(grads[0][1], grads[1][1])
+
+
+@pytest.mark.parametrize('dtype', list(DTYPES))
+@pytest.mark.parametrize('factor', [float('inf'), float('nan')])
+def test_linear_cross_entropy_ignored_rows_stay_out_of_an_infinite_factor(S, factor, dtype):
+    """A loss scale that has overflowed: what the factor does not enter is zero, in every way that the results are written."""
+    sizes = [(40, 24, 100), (3000, 16, 130)]                        # dW at once, and in parts of the rows that a launch joins
+    for n, d, v in sizes[:1] if EMU and dtype == 'bf16' else sizes:
+        x, w, t, g = lce_case(n, d, v, dtype, 0.3)
+        none = torch.full_like(t, IGNORE)
+        for reduction in ('mean', 'sum', 'none'):
+            for target, ignored in ((t, t == IGNORE), (none, none == IGNORE)):
+                xg, wg = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+                loss = S['ops'].linear_cross_entropy(xg, wg, target.cuda(), reduction=reduction)
+                loss.backward(torch.full_like(loss, factor))
+                dx = xg.grad.cpu()
+                assert float(dx[ignored].abs().max()) == 0.0
+                if not ignored.all():
+                    assert not torch.isfinite(dx[~ignored]).any() and not torch.isfinite(wg.grad).any()
+                else:
+                    assert float(wg.grad.abs().max()) == 0.0
