@@ -847,7 +847,7 @@ __global__ __launch_bounds__(64 * WR * WQ, BR == 256 ? 1 : 2) void product_k(Pro
 #pragma unroll
                 for (int j = 0; j < RI; ++j) {
                     const long long row = wr0 + j * 16 + fl;
-                    const bool in = row < live;                  // (rows behind are zeros: a factor of 0 keeps them so)
+                    const bool in = row < live;
                     lse[j] = in ? p.lse[row] : 0.f;
                     fac[j] = in ? (p.grad_out ? p.grad_out[p.rowmap[row]] : 1.f) : 0.f;
                     tgt[j] = in ? p.tgt[row] : -1;
@@ -872,6 +872,11 @@ __global__ __launch_bounds__(64 * WR * WQ, BR == 256 ? 1 : 2) void product_k(Pro
                         }
 #pragma unroll
                         for (int i = 0; i < QI * 4; ++i) g[j][i] *= fac[jj + j];
+                        if (t.r0 + BR > live) {                  // rows behind are zeros, which dW's products pass by (0 times a word's infinity is none)
+                            const bool in = wr0 + (jj + j) * 16 + fl < live;
+#pragma unroll
+                            for (int i = 0; i < QI * 4; ++i) g[j][i] = in ? g[j][i] : 0.f;
+                        }
                         __builtin_amdgcn_sched_barrier(0);
                     }
                     each<0, pieces, 1>([&](auto at_piece) {

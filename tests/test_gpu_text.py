@@ -916,3 +916,24 @@ def test_linear_cross_entropy_ignored_rows_stay_out_of_an_infinite_factor(S, fac
                     assert not torch.isfinite(dx[~ignored]).any() and not torch.isfinite(wg.grad).any()
                 else:
                     assert float(wg.grad.abs().max()) == 0.0
+
+
+@pytest.mark.parametrize('reduction', ['mean', 'none'])
+def test_linear_cross_entropy_words_ruled_out_by_infinities(S, reduction):
+    """bf16 words whose every logit is -infinity: the loss and the other words' gradient as if they were not there, a gradient of zero for
+    them (fp32 gives NaN, as is documented).  The input's gradient holds 0 times infinity: NaN."""
+    for n in (40, 64, 200):
+        x, w, t, g = lce_case(n, 24, 300, 'bf16', 0.2)
+        x = x.abs() + 0.125
+        t = torch.where(t == IGNORE, t, t % 250)
+        low = w.clone()
+        low[250:] = -float('inf')
+        gout = torch.randn(t.shape if reduction == 'none' else (), generator=g)
+        (l, lb), _, (dw, dwb) = lce_reference(x, w[:250], t, gout, reduction)
+        xg, wg = x.cuda().requires_grad_(True), low.cuda().requires_grad_(True)
+        loss = S['ops'].linear_cross_entropy(xg, wg, t.cuda(), reduction=reduction)
+        within(loss, l, lb)
+        loss.backward(gout.cuda())
+        within(wg.grad[:250], dw, dwb)
+        assert float(wg.grad[250:].abs().max()) == 0.0
+        assert torch.isnan(xg.grad.cpu()[t != IGNORE]).all() and float(xg.grad.cpu()[t == IGNORE].abs().max()) == 0.0
