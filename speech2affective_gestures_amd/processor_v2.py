@@ -12,10 +12,13 @@ What is MI355X-first here (DESIGN.md has the full story):
   * losses stay on the device; one 32-byte read-back per step replaces the reference's 5-7 ``.item()`` syncs.
 Rendering, FGD evaluation and the LMDB/npz data pipeline of the reference are outside this path.
 """
+import contextlib
+import gc
 import math
 import os
 import re
 import time
+import weakref
 from os.path import join as jn
 
 import numpy as np
@@ -88,6 +91,21 @@ PASSES_PER_STEP = 7      # forward passes (= noise snapshots) of one GAN step, i
                          # D(fake), tri-modal baseline, G(main), D(gen), G(rand)
 
 
+@contextlib.contextmanager
+def _capture(graph, **kw):
+    """torch.cuda.graph without Python's cyclic collector, which runs on whichever thread allocates next: an object that it
+    frees meanwhile (another graph, whose end waits for the device and gives its memory pool back) would end inside this capture.
+    'thread_local': the batch feeder's thread allocates / records events on its own stream meanwhile."""
+    on = gc.isenabled()
+    gc.disable()
+    try:
+        with torch.cuda.graph(graph, capture_error_mode='thread_local', **kw):
+            yield
+    finally:
+        if on:
+            gc.enable()
+
+
 class _GraphSegments:
     """Capture ``fns`` as consecutive HIP graphs sharing one memory pool; ``between[i]`` runs eagerly after
     segment i (the RCCL all-reduces).  Static shapes; inputs are copied into the buffers captured."""
@@ -107,8 +125,7 @@ class _GraphSegments:
             self.before()              # host-side state the captured functions branch on (GradExchange.precheck)
         for i, fn in enumerate(fns):
             g = torch.cuda.CUDAGraph()
-            # 'thread_local': the batch feeder's thread allocates / records events on its own stream meanwhile
-            with torch.cuda.graph(g, pool=pool, capture_error_mode='thread_local'):
+            with _capture(g, pool=pool):
                 fn()
             self.graphs.append(g)      # nothing executes during capture, so no collective here
 
@@ -521,7 +538,7 @@ class Processor(object):
                     if st['graph'] is None:
                         torch.cuda.synchronize()
                         gr = torch.cuda.CUDAGraph()
-                        with torch.cuda.graph(gr, capture_error_mode='thread_local'):     # nothing executes during capture
+                        with _capture(gr):                  # nothing executes during capture
                             window_step()
                         st['graph'] = gr
                     st['graph'].replay()
@@ -947,30 +964,34 @@ class Processor(object):
         use_gan = self._use_gan()
         ex = self._exchange()
 
+        # the segments know the trainer without keeping it: it and its graphs end where its last reference goes, not in a cycle that
+        # the collector finds at some time on some thread
+        me = weakref.proxy(self)
+
         def seg_dis():
             ops.begin_step()
-            self.s2ag_generator.share_passes = self._gen_passes() if self.share_encoders else None
-            out['pre'] = self._make_pre_seq(st['target'])
-            out['dis'] = self._dis_phase(st['text'], st['mfcc'] if self.use_mfcc else st['audio'], st['target'],
+            me.s2ag_generator.share_passes = me._gen_passes() if me.share_encoders else None
+            out['pre'] = me._make_pre_seq(st['target'])
+            out['dis'] = me._dis_phase(st['text'], st['mfcc'] if me.use_mfcc else st['audio'], st['target'],
                                          st['vid'], out['pre'], True, in_audio=st['audio'],
                                          cut=ex is not None) if use_gan else None
 
         def seg_gen():
             if use_gan:
-                self.s2ag_dis_optimizer.step(self.dp.grad_scale)
-            out['comps'] = self._gen_phase(st['text'], st['audio'], st['mfcc'], st['target'], st['vid'], out['pre'],
+                me.s2ag_dis_optimizer.step(me.dp.grad_scale)
+            out['comps'] = me._gen_phase(st['text'], st['audio'], st['mfcc'], st['target'], st['vid'], out['pre'],
                                            True, cut=ex is not None)
 
         def seg_gen_rest():
-            self._gen_backward_rest(st['text'], ex)
+            me._gen_backward_rest(st['text'], ex)
 
         def seg_opt():
             if ex is not None:
                 ex.merge_rows()
-            self.s2ag_gen_optimizer.step(self.dp.grad_scale)
+            me.s2ag_gen_optimizer.step(me.dp.grad_scale)
             ops.stamp('step end (G-Adam done)')
-            self.s2ag_generator.share_passes = None        # sharing is scoped to the step (see forward_pass_s2ag)
-            self.s2ag_generator._shared = None
+            me.s2ag_generator.share_passes = None        # sharing is scoped to the step (see forward_pass_s2ag)
+            me.s2ag_generator._shared = None
 
         # Single process: three segments, nothing between them.  Data parallel: the collectives run from the host
         # between the segments -- the graphs never contain RCCL nodes -- and bucket A's all-reduce runs BESIDE the
@@ -980,12 +1001,12 @@ class Processor(object):
         else:
             fns = [seg_dis, seg_gen, seg_gen_rest, seg_opt]
             def after_dis():
-                self.dp.all_reduce_grads(self.dis_arena)
-                self._sync_error_flag()              # before D's Adam (first kernel of the next segment)
+                me.dp.all_reduce_grads(me.dis_arena)
+                me._sync_error_flag()              # before D's Adam (first kernel of the next segment)
 
             def after_gen_rest():
                 ex.exchange_rest()
-                self._sync_error_flag()              # before G's Adam
+                me._sync_error_flag()              # before G's Adam
             between = [after_dis if use_gan else None, ex.launch_a, after_gen_rest, None]
         segs = _GraphSegments(fns, between, before=(lambda: ex.precheck(st['text'])) if ex is not None else None)
         self._graphed = dict(st=st, out=out, segs=segs, key=self._graph_key(in_text, in_audio, in_mfcc, target_poses))
