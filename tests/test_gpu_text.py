@@ -937,3 +937,71 @@ def test_linear_cross_entropy_words_ruled_out_by_infinities(S, reduction):
         within(wg.grad[:250], dw, dwb)
         assert float(wg.grad[250:].abs().max()) == 0.0
         assert torch.isnan(xg.grad.cpu()[t != IGNORE]).all() and float(xg.grad.cpu()[t == IGNORE].abs().max()) == 0.0
+
+
+# ---- fp32's precision over whole results ---------------------------------------------------------------------------------------
+# The bounds above are worst cases, element by element, which a missing product of two pieces can hide under where sums are long.  Over
+# a whole result errors are independent and its norm is what they add up to: a rounding is 0.58 U of its value at most (rms, half a
+# step uniformly over a step, a value at the low end of its binade), one for each of the contraction's `steps` instructions; 8 U for
+# G's own (its logarithm and exponent) and what the pieces leave.  A pair of pieces that is left out is 1.5e-6 to 3e-6 of the result.
+def norm_bound(steps):
+    return U * (8 + math.sqrt(steps))
+
+
+def pieces_of(v, count, kind):
+    out, rest = [], v.float()
+    for _ in range(count):
+        out.append(rest.to(kind).float())
+        rest = rest - out[-1]
+    return [p.double() for p in out]
+
+
+NORM_CASES = [(130, 300, 1000), (300, 36, 500), (129, 64, 257), (4100, 800, 700), (1000, 520, 65536), (1500, 700, 20000)]
+
+
+def norm_error(got, ref):
+    return float((got.detach().cpu().double() - ref).norm() / ref.norm())
+
+
+@pytest.mark.parametrize('case', [pytest.param(c, marks=pytest.mark.skipif(EMU and c[0] * c[2] > 1e6, reason='minutes on the device model'))
+                                  for c in NORM_CASES])
+def test_linear_cross_entropy_keeps_the_precision_of_fp32(S, case):
+    n, d, v = case
+    x, w, t, g = lce_case(n, d, v, 'fp32', 0.0)
+    gout = torch.randn(n, generator=g)                              # (a factor of 1 would be one piece)
+    x64, w64 = x.double(), w.double()
+    z = x64 @ w64.t()
+    lse = torch.logsumexp(z, 1)
+    loss = lse - z[torch.arange(n), t]
+    z.sub_(lse[:, None]).exp_()
+    z[torch.arange(n), t] -= 1.0
+    z.mul_(gout.double()[:, None])
+    xg, wg = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    out = S['ops'].linear_cross_entropy(xg, wg, t.cuda(), reduction='none')
+    out.backward(gout.cuda())
+    # a loss is a difference of numbers up to 16: two roundings of half of 2^-20, of a loss of 5 and more on average
+    assert norm_error(out, loss) < 2.0 ** -20 / 5
+    checked = 0
+    for got, a, b, long in ((xg.grad, z, w64, v), (wg.grad, z.t(), x64, n)):
+        bound = norm_bound(6 * -(-long // 32))
+        if bound < 1.5e-6:                                          # (longer ones would not notice a pair)
+            checked += 1
+            assert norm_error(got, a @ b) < bound
+    assert checked
+
+
+def test_the_bound_on_fp32s_precision_notices_a_missing_pair_of_pieces():
+    """The oracle with one product of two pieces left out, in 64 bits otherwise: beyond the bound of every contraction that is held to it."""
+    n, d, v = 130, 300, 1000
+    x, w, t, g = lce_case(n, d, v, 'fp32', 0.0)
+    G = torch.softmax(x.double() @ w.double().t(), 1)
+    G[torch.arange(n), t] -= 1.0
+    G = (G * torch.randn(n, generator=g).double()[:, None]).float()
+    for a, b in ((G, w), (G.t().contiguous(), x)):
+        A, B = pieces_of(a, 3, torch.bfloat16), pieces_of(b, 3, torch.bfloat16)
+        ref = a.double() @ b.double()
+        pairs = [(0, 2), (0, 1), (1, 1), (1, 0), (0, 0), (2, 0)]
+        full = sum(A[i] @ B[j] for i, j in pairs)
+        assert norm_error(full, ref) < 2 * U
+        for i, j in pairs:
+            assert norm_error(full - A[i] @ B[j], ref) > 1.5e-6, (i, j)
