@@ -89,7 +89,34 @@ def _arena_slot(p: Tensor) -> Optional[Tensor]:
     if getattr(p, '_s2ag_arena', None) is None:
         return None
     from .ops import _grad_slot
-    return _grad_slot(p)
+    slot = _grad_slot(p)
+    if slot is not None:
+        turn = p.__dict__.setdefault('_s2ag_turn', _Turn())
+        if turn.handle != _stream(slot):
+            turn.pass_on(torch.cuda.current_stream(slot.device))
+    return slot
+
+
+class _Turn:
+    """The stream that added to a parameter's gradient last.  The kernels add without atomics: another stream's pass waits for what that
+    one has been given.  (A captured pass does not wait for one outside, nor the other way round: a graph is ordered where it is replayed.)"""
+
+    def __init__(self):
+        self.handle, self.stream = -1, None
+
+    def pass_on(self, cur) -> None:
+        last = self.stream
+        if last is not None and _capturing(last) == _capturing(cur):
+            cur.wait_stream(last)
+        self.handle, self.stream = cur.cuda_stream, cur
+
+    def __reduce__(self):                                          # (a parameter that is saved or copied starts anew)
+        return _Turn, ()
+
+
+def _capturing(stream) -> bool:
+    with torch.cuda.stream(stream):
+        return torch.cuda.is_current_stream_capturing()
 
 
 # ----------------------------------------------------------------------------------------------------
