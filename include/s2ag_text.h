@@ -36,9 +36,8 @@ int s2ag_clip_grads(const s2ag_clip_tensor* t /*host*/, int tensors, float max_n
  * out[i] = round(scale * table[ids[i]]), rows of `dim` elements, contiguous.  An id outside [0, n_entries) reads as zeros. */
 int s2ag_emb_lookup(const void* ids, int ids_i32, const void* table, int bf16, long long n, int dim, long long n_entries,
                     float scale, void* out, void* stream);
-/* dtable[v] = round(scale * sum of dy[i] over the i with ids[i] == v, in an order that the ids
- * decide); rows without an id and the row
- * `padding_idx` (-1: none) are written as zeros.  accumulate: fp32 only, dtable[v] += ... and rows without an id are left as
+/* dtable[v] = round(scale * sum of dy[i] over the i with ids[i] == v, in an order that the ids decide); rows without an id and
+ * the row `padding_idx` (-1: none) are written as zeros.  accumulate: fp32 only, dtable[v] += ... and rows without an id are left as
  * they are.  `ldy`: row pitch of dy in elements.  ids outside [0, n_entries) send nothing.  n < 2^31 - 2^16, n_entries < 2^30. */
 long long s2ag_emb_grad_workspace_bytes(long long n, int dim, long long n_entries);
 int s2ag_emb_grad(const void* ids, int ids_i32, const void* dy, long long ldy, int bf16, long long n, int dim,
@@ -47,7 +46,10 @@ int s2ag_emb_grad(const void* ids, int ids_i32, const void* dy, long long ldy, i
 
 /* ---- linear cross entropy ----------------------------------------------------------------------------------------------------
  * z = x w^T (rows x vocab, never stored whole); loss_i = log(sum_v exp z_iv) - z_{i, target_i}, 0 for target_i == ignore_index.
- * A target outside [0, vocab) that is not ignore_index makes that row's loss NaN. */
+ * A target outside [0, vocab) that is not ignore_index makes that row's loss NaN.
+ * bf16: the gradient of z is rounded to bf16 before the products that make dx and dw.  Rows that are ignored get a gradient of zero
+ * whatever grad_out is, and so does dw where all are.
+ * The backward call takes the forward call's sizes, types, w, ldw and `state`; x and target have to be there and are not read again. */
 #define S2AG_LCE_MEAN 0 /* over the rows that are not ignored; 0 if there are none */
 #define S2AG_LCE_SUM 1
 #define S2AG_LCE_NONE 2

@@ -193,7 +193,8 @@ int blocks_of(unsigned chunks) { return chunks < 1 ? 1 : chunks < (unsigned)MAX_
 
 bool valid(const s2ag_clip_tensor* a, int tensors) {
     if (tensors < 0 || (tensors && !a)) return false;
-    for (int i = 0; i < tensors; ++i)                              // 2^43: the chunks of a launch's 128 tensors fit 32 bits
+    // 2^38 elements are 2^24 chunks of 2^14; a launch's 128 tensors have 2^31 at most, which an unsigned holds
+    for (int i = 0; i < tensors; ++i)
         if (a[i].n < 0 || a[i].n > (1LL << 38) || (a[i].n && !a[i].src)) return false;
     return true;
 }

@@ -20,7 +20,7 @@
 // for values below 2^-17 of it).  Six products of bf16 pieces took 32 us for the logits of 136 rows and 20 000 words of 300
 // values, these take 22.  For the gradient's products as three bf16 pieces (v = p0 + p1 + p2 to 2^-25) and the six products that
 // matter at fp32's own rounding: G has values of many magnitudes in a row, which bf16's range holds and a half's does not.
-// bf16 operands need one product; there G is rounded to bf16 (2^-9 of each value; sums stay in fp32), without its factor g where
+// bf16 operands need one product; there G is rounded to bf16 (2^-8 of each value at most; sums stay in fp32), without its factor g where
 // that is one number for all rows.
 //
 // Measured, 7373 of 8192 rows counting, 131072 words of 2048 values, bf16: max and sum 3.0 ms (1320 TFLOP/s), G 3.3 (1190), dX 3.1
@@ -872,7 +872,7 @@ __global__ __launch_bounds__(64 * WR * WQ, BR == 256 ? 1 : 2) void product_k(Pro
                         }
 #pragma unroll
                         for (int i = 0; i < QI * 4; ++i) g[j][i] *= fac[jj + j];
-                        if (t.r0 + BR > live) {                  // rows behind are zeros, which dW's products pass by (0 times a word's infinity is none)
+                        if (t.r0 + BR > live) {                  // rows behind are zeros for dW's product, whatever a word holds (0 times an infinity is none)
                             const bool in = wr0 + (jj + j) * 16 + fl < live;
 #pragma unroll
                             for (int i = 0; i < QI * 4; ++i) g[j][i] = in ? g[j][i] : 0.f;
@@ -920,7 +920,6 @@ __global__ __launch_bounds__(64 * WR * WQ, BR == 256 ? 1 : 2) void product_k(Pro
 }
 
 // ---- joins -------------------------------------------------------------------------------------------------------------------
-// A lane per row, sixteen wavefronts over the tiles.
 // 16 rows to a workgroup, 64 lanes to a row: a few loads in turn for any vocabulary (391 tiles: 7 us; 64 rows to a workgroup,
 // 16 lanes to a row, took 14)
 struct MaxSum {
